@@ -20,7 +20,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join("sheeprl_prey_amd", "ops", "csrc")
 ARCH = os.environ.get("SRL_OFFLOAD_ARCH", "gfx950")
 HIPCC_FLAGS = ["-O3", f"--offload-arch={ARCH}", "-std=c++17", "-fPIC", "-ffp-contract=fast-honor-pragmas", "-munsafe-fp-atomics",
-               "-Wno-unused-result"]
+               "-Wno-unused-result",
+               # packed fp32 arithmetic (v_pk_*_f32) has given wrong results now and then: scalar forms only
+               "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 ext_modules = []
 cmdclass = {}
