@@ -1057,3 +1057,8 @@ def gru_step(rnn: torch.nn.GRU, x: Tensor, h: Tensor):
     gh = torch.nn.functional.linear(h2, rnn.weight_hh_l0, rnn.bias_hh_l0).contiguous()
     hn = _GRUCellAct.apply(gi, gh, h2.contiguous()).view(1, -1, rnn.hidden_size)
     return hn, hn
+
+
+# =============================================================== gated delta rule, gated residual norms
+from sheeprl_prey_amd.ops.delta import gated_delta, gated_delta_step  # noqa: E402,F401
+from sheeprl_prey_amd.ops.residual_norm import gated_residual_norm  # noqa: E402,F401

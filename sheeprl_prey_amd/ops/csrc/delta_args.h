@@ -1,0 +1,59 @@
+// Arguments and launchers of the gated delta rule (host side; the kernels: delta.h).
+#pragma once
+#include <hip/hip_runtime_api.h>
+#include <stdint.h>
+
+namespace srl {
+namespace delta {
+
+constexpr int MAXD = 128;        // head dimensions
+constexpr float GONE = -104.0f;  // exp(g) rounds to zero in fp32 below this: the step forgets all that was before it
+
+struct Args {
+  const void *q, *k, *v;
+  const float *g, *beta;
+  const uint8_t* first;   // [T, B] or null
+  const int* lengths;     // [B] or null
+  const float* state;     // [B, Hv, Dk, Dv] contiguous, or null (zeros)
+  long qt, qb, qh, kt, kb, kh, vt, vb, vh, gt, gb, gh, bt, bb, bh_, ft, fb;  // element strides of t, b, head
+  int T, B, Hk, Hv, Dk, Dv;
+  int normalize, vecq, veck;
+  float scale, eps;
+  // plan: N chunks of C steps, in nseg segments of cps chunks
+  int N, nseg, cps;
+};
+
+struct FwdOut {
+  void* out;        // [T, B, Hv, Dv] contiguous
+  float* last;      // [B, Hv, Dk, Dv]
+  float* Sc;        // [BH, N, DKp, Dvp] each chunk's first state, or null
+  float* U;         // [BH, N, C, Dvp], or null
+  float* Sseg;      // [BH, nseg, DKp, Dvp] each segment's first state (nseg > 1)
+  float* Rseg;      // [BH, nseg, DKp, Dvp] a segment's last state from a zero first state
+  float* Pseg;      // [BH, nseg, DKp, DKp] the map from a segment's first to its last state
+};
+
+struct BwdArgs {
+  const void* dout;  // [T, B, Hv, Dv] by strides, or null
+  long ot, ob, oh;
+  const float* dlast;  // [B, Hv, Dk, Dv] contiguous, or null
+  const float *Sc, *U, *Pseg;
+  float* dSc;   // [BH, N, DKp, Dvp] gradient of each chunk's last state
+  float* dR;    // [BH, N, C, Dvp]
+  float* Xseg;  // [BH, nseg, DKp, Dvp]
+  float* dSseg; // [BH, nseg, DKp, Dvp]
+  void *dq, *dk;  // [T, B, H?, Dk] contiguous: per key head in the input's type (Hv == Hk), else per value head in fp32
+  void* dv;
+  float *dg, *db, *dstate;
+};
+
+void launch_delta_fwd(const Args& a, const FwdOut& o, int C, bool is_bf16, hipStream_t st);
+void launch_delta_bwd(const Args& a, const BwdArgs& o, int C, bool is_bf16, bool per_value_head, hipStream_t st);
+void launch_delta_scan_rev(const float* dlast, const float* P, const float* X, float* dS, int BH, int nseg, int Dk, int Dv,
+                           hipStream_t st);
+void launch_delta_head_sum(const float* x, void* y, long rows, int rep, int Dk, bool is_bf16, hipStream_t st);
+// delta_step.hip: the recurrent form; S2 (the state after it) may be a.state itself
+void launch_delta_steps(const Args& a, void* out, float* S2, long sb, long sh, bool is_bf16, hipStream_t st);
+
+}  // namespace delta
+}  // namespace srl

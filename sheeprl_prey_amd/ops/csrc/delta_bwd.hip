@@ -1,0 +1,530 @@
+// The gated delta rule, chunked form, backward (the mathematics and the layout: delta.h).
+//
+// With dS the gradient of a chunk's last state, dO that of its outputs, and T = (I + A)^-1:
+//   dU = P^T dO + diag(e) K dS,   dR = T^T dU,   dV = diag(beta) dR,
+//   dS0 = gam_C dS + scale Q^T diag(gam) dO - K^T diag(beta gam) dR:
+// again nothing mixes the value columns, so delta_bwd_state_kernel walks the chunks backwards with one wave a strip of 16
+// of them, dS in registers, split into segments over a long axis as the forward walk is (the map of dS over a segment
+// is the transpose of Pseg).  What sums over the value columns is left to delta_bwd_pair_kernel, one workgroup a chunk
+// and no order among them:
+//   W1 = M o tril(dO U^T),  W2 = -diag(beta) M o tril(dR U^T, -1),  GO = dO S0^T, GR = dR S0^T, GU = U dS^T,
+//   dQ = scale (diag(gam) GO + W1 K),
+//   dK = -diag(beta gam) GR + diag(e) GU + scale W1^T Q + (W2 + W2^T) K,
+//   dbeta_i = dR_i . v_i - gam_i k_i . GR_i + sum_j (W2 / beta o K K^T)_ij,
+//   dG_i = scale gam_i q_i . GO_i - beta_i gam_i k_i . GR_i + (row_i - column_i)(scale W1 o Q K^T + W2 o K K^T) - F_i,
+// F_i = e_i k_i . GU_i, dG of the chunk's last step takes sum F + gam_C <S0, dS> too, and the gradient of g_i is the
+// sum of dG over the steps from i to the end of its segment.
+#include "delta.h"
+
+namespace srl {
+namespace delta {
+
+template <typename T, int DKT, int C, bool MAP>
+__global__ void __launch_bounds__(512) delta_bwd_state_kernel(Args a, BwdArgs o) {
+  constexpr int LD = 16 * DKT + 4, LC = C + 4, NT = C / 16, DKp = 16 * DKT;
+  extern __shared__ __align__(16) unsigned char lds[];
+  Gates<C>& s = *reinterpret_cast<Gates<C>*>(lds);
+  float* K = reinterpret_cast<float*>(lds + sizeof(Gates<C>));
+  float* Q = K + C * LD;
+  float* A = Q + C * LD;
+  float* P = A + C * LC;
+  float* Td = P + C * LC;
+
+  const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  const int BH = a.B * a.Hv, bh = blockIdx.x % BH, seg = blockIdx.x / BH;
+  const int b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
+  const int Dvp = 16 * ((a.Dv + 15) >> 4), dv = 16 * wave + l16;
+  const int len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
+  const T* qp = reinterpret_cast<const T*>(a.q) + (long)b * a.qb + (long)hk * a.qh;
+  const T* kp = reinterpret_cast<const T*>(a.k) + (long)b * a.kb + (long)hk * a.kh;
+  const T* gp = o.dout ? reinterpret_cast<const T*>(o.dout) + (long)b * o.ob + (long)h * o.oh : nullptr;
+
+  f4 S[DKT];  // the gradient of the state
+#pragma unroll
+  for (int m = 0; m < DKT; ++m)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int d = 16 * m + 4 * kq + r;
+      if (MAP) S[m][r] = 0.f;
+      else if (a.nseg > 1) S[m][r] = o.dSseg[(((long)bh * a.nseg + seg) * DKp + d) * Dvp + dv];
+      else S[m][r] = (o.dlast && d < a.Dk && dv < a.Dv) ? o.dlast[((long)bh * a.Dk + d) * a.Dv + dv] : 0.f;
+    }
+
+  for (int n = min(a.N, (seg + 1) * a.cps) - 1; n >= seg * a.cps; --n) {
+    const int t0 = n * C;
+    if (t0 >= len) {
+      if (!MAP && dv < a.Dv) {
+        T* p = reinterpret_cast<T*>(o.dv) + (long)bh * a.Dv + dv;
+        for (int i = kq; i < C && t0 + i < a.T; i += 4) st1(p + (long)(t0 + i) * BH * a.Dv, 0.f);
+      }
+      continue;
+    }
+    if (!MAP) {
+      float* p = o.dSc + ((long)bh * a.N + n) * DKp * Dvp + dv;
+#pragma unroll
+      for (int m = 0; m < DKT; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) p[(16 * m + 4 * kq + r) * Dvp] = S[m][r];
+    }
+    __syncthreads();
+    load_rows<T, DKT, C>(K, s.rk, kp, a.kt, a.Dk, t0, len, a.veck, a.normalize, a.eps);
+    load_rows<T, DKT, C>(Q, s.rq, qp, a.qt, a.Dk, t0, len, a.vecq, a.normalize, a.eps);
+    if (wave == 0) chunk_gates<C>(a, s, b, h, t0, len, lane);
+    f4 dy[NT];
+#pragma unroll
+    for (int ti = 0; ti < NT; ++ti)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int t = t0 + 16 * ti + 4 * kq + r;
+        dy[ti][r] = (gp && t < len && dv < a.Dv) ? ld1(gp + (long)t * o.ot + dv) : 0.f;
+      }
+    __syncthreads();
+    pair_tiles<DKT, C>(K, Q, A, P, s, a.scale, wave, nw);
+    f4 u[NT];
+#pragma unroll
+    for (int ti = 0; ti < NT; ++ti) u[ti] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int m = 0; m < DKT; ++m) {
+      f4 x[NT];
+#pragma unroll
+      for (int ti = 0; ti < NT; ++ti) x[ti] = row4(K + (16 * ti + l16) * LD + 16 * m + 4 * kq);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int ti = 0; ti < NT; ++ti) u[ti] = mfma4(x[ti][j], S[m][j], u[ti]);
+    }
+    __syncthreads();
+    if (wave == 0) diag_inverse<C>(A, Td);
+    __syncthreads();
+    // dR: backward substitution by blocks of 16 steps
+#pragma unroll
+    for (int ti = NT - 1; ti >= 0; --ti) {
+      f4 r = u[ti] * row4(s.e + 16 * ti + 4 * kq);
+#pragma unroll
+      for (int tr = ti; tr < NT; ++tr) r = mm16(col4(P + (16 * tr + 4 * kq) * LC + 16 * ti + l16, LC), dy[tr], r);
+#pragma unroll
+      for (int tr = ti + 1; tr < NT; ++tr) r = mm16(-col4(A + (16 * tr + 4 * kq) * LC + 16 * ti + l16, LC), u[tr], r);
+      u[ti] = mm16(col4(Td + (16 * ti + 4 * kq) * LT + l16, LT), r, f4{0.f, 0.f, 0.f, 0.f});
+    }
+    if (!MAP) {
+      float* p = o.dR + ((long)bh * a.N + n) * C * Dvp + dv;
+      T* vp = reinterpret_cast<T*>(o.dv) + (long)bh * a.Dv + dv;
+#pragma unroll
+      for (int ti = 0; ti < NT; ++ti) {
+        const f4 g = u[ti] * row4(s.beta + 16 * ti + 4 * kq);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int i = 16 * ti + 4 * kq + r;
+          p[i * Dvp] = u[ti][r];
+          if (t0 + i < a.T && dv < a.Dv) st1(vp + (long)(t0 + i) * BH * a.Dv, t0 + i < len ? g[r] : 0.f);
+        }
+      }
+    }
+    const float gc = s.gam[C - 1];
+#pragma unroll
+    for (int m = 0; m < DKT; ++m) S[m] *= gc;
+#pragma unroll
+    for (int ti = 0; ti < NT; ++ti) {
+      const f4 ga = row4(s.gam + 16 * ti + 4 * kq);
+      const f4 w = dy[ti] * (a.scale * ga), z = -(u[ti] * ga * row4(s.beta + 16 * ti + 4 * kq));
+      f4 x[DKT], y[DKT];
+#pragma unroll
+      for (int m = 0; m < DKT; ++m) {
+        x[m] = col4(Q + (16 * ti + 4 * kq) * LD + 16 * m + l16, LD);
+        y[m] = col4(K + (16 * ti + 4 * kq) * LD + 16 * m + l16, LD);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int m = 0; m < DKT; ++m) S[m] = mfma4(x[m][j], w[j], S[m]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int m = 0; m < DKT; ++m) S[m] = mfma4(y[m][j], z[j], S[m]);
+    }
+  }
+  if (MAP) {
+    float* p = o.Xseg + ((long)bh * a.nseg + seg) * DKp * Dvp + dv;
+#pragma unroll
+    for (int m = 0; m < DKT; ++m)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) p[(16 * m + 4 * kq + r) * Dvp] = S[m][r];
+  } else if (seg == 0 && o.dstate && dv < a.Dv) {
+#pragma unroll
+    for (int m = 0; m < DKT; ++m)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int d = 16 * m + 4 * kq + r;
+        if (d < a.Dk) o.dstate[((long)bh * a.Dk + d) * a.Dv + dv] = S[m][r];
+      }
+  }
+}
+
+constexpr int DVB = 32;  // value columns staged at once
+
+template <int DKT, int C>
+struct PairLds {
+  static constexpr int LD = 16 * DKT + 4, LC = C + 4, LV = DVB + 4, NT = C / 16, NTL = NT * (NT + 1) / 2;
+  static constexpr int stage = 3 * C * LV, w = 2 * C * LC, big = stage > w ? stage : w;
+  float K[C * LD], Q[C * LD], big_[big];
+  Gates<C> s;
+  float rows[2 * NTL][16], cols[2 * NTL][16], rowb[NTL][16], dots[5][DKT][C], dRv[C], sd[DKT];
+};
+
+template <typename T, int DKT, int C>
+__global__ void __launch_bounds__(64 * DKT) delta_bwd_pair_kernel(Args a, BwdArgs o, int per_value_head) {
+  using L = PairLds<DKT, C>;
+  constexpr int LD = L::LD, LC = L::LC, LV = L::LV, NT = L::NT, NTL = L::NTL, DKp = 16 * DKT, NW = DKT;
+  constexpr int TPW = (2 * NTL + NW - 1) / NW, RPT = (C * (DVB / 4) + 64 * NW - 1) / (64 * NW);
+  extern __shared__ __align__(16) unsigned char lds[];
+  L& l = *reinterpret_cast<L*>(lds);
+  Gates<C>& s = l.s;
+  float *sO = l.big_, *sR = sO + C * LV, *sU = sR + C * LV, *W1 = l.big_, *W2 = W1 + C * LC;
+
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, kq = lane >> 4, wave = tid >> 6;
+  const int BH = a.B * a.Hv, bh = blockIdx.x % BH, n = blockIdx.x / BH, t0 = n * C;
+  const int b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
+  const int Dvp = 16 * ((a.Dv + 15) >> 4);
+  const int len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
+  const int Ho = per_value_head ? a.Hv : a.Hk, ho = per_value_head ? h : hk;
+  const bool same = per_value_head == 0;  // the outputs have the inputs' type
+
+  auto put = [&](void* base, int i, int d, float v) {
+    const long at = (((long)(t0 + i) * a.B + b) * Ho + ho) * a.Dk + d;
+    if (same) st1(reinterpret_cast<T*>(base) + at, v);
+    else reinterpret_cast<float*>(base)[at] = v;
+  };
+
+  if (t0 >= len) {
+    const int m = min(C, a.T - t0);
+    for (int x = tid; x < m * a.Dk; x += 64 * NW) {
+      put(o.dq, x / a.Dk, x % a.Dk, 0.f);
+      put(o.dk, x / a.Dk, x % a.Dk, 0.f);
+    }
+    if (tid < m) {
+      o.dg[(long)(t0 + tid) * BH + bh] = 0.f;
+      o.db[(long)(t0 + tid) * BH + bh] = 0.f;
+    }
+    return;
+  }
+
+  load_rows<T, DKT, C>(l.K, s.rk, reinterpret_cast<const T*>(a.k) + (long)b * a.kb + (long)hk * a.kh, a.kt, a.Dk, t0, len, a.veck,
+                       a.normalize, a.eps);
+  load_rows<T, DKT, C>(l.Q, s.rq, reinterpret_cast<const T*>(a.q) + (long)b * a.qb + (long)hk * a.qh, a.qt, a.Dk, t0, len, a.vecq,
+                       a.normalize, a.eps);
+  if (wave == 0) chunk_gates<C>(a, s, b, h, t0, len, lane);
+
+  const T* vp = reinterpret_cast<const T*>(a.v) + (long)b * a.vb + (long)h * a.vh;
+  const T* gp = o.dout ? reinterpret_cast<const T*>(o.dout) + (long)b * o.ob + (long)h * o.oh : nullptr;
+  const float* up = o.U + ((long)bh * a.N + n) * C * Dvp;
+  const float* rp = o.dR + ((long)bh * a.N + n) * C * Dvp;
+  const float* s0 = o.Sc + (((long)bh * a.N + n) * DKp + 16 * wave + l16) * Dvp;
+  const float* ds = o.dSc + (((long)bh * a.N + n) * DKp + 16 * wave + l16) * Dvp;
+
+  f4 GO[NT], GR[NT], GU[NT], D[TPW];
+  float dRv[RPT], sdot = 0.f;
+  const f4 zero = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int ti = 0; ti < NT; ++ti) GO[ti] = GR[ti] = GU[ti] = zero;
+#pragma unroll
+  for (int x = 0; x < TPW; ++x) D[x] = zero;
+#pragma unroll
+  for (int x = 0; x < RPT; ++x) dRv[x] = 0.f;
+
+  for (int c0 = 0; c0 < Dvp; c0 += DVB) {
+#pragma unroll
+    for (int x = 0; x < RPT; ++x) {
+      const int at = tid + x * 64 * NW, i = at / (DVB / 4), c = c0 + 4 * (at % (DVB / 4));
+      if (i < C) {
+        f4 g = zero, r = zero, u = zero;
+        if (c < Dvp) {
+          r = row4(rp + i * Dvp + c);
+          u = row4(up + i * Dvp + c);
+          const int t = t0 + i;
+          if (t < len) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (c + j < a.Dv) {
+                if (gp) g[j] = ld1(gp + (long)t * o.ot + c + j);
+                dRv[x] = fmaf(r[j], ld1(vp + (long)t * a.vt + c + j), dRv[x]);
+              }
+          }
+        }
+        const int w = i * LV + c - c0;
+        *reinterpret_cast<f4*>(sO + w) = g;
+        *reinterpret_cast<f4*>(sR + w) = r;
+        *reinterpret_cast<f4*>(sU + w) = u;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < DVB / 16; ++m) {
+      const int c = c0 + 16 * m;
+      if (c < Dvp) {
+        const f4 x = row4(s0 + c + 4 * kq), y = row4(ds + c + 4 * kq);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sdot = fmaf(x[j], y[j], sdot);
+#pragma unroll
+        for (int ti = 0; ti < NT; ++ti) {
+          const int w = (16 * ti + l16) * LV + 16 * m + 4 * kq;
+          GO[ti] = mm16(x, row4(sO + w), GO[ti]);
+          GR[ti] = mm16(x, row4(sR + w), GR[ti]);
+          GU[ti] = mm16(y, row4(sU + w), GU[ti]);
+        }
+#pragma unroll
+        for (int x2 = 0; x2 < TPW; ++x2) {
+          const int task = wave + x2 * NW;
+          if (task < 2 * NTL) {
+            int ti, tj;
+            lower_tile(task < NTL ? task : task - NTL, ti, tj);
+            D[x2] = mm16(row4(sU + (16 * tj + l16) * LV + 16 * m + 4 * kq),
+                         row4((task < NTL ? sO : sR) + (16 * ti + l16) * LV + 16 * m + 4 * kq), D[x2]);
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int x = 0; x < RPT; ++x) {
+    const int i = (tid + x * 64 * NW) / (DVB / 4);
+    const float v = seg_sum(dRv[x], DVB / 4);
+    if (i < C && (tid & (DVB / 4 - 1)) == 0) l.dRv[i] = v;
+  }
+  sdot = wave_sum(sdot);
+  if (lane == 0) l.sd[wave] = sdot;
+
+  // W1, W2 (over the staging area) and the row and column sums of what the decays see of them
+#pragma unroll
+  for (int x2 = 0; x2 < TPW; ++x2) {
+    const int task = wave + x2 * NW;
+    if (task < 2 * NTL) {
+      const bool first = task < NTL;
+      int ti, tj;
+      lower_tile(first ? task : task - NTL, ti, tj);
+      const float* kj = l.K + (16 * tj + l16) * LD + 4 * kq;
+      const float* xi = (first ? l.Q : l.K) + (16 * ti + l16) * LD + 4 * kq;
+      f4 d = zero;
+#pragma unroll
+      for (int m = 0; m < DKT; ++m) d = mm16(row4(kj + 16 * m), row4(xi + 16 * m), d);
+      const int i = 16 * ti + l16, j0 = 16 * tj + 4 * kq;
+      const double Gi = s.G[i];
+      const int segi = s.seg[i];
+      const float be = s.beta[i];
+      f4 w;
+      float rs = 0.f, rb = 0.f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float m = pair_decay<C>(s, i, j0 + r, Gi, segi);
+        float e;
+        if (first) {
+          w[r] = m * D[x2][r];
+          e = a.scale * w[r] * d[r];
+        } else {
+          const float z = j0 + r < i ? -m * D[x2][r] : 0.f;
+          w[r] = be * z;
+          rb = fmaf(z, d[r], rb);
+          e = w[r] * d[r];
+        }
+        rs += e;
+        const float cs = row16_sum(e);
+        if (l16 == 0) l.cols[task][4 * kq + r] = cs;
+      }
+      *reinterpret_cast<f4*>((first ? W1 : W2) + i * LC + j0) = w;
+      rs += __shfl_xor(rs, 16, 64);
+      rs += __shfl_xor(rs, 32, 64);
+      rb += __shfl_xor(rb, 16, 64);
+      rb += __shfl_xor(rb, 32, 64);
+      if (kq == 0) {
+        l.rows[task][l16] = rs;
+        if (!first) l.rowb[task - NTL][l16] = rb;
+      }
+    }
+  }
+  __syncthreads();
+
+  // this wave's 16 key columns of dQ^T and dK^T
+  f4 dQ[NT], dK[NT];
+  const int kc = 16 * wave;
+#pragma unroll
+  for (int ti = 0; ti < NT; ++ti) {
+    const int i = 16 * ti + l16;
+    const float ga = s.gam[i], be = s.beta[i], e = s.e[i];
+    const f4 q = row4(l.Q + i * LD + kc + 4 * kq), k = row4(l.K + i * LD + kc + 4 * kq);
+    float d0 = 0.f, d1 = 0.f, d2 = 0.f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      d0 = fmaf(q[r], GO[ti][r], d0);
+      d1 = fmaf(k[r], GR[ti][r], d1);
+      d2 = fmaf(k[r], GU[ti][r], d2);
+    }
+    dQ[ti] = ga * GO[ti];
+    f4 w = zero;
+#pragma unroll
+    for (int tj = 0; tj <= ti; ++tj) {
+      const f4 x = col4(l.K + (16 * tj + 4 * kq) * LD + kc + l16, LD);
+      dQ[ti] = mm16(x, row4(W1 + i * LC + 16 * tj + 4 * kq), dQ[ti]);
+      w = mm16(x, row4(W2 + i * LC + 16 * tj + 4 * kq), w);
+    }
+    f4 z = zero;
+#pragma unroll
+    for (int tr = ti; tr < NT; ++tr) {
+      z = mm16(col4(l.Q + (16 * tr + 4 * kq) * LD + kc + l16, LD), col4(W1 + (16 * tr + 4 * kq) * LC + i, LC), z);
+      w = mm16(col4(l.K + (16 * tr + 4 * kq) * LD + kc + l16, LD), col4(W2 + (16 * tr + 4 * kq) * LC + i, LC), w);
+    }
+    dQ[ti] *= a.scale;
+    dK[ti] = w + a.scale * z - (be * ga) * GR[ti] + e * GU[ti];
+    float d3 = 0.f, d4 = 0.f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      d3 = fmaf(q[r], dQ[ti][r], d3);
+      d4 = fmaf(k[r], dK[ti][r], d4);
+    }
+    float dd[5] = {d0, d1, d2, d3, d4};
+#pragma unroll
+    for (int x = 0; x < 5; ++x) {
+      dd[x] += __shfl_xor(dd[x], 16, 64);
+      dd[x] += __shfl_xor(dd[x], 32, 64);
+      if (kq == 0) l.dots[x][wave][i] = dd[x];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int ti = 0; ti < NT; ++ti) {
+    const int i = 16 * ti + l16;
+    float dq = 0.f, dk = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      dq += l.dots[3][w][i];
+      dk += l.dots[4][w][i];
+    }
+    const f4 q = row4(l.Q + i * LD + kc + 4 * kq), k = row4(l.K + i * LD + kc + 4 * kq);
+    if (a.normalize) {
+      dQ[ti] = s.rq[i] * (dQ[ti] - dq * q);
+      dK[ti] = s.rk[i] * (dK[ti] - dk * k);
+    }
+    if (t0 + i < a.T) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int d = kc + 4 * kq + r;
+        if (d < a.Dk) {
+          put(o.dq, i, d, t0 + i < len ? dQ[ti][r] : 0.f);
+          put(o.dk, i, d, t0 + i < len ? dK[ti][r] : 0.f);
+        }
+      }
+    }
+  }
+  if (wave == 0) {
+    const int i = lane;
+    double dG = 0.0;
+    float F = 0.f, db = 0.f;
+    if (i < C) {
+      float go = 0.f, gr = 0.f, gu = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        go += l.dots[0][w][i];
+        gr += l.dots[1][w][i];
+        gu += l.dots[2][w][i];
+      }
+      const float ga = s.gam[i], be = s.beta[i];
+      F = s.e[i] * gu;
+      db = l.dRv[i] - ga * gr;
+      dG = (double)(a.scale * ga * go) - (double)(be * ga * gr) - (double)F;
+#pragma unroll
+      for (int task = 0; task < 2 * NTL; ++task) {
+        int ti, tj;
+        lower_tile(task < NTL ? task : task - NTL, ti, tj);
+        if (ti == i >> 4) {
+          dG += (double)l.rows[task][i & 15];
+          if (task >= NTL) db += l.rowb[task - NTL][i & 15];
+        }
+        if (tj == i >> 4) dG -= (double)l.cols[task][i & 15];
+      }
+    }
+    float sumF = wave_sum(F);
+    if (i == C - 1) {
+      float sd = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) sd += l.sd[w];
+      dG += (double)(sumF + s.gam[C - 1] * sd);
+    }
+    // sums over the steps from i to the end of the segment: suffix sums, less that of the next segment's first step
+    double suf = dG;
+#pragma unroll
+    for (int x = 1; x < C; x <<= 1) {
+      const double y = __shfl_down(suf, x, 64);
+      if (i + x < C) suf += y;
+    }
+    const unsigned long long starts = __ballot(i < C && i > 0 && s.seg[i < C ? i : 0] != s.seg[i > 0 && i < C ? i - 1 : 0]);
+    const unsigned long long later = i < 63 ? starts >> (i + 1) : 0ull;
+    const int nx = later ? i + __ffsll((long long)later) : i;
+    const double beyond = __shfl(suf, nx, 64);
+    const double g = suf - (later ? beyond : 0.0);
+    if (i < C && t0 + i < a.T) {
+      o.dg[(long)(t0 + i) * BH + bh] = s.rst[i] ? 0.f : (float)g;
+      o.db[(long)(t0 + i) * BH + bh] = t0 + i < len ? db : 0.f;
+    }
+  }
+}
+
+// Per-value-head dq, dk in fp32 -> the sum over the value heads that share a key head, rounded once.
+template <typename T>
+__global__ void delta_head_sum_kernel(const float* x, T* y, long n, int rep, int Dk) {
+  const long i = (long)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= n) return;
+  const long row = i / Dk, d = i % Dk;
+  float v = 0.f;
+  for (int r = 0; r < rep; ++r) v += x[(row * rep + r) * Dk + d];
+  st1(y + i, v);
+}
+
+template <typename T, int DKT, int C, bool MAP>
+static void launch_state(const Args& a, const BwdArgs& o, hipStream_t st) {
+  const size_t lds = strip_lds<DKT, C>(true);
+  auto* f = delta_bwd_state_kernel<T, DKT, C, MAP>;
+  (void)hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  f<<<a.B * a.Hv * a.nseg, 64 * ((a.Dv + 15) / 16), lds, st>>>(a, o);
+}
+
+template <typename T, int DKT, int C>
+static void launch_c(const Args& a, const BwdArgs& o, bool per_value_head, hipStream_t st) {
+  if constexpr (C == 64) {
+    if (a.nseg > 1) {
+      launch_state<T, DKT, C, true>(a, o, st);
+      launch_delta_scan_rev(o.dlast, o.Pseg, o.Xseg, o.dSseg, a.B * a.Hv, a.nseg, a.Dk, a.Dv, st);
+    }
+  }
+  launch_state<T, DKT, C, false>(a, o, st);
+  auto* f = delta_bwd_pair_kernel<T, DKT, C>;
+  const int lds = (int)sizeof(PairLds<DKT, C>);
+  (void)hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  f<<<a.B * a.Hv * a.N, 64 * DKT, lds, st>>>(a, o, per_value_head ? 1 : 0);
+}
+
+template <typename T>
+static void launch_t(const Args& a, const BwdArgs& o, int C, bool pv, hipStream_t st) {
+  if (C == 16) {
+    if (a.Dk <= 32) launch_c<T, 2, 16>(a, o, pv, st);
+    else if (a.Dk <= 64) launch_c<T, 4, 16>(a, o, pv, st);
+    else launch_c<T, 8, 16>(a, o, pv, st);
+  } else {
+    if (a.Dk <= 32) launch_c<T, 2, 64>(a, o, pv, st);
+    else if (a.Dk <= 64) launch_c<T, 4, 64>(a, o, pv, st);
+    else launch_c<T, 8, 64>(a, o, pv, st);
+  }
+}
+
+void launch_delta_bwd(const Args& a, const BwdArgs& o, int C, bool is_bf16, bool per_value_head, hipStream_t st) {
+  if (is_bf16) launch_t<bf16>(a, o, C, per_value_head, st);
+  else launch_t<float>(a, o, C, per_value_head, st);
+}
+
+void launch_delta_head_sum(const float* x, void* y, long rows, int rep, int Dk, bool is_bf16, hipStream_t st) {
+  const long n = rows * Dk;
+  const dim3 g((unsigned)((n + 255) / 256));
+  if (is_bf16) delta_head_sum_kernel<bf16><<<g, 256, 0, st>>>(x, reinterpret_cast<bf16*>(y), n, rep, Dk);
+  else delta_head_sum_kernel<float><<<g, 256, 0, st>>>(x, reinterpret_cast<float*>(y), n, rep, Dk);
+}
+
+}  // namespace delta
+}  // namespace srl

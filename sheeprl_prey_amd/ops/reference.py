@@ -211,3 +211,53 @@ def truncnorm_log_prob(value: Tensor, loc: Tensor, scale: Tensor, lo: Tensor, hi
     _, _, _, Z = truncnorm_terms(loc, scale, lo, hi)
     z = (value - loc) / scale
     return _LOG_INV_SQRT_2PI - Z.log() - 0.5 * z * z - scale.log()
+
+
+def gated_delta(q: Tensor, k: Tensor, v: Tensor, decay: Tensor, beta: Tensor, state: Optional[Tensor], is_first: Optional[Tensor],
+                lengths: Optional[Tensor], scale: float, normalize: bool, eps: float) -> Tuple[Tensor, Tensor]:
+    """The gated delta rule step by step, in fp32 (fp64 for fp64 inputs): ``ops.gated_delta`` off the GPU."""
+    T, B, Hv, Dv = v.shape
+    Hk, Dk = q.shape[2:]
+    ct = torch.float64 if v.dtype == torch.float64 else torch.float32
+    qf, kf, vf, gf, bf = (t.to(ct) for t in (q, k, v, decay, beta))
+    if lengths is not None:  # what lies behind a sequence's end is not read
+        live = torch.arange(T, device=v.device)[:, None] < lengths[None]
+        wide, narrow = live[..., None, None], live[..., None]
+        qf, kf, vf = (torch.where(wide, t, 0.0) for t in (qf, kf, vf))
+        gf, bf = (torch.where(narrow, t, 0.0) for t in (gf, bf))
+        is_first = None if is_first is None else is_first.bool() & live
+    if normalize:
+        qf, kf = (t * torch.rsqrt((t * t).sum(-1, keepdim=True) + eps) for t in (qf, kf))
+    qf, kf = (t.repeat_interleave(Hv // Hk, 2) for t in (qf, kf))
+    S = torch.zeros(B, Hv, Dk, Dv, device=v.device, dtype=ct) if state is None else state
+    keep = gf.exp()[..., None, None]
+    out = []
+    for t in range(T):
+        S = keep[t] * S
+        if is_first is not None:
+            S = torch.where(is_first[t].bool()[:, None, None, None], 0.0, S)
+        u = bf[t][..., None] * (vf[t] - (kf[t].unsqueeze(-2) @ S).squeeze(-2))
+        S = S + kf[t].unsqueeze(-1) * u.unsqueeze(-2)
+        out.append(scale * (qf[t].unsqueeze(-2) @ S).squeeze(-2))
+    o = torch.stack(out).to(v.dtype) if out else torch.zeros_like(v)
+    return o, S if T or state is None else S.clone()
+
+
+def gated_residual_norm(x: Tensor, h: Tensor, gate: Optional[Tensor], scale, post_weight: Optional[Tensor], post_bias: Optional[Tensor],
+                        pre_weight: Optional[Tensor], pre_bias: Optional[Tensor], norm: str, act: str, eps: float) -> Tuple[Tensor, Tensor]:
+    """``ops.gated_residual_norm`` off the GPU, in fp32 (fp64 for fp64 inputs)."""
+    ct = torch.float64 if x.dtype == torch.float64 else torch.float32
+
+    def nrm(z, w, b):
+        if norm == "layer":
+            z = z - z.mean(-1, keepdim=True)
+        z = z * torch.rsqrt((z * z).mean(-1, keepdim=True) + eps)
+        z = z if w is None else z * w.to(ct)
+        return z if b is None else z + b.to(ct)
+
+    a = scale if not isinstance(scale, Tensor) else scale.to(ct)
+    if gate is not None:
+        g = gate.to(ct)
+        a = a * (F.silu(g) if act == "silu" else torch.sigmoid(g) if act == "sigmoid" else g)
+    y = x.to(ct) + a * nrm(h.to(ct), post_weight, post_bias)
+    return y.to(x.dtype), nrm(y, pre_weight, pre_bias).to(x.dtype)

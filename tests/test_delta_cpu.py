@@ -1,0 +1,175 @@
+"""The gated delta rule and the gated residual norms off the GPU: the definitions in 64 bits, differences, refusals."""
+import pytest
+import torch
+
+from sheeprl_prey_amd import ops
+
+
+def delta_oracle(q, k, v, decay, beta, state=None, is_first=None, lengths=None, scale=None, normalize=True, eps=1e-6):
+    """The rule sequence by sequence, head by head, step by step, in fp64; differentiable."""
+    T, B, Hv, Dv = v.shape
+    Hk, Dk = q.shape[2:]
+    scale = Dk**-0.5 if scale is None else scale
+    outs, lasts = [], []
+    for b in range(B):
+        n = T if lengths is None else max(0, min(T, int(lengths[b])))
+        for h in range(Hv):
+            S = torch.zeros(Dk, Dv, dtype=torch.float64) if state is None else state[b, h].double()
+            o = []
+            for t in range(n):
+                qt, kt, vt = q[t, b, h // (Hv // Hk)].double(), k[t, b, h // (Hv // Hk)].double(), v[t, b, h].double()
+                if normalize:
+                    qt, kt = qt / (qt @ qt + eps).sqrt(), kt / (kt @ kt + eps).sqrt()
+                if is_first is not None and bool(is_first[t, b]):
+                    S = torch.zeros_like(S)
+                else:
+                    S = decay[t, b, h].double().exp() * S
+                u = beta[t, b, h].double() * (vt - kt @ S)
+                S = S + torch.outer(kt, u)
+                o.append(scale * (qt @ S))
+            o += [torch.zeros(Dv, dtype=torch.float64)] * (T - n)
+            outs.append(torch.stack(o))
+            lasts.append(S)
+    return torch.stack(outs, 1).view(T, B, Hv, Dv), torch.stack(lasts).view(B, Hv, Dk, Dv)
+
+
+def norm_oracle(x, h, gate, scale, pw, pb, rw, rb, norm, act, eps):
+    def nrm(z, w, b):
+        m = z.mean(-1, keepdim=True) if norm == "layer" else 0.0
+        z = (z - m) / (((z - m) ** 2).mean(-1, keepdim=True) + eps).sqrt()
+        return (z if w is None else z * w.double()) + (0.0 if b is None else b.double())
+
+    a = 1.0 if scale is None else scale.double() if isinstance(scale, torch.Tensor) else scale
+    if gate is not None:
+        g = gate.double()
+        a = a * {"silu": g * torch.sigmoid(g), "sigmoid": torch.sigmoid(g), "none": g}[act]
+    y = x.double() + a * nrm(h.double(), pw, pb)
+    return y, nrm(y, rw, rb)
+
+
+def delta_inputs(T, B, Hk, Hv, Dk, Dv, dtype=torch.float32, seed=0, device="cpu"):
+    g = torch.Generator().manual_seed(seed)
+    n = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    d = dict(q=n(T, B, Hk, Dk).to(dtype), k=n(T, B, Hk, Dk).to(dtype), v=n(T, B, Hv, Dv).to(dtype),
+             decay=-torch.nn.functional.softplus(n(T, B, Hv) - 1), beta=torch.sigmoid(n(T, B, Hv)), state=n(B, Hv, Dk, Dv) * 0.5)
+    return {k: t.to(device) for k, t in d.items()}
+
+
+@pytest.mark.parametrize("T,B,Hk,Hv,Dk,Dv", [(1, 1, 1, 1, 1, 1), (7, 3, 2, 4, 5, 6), (20, 2, 1, 3, 16, 9)])
+def test_delta_reference_matches_oracle(T, B, Hk, Hv, Dk, Dv):
+    x = delta_inputs(T, B, Hk, Hv, Dk, Dv)
+    first = torch.rand(T, B) < 0.2
+    lengths = torch.randint(0, T + 1, (B,))
+    for kw in ({}, {"is_first": first}, {"lengths": lengths}, {"is_first": first, "lengths": lengths, "scale": 0.7, "normalize": False}):
+        args = dict(x) if kw.get("normalize", True) else {**x, "k": 0.3 * x["k"]}
+        out, last = ops.gated_delta(**args, **kw)
+        eo, el = delta_oracle(**args, **kw)
+        # fp32 along T steps of Dk-term sums: (T + Dk) roundings, terms at most 8 times the result
+        tol = (T + Dk) * 8 * 2.0**-24
+        torch.testing.assert_close(out.double(), eo, rtol=tol, atol=tol)
+        torch.testing.assert_close(last.double(), el, rtol=tol, atol=tol * 8)
+
+
+def test_delta_reference_gradients_by_differences():
+    x = {k: t.double().requires_grad_() for k, t in delta_inputs(6, 2, 1, 2, 3, 4).items()}
+    first = torch.tensor([[1, 0], [0, 0], [0, 1], [0, 0], [1, 0], [0, 0]], dtype=torch.bool)
+    lengths = torch.tensor([6, 4])
+    names = list(x)
+
+    def f(*t):
+        return ops.gated_delta(**dict(zip(names, t)), is_first=first, lengths=lengths)
+
+    assert torch.autograd.gradcheck(f, tuple(x.values()), atol=1e-6)
+
+
+def test_delta_step_is_one_step_and_updates_in_place():
+    x = delta_inputs(1, 3, 2, 4, 8, 6)
+    out, last = ops.gated_delta(**x)
+    store = torch.zeros(5, 3, 4, 8, 6)
+    store[2] = x["state"]
+    got = ops.gated_delta_step(*(x[n][0] for n in ("q", "k", "v", "decay", "beta")), store[2])
+    assert torch.equal(got, out[0]) and torch.equal(store[2], last)
+    assert torch.equal(store[0], torch.zeros_like(store[0]))
+
+
+def test_delta_no_steps_and_no_sequences():
+    x = delta_inputs(0, 2, 1, 1, 4, 4)
+    out, last = ops.gated_delta(**x)
+    assert out.shape == (0, 2, 1, 4) and torch.equal(last, x["state"]) and last is not x["state"]
+    x = delta_inputs(3, 0, 1, 1, 4, 4)
+    out, last = ops.gated_delta(**x)
+    assert out.shape == (3, 0, 1, 4) and last.shape == (0, 1, 4, 4)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(k=torch.zeros(4, 2, 1, 7)), "one shape"),
+    (dict(v=torch.zeros(4, 2, 3, 8)), "multiple of the key heads"),
+    (dict(q=torch.zeros(4, 2, 2, 129), k=torch.zeros(4, 2, 2, 129)), "1..128"),
+    (dict(v=torch.zeros(4, 2, 2, 8, dtype=torch.bfloat16)), "one type"),
+    (dict(decay=torch.zeros(4, 2)), "decay and beta"),
+    (dict(beta=torch.zeros(4, 2, 2, dtype=torch.int64)), "floating point"),
+    (dict(state=torch.zeros(2, 2, 8, 7)), "state must be"),
+    (dict(state=torch.zeros(2, 2, 8, 8, dtype=torch.bfloat16)), "state must be"),
+    (dict(is_first=torch.zeros(2, 4, dtype=torch.bool)), "is_first must be"),
+    (dict(lengths=torch.zeros(2)), "lengths must be"),
+    (dict(lengths=torch.zeros(3, dtype=torch.int32)), "lengths must be"),
+    (dict(q=torch.zeros(4, 2, 8)), "heads, dim"),
+])
+def test_delta_refusals(change, match):
+    x = delta_inputs(4, 2, 2, 2, 8, 8)
+    with pytest.raises(ValueError, match=match):
+        ops.gated_delta(**{**x, **change})
+
+
+def test_delta_other_types_refused():
+    x = delta_inputs(4, 2, 2, 2, 8, 8, torch.float16)
+    with pytest.raises(ValueError, match="float32 or bfloat16"):
+        ops.gated_delta(**x)
+
+
+def test_delta_step_refusals():
+    x = {k: t if k == "state" else t[0] for k, t in delta_inputs(1, 2, 1, 2, 8, 8).items()}
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ops.gated_delta_step(**{**x, "q": x["q"].clone().requires_grad_()})
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.gated_delta_step(**{**x, "state": x["state"].transpose(2, 3)})
+    with pytest.raises(ValueError, match="overlap"):
+        ops.gated_delta_step(**{**x, "state": x["state"][:1].expand(2, 2, 8, 8)})
+    with pytest.raises(ValueError, match="heads, dim"):
+        ops.gated_delta_step(**{**x, "q": x["q"][None]})
+
+
+@pytest.mark.parametrize("norm", ["layer", "rms"])
+@pytest.mark.parametrize("act", ["silu", "sigmoid", "none"])
+def test_norm_reference_matches_oracle_and_differences(norm, act):
+    g = torch.Generator().manual_seed(1)
+    n = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64).requires_grad_()  # noqa: E731
+    args = (n(2, 3, 5), n(2, 3, 5), n(2, 3, 5), n(5), n(5), n(5), n(5), n(5))
+    y, u = ops.gated_residual_norm(*args, norm=norm, act=act, eps=1e-3)
+    ey, eu = norm_oracle(*args, norm, act, 1e-3)
+    torch.testing.assert_close(y, ey)
+    torch.testing.assert_close(u, eu)
+    assert torch.autograd.gradcheck(lambda *t: ops.gated_residual_norm(*t, norm=norm, act=act, eps=1e-3), args, atol=1e-6)
+
+
+def test_norm_defaults_and_broadcast_gate():
+    x, h = torch.randn(4, 6), torch.randn(4, 6)
+    y, u = ops.gated_residual_norm(x, h)
+    torch.testing.assert_close(y, x + torch.nn.functional.layer_norm(h, (6,)))
+    torch.testing.assert_close(u, torch.nn.functional.layer_norm(y, (6,)))
+    gate = torch.randn(4, 1, requires_grad=True)
+    y, u = ops.gated_residual_norm(x, h, gate, 0.5)
+    y.sum().backward()
+    torch.testing.assert_close(y, x + 0.5 * torch.nn.functional.silu(gate) * torch.nn.functional.layer_norm(h, (6,)))
+    assert gate.grad.shape == (4, 1)
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(norm="batch"), "norm must be"), (dict(act="relu"), "act must be"), (dict(h=torch.zeros(4, 5)), "one shape"),
+    (dict(scale=torch.zeros(5)), "scale must be"), (dict(pre_bias=torch.zeros(4, 6)), "pre_bias must be"),
+    (dict(x=torch.zeros(1, 8193), h=torch.zeros(1, 8193)), "1..8192"), (dict(x=torch.zeros(4, 6).half()), "float32 or bfloat16"),
+    (dict(post_weight=torch.zeros(6, dtype=torch.int32)), "floating point"),
+])
+def test_norm_refusals(kw, match):
+    with pytest.raises(ValueError, match=match):
+        ops.gated_residual_norm(**{**dict(x=torch.zeros(4, 6), h=torch.zeros(4, 6)), **kw})
