@@ -22,12 +22,13 @@ namespace delta {
 typedef float f4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float bf2f(uint16_t h) { return __builtin_bit_cast(float, (uint32_t)h << 16); }
-// round to nearest, ties to even; NaN stays NaN
-__device__ __forceinline__ uint16_t f2bf(float f) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, f);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40);
-  return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+// round to nearest, ties to even (v_cvt_pk_bf16_f32)
+typedef float f2_ __attribute__((ext_vector_type(2)));
+typedef __bf16 b2_ __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t f2bf2(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_{lo, hi}), b2_));
 }
+__device__ __forceinline__ uint16_t f2bf(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }
 struct bf16 { uint16_t x; };
 __device__ __forceinline__ float ld1(const float* p) { return *p; }
 __device__ __forceinline__ float ld1(const bf16* p) { return bf2f(p->x); }

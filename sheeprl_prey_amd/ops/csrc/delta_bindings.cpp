@@ -219,15 +219,15 @@ const float* par(const OptT& t, const Tensor& x, const char* name) {
   return t->data_ptr<float>();
 }
 
-// rows [R, D] with unit last stride; clears `vec` if 4 elements at a time cannot be read
+// rows [R, D] with unit last stride; clears `vec` if 16 bytes at a time cannot be read
 void rows_of(const Tensor& t, const Tensor& x, const char* name, const void** p, long* stride, bool* vec) {
   on(t, x, name);
   TORCH_CHECK(t.scalar_type() == x.scalar_type() && t.sizes() == x.sizes() && (t.stride(1) == 1 || t.size(1) == 1), name,
               ": rows like x with unit last stride");
-  const int bytes = 4 * (int)t.element_size();
+  const int n = 16 / (int)t.element_size();
   *p = t.data_ptr();
   *stride = t.stride(0);
-  *vec = *vec && x.size(1) % 4 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % bytes == 0 && t.stride(0) % 4 == 0;
+  *vec = *vec && x.size(1) % n == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && t.stride(0) % n == 0;
 }
 
 srl::rnorm::Args norm_args(const Tensor& x, const Tensor& h, const OptT& gate, const OptT& scale, const OptT& pw, const OptT& pb,
@@ -274,7 +274,7 @@ std::vector<Tensor> residual_norm_bwd(Tensor x, Tensor h, OptT gate, OptT scale,
   auto dg = has(gate) ? torch::empty_like(dx) : torch::empty({0}, x.options());
   auto f = x.options().dtype(torch::kFloat32);
   auto sums = torch::empty({5, x.size(1)}, f);
-  auto part = torch::empty({srl::rnorm::residual_norm_groups(a.rows, a.D), 5, x.size(1)}, f);
+  auto part = torch::empty({srl::rnorm::residual_norm_groups(a.rows, a.D), 4, x.size(1)}, f);
   o.dx = dx.data_ptr(), o.dh = dh.data_ptr(), o.dgate = has(gate) ? dg.data_ptr() : nullptr, o.part = part.data_ptr<float>();
   srl::rnorm::launch_residual_norm_bwd(a, o, sums.data_ptr<float>(), x.scalar_type() == torch::kBFloat16, vec, cur());
   launched("residual_norm_bwd");

@@ -20,7 +20,7 @@ struct BwdArgs {
   const void *dy, *du;  // rows of D by strides; either may be null
   long dys, dus;
   void *dx, *dh, *dgate;  // [rows, D] contiguous; dgate null without a gate
-  float* part;            // [workgroups, 5, D]: scale, pw, pb, rw, rb
+  float* part;            // [workgroups, 4, D]: sums of g act norm(h), g act, du norm(y), du
 };
 
 constexpr int SIGMOID = 5;
