@@ -5,6 +5,8 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
 #include "delta_args.h"
 #include "residual_norm.h"
 
@@ -20,36 +22,89 @@ void launched(const char* name) {
 }
 bool has(const OptT& t) { return t.has_value() && t->defined(); }
 
-void on(const Tensor& t, const Tensor& like, const char* name) {
-  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, ": must be on ", like.device(), ", is on ", t.device());
+void on(const Tensor& t, const Tensor& like) {
+  TORCH_CHECK_VALUE(t.device() == like.device(), "every operand must be on ", like.device(), ", got ", t.device());
 }
 void shape(const Tensor& t, c10::IntArrayRef s, const char* name) {
-  TORCH_CHECK(t.sizes() == s, name, ": shape ", t.sizes(), ", expected ", s);
+  TORCH_CHECK_VALUE(t.sizes() == s, name, " must be ", s, ", got ", t.sizes());
+}
+bool two_types(const Tensor& t) { return t.scalar_type() == torch::kFloat32 || t.scalar_type() == torch::kBFloat16; }
+Tensor unit_last(const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+Tensor f32(const Tensor& t) { return t.scalar_type() == torch::kFloat32 ? t : t.to(torch::kFloat32); }
+bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
+OptT opt_of(const Tensor& t) { return t.defined() ? OptT(t) : OptT(); }
+Tensor val(const OptT& t) { return has(t) ? *t : Tensor(); }
+const float* fp(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
+
+// The gradients of an operator that is differentiable once: a second differentiation raises an error.
+void once(torch::autograd::variable_list& g, const char* name) {
+  if (!at::GradMode::is_enabled()) return;
+  torch::autograd::variable_list in;
+  std::vector<size_t> at;
+  for (size_t i = 0; i < g.size(); ++i)
+    if (g[i].defined()) {
+      in.push_back(g[i].detach().requires_grad_());
+      at.push_back(i);
+    }
+  auto err = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " is differentiable once", (int64_t)in.size());
+  auto out = (*err)(std::move(in));
+  for (size_t j = 0; j < at.size(); ++j) g[at[j]] = out[j];
 }
 
-// q, k, v [T, B, H, D] with unit last stride, decay, beta [T, B, Hv] fp32, first [T, B] bytes, lengths [B] int32
+// ------------------------------------------------------------------ gated delta rule
+// What every entry takes, checked: q, k [T, B, Hk, Dk], v [T, B, Hv, Dv] (a single step comes as T = 1) of one type,
+// decay, beta [T, B, Hv], state [B, Hv, Dk, Dv] fp32, first [T, B], lengths [B].
+void delta_check(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& decay, const Tensor& beta, const Tensor& state,
+                 int lead) {
+  const char* where = lead == 2 ? "[T, B, heads, dim]" : "[B, heads, dim]";
+  TORCH_CHECK_VALUE(q.dim() == lead + 2 && k.dim() == lead + 2 && v.dim() == lead + 2, "q, k, v must be ", where, ", got ", q.sizes(), ", ",
+                    k.sizes(), ", ", v.sizes());
+  TORCH_CHECK_VALUE(q.sizes() == k.sizes() && q.sizes().slice(0, lead) == v.sizes().slice(0, lead),
+                    "q and k must have one shape and v their leading sizes: ", q.sizes(), ", ", k.sizes(), ", ", v.sizes());
+  const int64_t Hk = q.size(lead), Dk = q.size(lead + 1), Hv = v.size(lead), Dv = v.size(lead + 1), B = v.size(lead - 1);
+  TORCH_CHECK_VALUE(Hk >= 1 && Hv >= Hk && Hv % Hk == 0, "the value heads (", Hv, ") must be a multiple of the key heads (", Hk, ")");
+  TORCH_CHECK_VALUE(Dk >= 1 && Dk <= srl::delta::MAXD && Dv >= 1 && Dv <= srl::delta::MAXD, "head dimensions must be 1..",
+                    srl::delta::MAXD, ", got ", Dk, " and ", Dv);
+  TORCH_CHECK_VALUE((lead == 1 || v.size(0) < (1 << 24)) && B * Hv < (1 << 20), "at most 2^24 steps and 2^20 states, got ", v.sizes());
+  TORCH_CHECK_VALUE(q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type(), "q, k, v must have one type, got ",
+                    q.scalar_type(), ", ", k.scalar_type(), ", ", v.scalar_type());
+  TORCH_CHECK_VALUE(two_types(v), "q, k, v must be float32 or bfloat16, got ", v.scalar_type());
+  shape(decay, v.sizes().slice(0, lead + 1), "decay and beta");
+  shape(beta, v.sizes().slice(0, lead + 1), "decay and beta");
+  TORCH_CHECK_VALUE(decay.is_floating_point() && beta.is_floating_point(), "decay and beta must be floating point");
+  for (auto* t : {&q, &k, &decay, &beta}) on(*t, v);
+  if (state.defined()) {
+    shape(state, {B, Hv, Dk, Dv}, "state");
+    TORCH_CHECK_VALUE(state.scalar_type() == torch::kFloat32, "state must be float32, got ", state.scalar_type());
+    on(state, v);
+  }
+}
+
+Tensor delta_first(const OptT& x, c10::IntArrayRef s, const Tensor& like) {
+  if (!has(x)) return Tensor();
+  Tensor f = x->dim() == (int64_t)s.size() + 1 && x->size(-1) == 1 ? x->squeeze(-1) : *x;
+  shape(f, s, "is_first");
+  on(f, like);
+  return f.scalar_type() == torch::kBool || f.scalar_type() == torch::kUInt8 ? f : f.ne(0);
+}
+
+Tensor delta_lengths(const OptT& x, int64_t B, const Tensor& like) {
+  if (!has(x)) return Tensor();
+  TORCH_CHECK_VALUE(x->dim() == 1 && x->size(0) == B && (x->scalar_type() == torch::kInt32 || x->scalar_type() == torch::kInt64),
+                    "lengths must be int32 or int64 [", B, "], got ", x->scalar_type(), " ", x->sizes());
+  on(*x, like);
+  return x->to(torch::kInt32).contiguous();
+}
+
+struct DeltaOpts {
+  double scale, eps;
+  bool normalize;
+};
+
+// operands as delta_check and the conversions above leave them, each with a unit last stride
 srl::delta::Args delta_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& decay, const Tensor& beta,
-                            const OptT& state, const OptT& first, const OptT& lengths, double scale, bool normalize, double eps) {
+                            const Tensor& first, const Tensor& lengths, const DeltaOpts& o) {
   using namespace srl::delta;
-  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "gated_delta: q, k, v [T, B, H, D]");
-  TORCH_CHECK(q.scalar_type() == torch::kFloat32 || q.scalar_type() == torch::kBFloat16, "gated_delta: fp32 or bf16");
-  const int64_t T = v.size(0), B = v.size(1), Hv = v.size(2), Dv = v.size(3), Hk = q.size(2), Dk = q.size(3);
-  TORCH_CHECK(T >= 1 && B >= 1 && Hk >= 1 && Hv >= Hk && Hv % Hk == 0, "gated_delta: T, B >= 1 and Hv a multiple of Hk");
-  TORCH_CHECK(Dk >= 1 && Dk <= MAXD && Dv >= 1 && Dv <= MAXD, "gated_delta: head dimensions 1..", MAXD);
-  TORCH_CHECK(T < (1 << 24) && B * Hv < (1 << 20), "gated_delta: too many steps or heads");
-  shape(q, {T, B, Hk, Dk}, "gated_delta q");
-  shape(k, {T, B, Hk, Dk}, "gated_delta k");
-  shape(decay, {T, B, Hv}, "gated_delta decay");
-  shape(beta, {T, B, Hv}, "gated_delta beta");
-  for (auto* t : {&q, &k, &v}) {
-    on(*t, q, "gated_delta q, k, v");
-    TORCH_CHECK(t->scalar_type() == q.scalar_type(), "gated_delta: q, k, v of one type");
-    TORCH_CHECK(t->stride(3) == 1 || t->size(3) == 1, "gated_delta: unit last stride");
-  }
-  for (auto* t : {&decay, &beta}) {
-    on(*t, q, "gated_delta decay, beta");
-    TORCH_CHECK(t->scalar_type() == torch::kFloat32, "gated_delta: decay, beta fp32");
-  }
   Args a{};
   a.q = q.data_ptr(), a.k = k.data_ptr(), a.v = v.data_ptr();
   a.g = decay.data_ptr<float>(), a.beta = beta.data_ptr<float>();
@@ -58,29 +113,15 @@ srl::delta::Args delta_args(const Tensor& q, const Tensor& k, const Tensor& v, c
   a.vt = v.stride(0), a.vb = v.stride(1), a.vh = v.stride(2);
   a.gt = decay.stride(0), a.gb = decay.stride(1), a.gh = decay.stride(2);
   a.bt = beta.stride(0), a.bb = beta.stride(1), a.bh_ = beta.stride(2);
-  if (has(first)) {
-    on(*first, q, "gated_delta is_first");
-    shape(*first, {T, B}, "gated_delta is_first");
-    TORCH_CHECK(first->element_size() == 1, "gated_delta: is_first bool or uint8");
-    a.first = reinterpret_cast<const uint8_t*>(first->data_ptr());
-    a.ft = first->stride(0), a.fb = first->stride(1);
+  if (first.defined()) {
+    a.first = reinterpret_cast<const uint8_t*>(first.data_ptr());
+    a.ft = first.stride(0), a.fb = first.stride(1);
   }
-  if (has(lengths)) {
-    on(*lengths, q, "gated_delta lengths");
-    shape(*lengths, {B}, "gated_delta lengths");
-    TORCH_CHECK(lengths->scalar_type() == torch::kInt32 && lengths->is_contiguous(), "gated_delta: lengths int32, contiguous");
-    a.lengths = lengths->data_ptr<int>();
-  }
-  if (has(state)) {
-    on(*state, q, "gated_delta state");
-    shape(*state, {B, Hv, Dk, Dv}, "gated_delta state");
-    TORCH_CHECK(state->scalar_type() == torch::kFloat32, "gated_delta: state fp32");
-    a.state = state->data_ptr<float>();
-  }
-  a.T = (int)T, a.B = (int)B, a.Hk = (int)Hk, a.Hv = (int)Hv, a.Dk = (int)Dk, a.Dv = (int)Dv;
-  a.normalize = normalize, a.scale = (float)scale, a.eps = (float)eps;
+  if (lengths.defined()) a.lengths = lengths.data_ptr<int>();
+  a.T = (int)v.size(0), a.B = (int)v.size(1), a.Hk = (int)q.size(2), a.Hv = (int)v.size(2), a.Dk = (int)q.size(3), a.Dv = (int)v.size(3);
+  a.normalize = o.normalize, a.scale = (float)o.scale, a.eps = (float)o.eps;
   // wide reads of a row: 16 lanes take a sixteenth of the padded width each
-  const int ne = Dk <= 32 ? 2 : Dk <= 64 ? 4 : 8, bytes = std::min<int>(16, ne * (int)q.element_size());
+  const int Dk = a.Dk, ne = Dk <= 32 ? 2 : Dk <= 64 ? 4 : 8, bytes = std::min<int>(16, ne * (int)q.element_size());
   auto wide = [&](const Tensor& t) {
     bool ok = Dk % ne == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % bytes == 0;
     for (int i = 0; i < 3; ++i) ok = ok && t.stride(i) * t.element_size() % bytes == 0;
@@ -107,186 +148,346 @@ int delta_plan(srl::delta::Args& a) {
   return C;
 }
 
-// -> {out, last, Sc, U, Pseg}; the last three (what the backward pass needs) are empty unless `save`
-std::vector<Tensor> gated_delta_fwd(Tensor q, Tensor k, Tensor v, Tensor decay, Tensor beta, OptT state, OptT first, OptT lengths,
-                                    double scale, bool normalize, double eps, bool save) {
-  auto a = delta_args(q, k, v, decay, beta, state, first, lengths, scale, normalize, eps);
-  if (a.state) TORCH_CHECK(state->is_contiguous(), "gated_delta: contiguous state");
+// One allocation for several fp32 workspaces, each on a 256-byte boundary
+struct Workspace {
+  int64_t n = 0;
+  int64_t add(int64_t count) {
+    const int64_t at = n;
+    n += (count + 63) / 64 * 64;
+    return at;
+  }
+  Tensor make(const Tensor& like) const { return torch::empty({n}, like.options().dtype(torch::kFloat32)); }
+};
+
+// What a forward pass leaves for the backward pass, in one workspace: Sc, U, Pseg
+struct DeltaSaved {
+  int64_t Sc, U, P, n;
+  DeltaSaved(const srl::delta::Args& a, int C) {
+    const int64_t BH = (int64_t)a.B * a.Hv, DKp = dkp(a.Dk), Dvp = (a.Dv + 15) / 16 * 16;
+    Workspace w;
+    Sc = w.add(BH * a.N * DKp * Dvp);
+    U = w.add(BH * a.N * C * Dvp);
+    P = w.add(a.nseg > 1 ? BH * a.nseg * DKp * DKp : 0);
+    n = w.n;
+  }
+};
+
+// -> {out, last} and, in `saved` if it is not null, what the backward pass needs
+std::pair<Tensor, Tensor> delta_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& decay, const Tensor& beta,
+                                        const Tensor& state, const Tensor& first, const Tensor& lengths, const DeltaOpts& opt,
+                                        Tensor* saved) {
+  auto a = delta_args(q, k, v, decay, beta, first, lengths, opt);
+  a.state = fp(state);
   const c10::DeviceGuard guard(q.device());
-  const int C = delta_plan(a), BH = a.B * a.Hv, DKp = dkp(a.Dk), Dvp = (a.Dv + 15) / 16 * 16;
-  auto f = decay.options();
+  const int C = delta_plan(a);
+  const int64_t BH = (int64_t)a.B * a.Hv, DKp = dkp(a.Dk), Dvp = (a.Dv + 15) / 16 * 16;
   auto out = torch::empty({a.T, a.B, a.Hv, a.Dv}, v.options());
-  auto last = torch::empty({a.B, a.Hv, a.Dk, a.Dv}, f);
-  Tensor Sc = torch::empty({0}, f), U = Sc, Ps = Sc, Ss, Rs;
+  auto last = torch::empty({a.B, a.Hv, a.Dk, a.Dv}, decay.options());
   srl::delta::FwdOut o{};
   o.out = out.data_ptr(), o.last = last.data_ptr<float>();
-  if (save) {
-    Sc = torch::empty({BH, a.N, DKp, Dvp}, f);
-    U = torch::empty({BH, a.N, C, Dvp}, f);
-    o.Sc = Sc.data_ptr<float>(), o.U = U.data_ptr<float>();
+  const DeltaSaved at(a, C);
+  if (saved) {
+    *saved = torch::empty({at.n}, decay.options());
+    float* p = saved->data_ptr<float>();
+    o.Sc = p + at.Sc, o.U = p + at.U, o.Pseg = p + at.P;
   }
+  Tensor ws;
   if (a.nseg > 1) {
-    Ss = torch::empty({BH, a.nseg, DKp, Dvp}, f);
-    Rs = torch::empty({BH, a.nseg, DKp, Dvp}, f);
-    Ps = torch::empty({BH, a.nseg, DKp, DKp}, f);
-    o.Sseg = Ss.data_ptr<float>(), o.Rseg = Rs.data_ptr<float>(), o.Pseg = Ps.data_ptr<float>();
+    Workspace w;
+    const int64_t s = w.add(BH * a.nseg * DKp * Dvp), r = w.add(BH * a.nseg * DKp * Dvp), m = saved ? 0 : w.add(BH * a.nseg * DKp * DKp);
+    ws = w.make(q);
+    float* p = ws.data_ptr<float>();
+    o.Sseg = p + s, o.Rseg = p + r;
+    if (!saved) o.Pseg = p + m;
   }
   srl::delta::launch_delta_fwd(a, o, C, q.scalar_type() == torch::kBFloat16, cur());
-  launched("gated_delta_fwd");
-  return {out, last, Sc, U, Ps};
+  launched("gated_delta");
+  return {out, last};
 }
 
-// -> {dq, dk, dv, ddecay, dbeta, dstate}
-std::vector<Tensor> gated_delta_bwd(Tensor q, Tensor k, Tensor v, Tensor decay, Tensor beta, OptT state, OptT first, OptT lengths,
-                                    double scale, bool normalize, double eps, Tensor Sc, Tensor U, Tensor Pseg, OptT dout,
-                                    OptT dlast) {
-  auto a = delta_args(q, k, v, decay, beta, state, first, lengths, scale, normalize, eps);
-  const c10::DeviceGuard guard(q.device());
-  const int C = delta_plan(a), BH = a.B * a.Hv, DKp = dkp(a.Dk), Dvp = (a.Dv + 15) / 16 * 16;
-  shape(Sc, {BH, a.N, DKp, Dvp}, "gated_delta_bwd states");
-  shape(U, {BH, a.N, C, Dvp}, "gated_delta_bwd updates");
-  auto f = decay.options();
-  srl::delta::BwdArgs o{};
-  if (has(dout)) {
-    on(*dout, q, "gated_delta_bwd dout");
-    shape(*dout, {a.T, a.B, a.Hv, a.Dv}, "gated_delta_bwd dout");
-    TORCH_CHECK(dout->scalar_type() == q.scalar_type() && (dout->stride(3) == 1 || a.Dv == 1), "gated_delta_bwd: dout's type, unit last stride");
-    o.dout = dout->data_ptr();
-    o.ot = dout->stride(0), o.ob = dout->stride(1), o.oh = dout->stride(2);
+struct GatedDeltaFn : public torch::autograd::Function<GatedDeltaFn> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, Tensor q, Tensor k, Tensor v, Tensor decay, Tensor beta,
+                                                OptT state, OptT first_, OptT lengths_, double scale, bool normalize, double eps,
+                                                bool want_state) {
+    Tensor saved;
+    const Tensor first = val(first_), lengths = val(lengths_);
+    auto r = delta_forward(q, k, v, decay, beta, val(state), first, lengths, DeltaOpts{scale, eps, normalize}, &saved);
+    ctx->save_for_backward({q, k, v, decay, beta, first, lengths, saved});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["normalize"] = normalize;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["want_state"] = want_state;
+    ctx->set_materialize_grads(false);
+    return {r.first, r.second};
   }
-  if (has(dlast)) {
-    on(*dlast, q, "gated_delta_bwd dlast");
-    shape(*dlast, {a.B, a.Hv, a.Dk, a.Dv}, "gated_delta_bwd dlast");
-    TORCH_CHECK(dlast->scalar_type() == torch::kFloat32 && dlast->is_contiguous(), "gated_delta_bwd: dlast fp32, contiguous");
-    o.dlast = dlast->data_ptr<float>();
-  }
-  auto dSc = torch::empty({BH, a.N, DKp, Dvp}, f), dR = torch::empty({BH, a.N, C, Dvp}, f);
-  Tensor X, dSs;
-  if (a.nseg > 1) {
-    shape(Pseg, {BH, a.nseg, DKp, DKp}, "gated_delta_bwd maps");
-    X = torch::empty({BH, a.nseg, DKp, Dvp}, f);
-    dSs = torch::empty({BH, a.nseg, DKp, Dvp}, f);
-    o.Pseg = Pseg.data_ptr<float>(), o.Xseg = X.data_ptr<float>(), o.dSseg = dSs.data_ptr<float>();
-  }
-  const bool shared = a.Hk != a.Hv, bf = q.scalar_type() == torch::kBFloat16;
-  auto dq = torch::empty({a.T, a.B, a.Hk, a.Dk}, q.options()), dk = torch::empty_like(dq);
-  auto dv = torch::empty({a.T, a.B, a.Hv, a.Dv}, q.options());
-  auto dg = torch::empty({a.T, a.B, a.Hv}, f), db = torch::empty({a.T, a.B, a.Hv}, f);
-  auto ds = torch::empty({a.B, a.Hv, a.Dk, a.Dv}, f);
-  Tensor dqh, dkh;
-  if (shared) {
-    dqh = torch::empty({a.T, a.B, a.Hv, a.Dk}, f);
-    dkh = torch::empty({a.T, a.B, a.Hv, a.Dk}, f);
-  }
-  o.Sc = Sc.data_ptr<float>(), o.U = U.data_ptr<float>();
-  o.dSc = dSc.data_ptr<float>(), o.dR = dR.data_ptr<float>();
-  o.dq = shared ? dqh.data_ptr() : dq.data_ptr();
-  o.dk = shared ? dkh.data_ptr() : dk.data_ptr();
-  o.dv = dv.data_ptr(), o.dg = dg.data_ptr<float>(), o.db = db.data_ptr<float>(), o.dstate = ds.data_ptr<float>();
-  srl::delta::launch_delta_bwd(a, o, C, bf, shared, cur());
-  if (shared) {
-    const long rows = (long)a.T * a.B * a.Hk;
-    srl::delta::launch_delta_head_sum(dqh.data_ptr<float>(), dq.data_ptr(), rows, a.Hv / a.Hk, a.Dk, bf, cur());
-    srl::delta::launch_delta_head_sum(dkh.data_ptr<float>(), dk.data_ptr(), rows, a.Hv / a.Hk, a.Dk, bf, cur());
-  }
-  launched("gated_delta_bwd");
-  return {dq, dk, dv, dg, db, ds};
-}
 
-// The recurrent form over all T steps: out [T, B, Hv, Dv]; the state after them goes to state_out (which may be state)
-Tensor gated_delta_steps(Tensor q, Tensor k, Tensor v, Tensor decay, Tensor beta, OptT state, OptT first, OptT lengths, double scale,
-                         bool normalize, double eps, Tensor state_out) {
-  auto a = delta_args(q, k, v, decay, beta, state, first, lengths, scale, normalize, eps);
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    torch::autograd::variable_list g(12);
+    Tensor dout = grads[0], dlast = grads[1];
+    if (!dout.defined() && !dlast.defined()) return g;
+    const auto s = ctx->get_saved_variables();
+    const Tensor &q = s[0], &k = s[1], &v = s[2], &decay = s[3], &beta = s[4];
+    auto a = delta_args(q, k, v, decay, beta, s[5], s[6],
+                        DeltaOpts{ctx->saved_data["scale"].toDouble(), ctx->saved_data["eps"].toDouble(), ctx->saved_data["normalize"].toBool()});
+    const c10::DeviceGuard guard(q.device());
+    const int C = delta_plan(a);
+    const int64_t BH = (int64_t)a.B * a.Hv, DKp = dkp(a.Dk), Dvp = (a.Dv + 15) / 16 * 16;
+    srl::delta::BwdArgs o{};
+    if (dout.defined()) {
+      dout = unit_last(dout);
+      o.dout = dout.data_ptr();
+      o.ot = dout.stride(0), o.ob = dout.stride(1), o.oh = dout.stride(2);
+    }
+    if (dlast.defined()) {
+      dlast = dlast.contiguous();
+      o.dlast = dlast.data_ptr<float>();
+    }
+    const DeltaSaved at(a, C);
+    TORCH_CHECK(s[7].numel() == at.n, "gated_delta: the plan changed between the passes");
+    const float* sp = s[7].data_ptr<float>();
+    o.Sc = sp + at.Sc, o.U = sp + at.U, o.Pseg = sp + at.P;
+    const bool shared = a.Hk != a.Hv, bf = q.scalar_type() == torch::kBFloat16;
+    Workspace w;
+    const int64_t segs = a.nseg > 1 ? BH * a.nseg * DKp * Dvp : 0, heads = shared ? (int64_t)a.T * BH * a.Dk : 0;
+    const int64_t ds = w.add(BH * a.N * DKp * Dvp), dr = w.add(BH * a.N * C * Dvp), x = w.add(segs), dss = w.add(segs), hq = w.add(heads),
+                  hk = w.add(heads);
+    const Tensor ws = w.make(q);
+    float* p = ws.data_ptr<float>();
+    o.dSc = p + ds, o.dR = p + dr, o.Xseg = p + x, o.dSseg = p + dss;
+    auto dq = torch::empty({a.T, a.B, a.Hk, a.Dk}, q.options()), dk = torch::empty({a.T, a.B, a.Hk, a.Dk}, q.options());
+    auto dv = torch::empty({a.T, a.B, a.Hv, a.Dv}, q.options());
+    auto dg = torch::empty({a.T, a.B, a.Hv}, decay.options()), db = torch::empty({a.T, a.B, a.Hv}, decay.options());
+    o.dq = shared ? (void*)(p + hq) : dq.data_ptr();
+    o.dk = shared ? (void*)(p + hk) : dk.data_ptr();
+    o.dv = dv.data_ptr(), o.dg = dg.data_ptr<float>(), o.db = db.data_ptr<float>();
+    if (ctx->saved_data["want_state"].toBool()) {
+      g[5] = torch::empty({a.B, a.Hv, a.Dk, a.Dv}, decay.options());
+      o.dstate = g[5].data_ptr<float>();
+    }
+    srl::delta::launch_delta_bwd(a, o, C, bf, shared, cur());
+    if (shared) {
+      const long rows = (long)a.T * a.B * a.Hk;
+      srl::delta::launch_delta_head_sum(p + hq, dq.data_ptr(), rows, a.Hv / a.Hk, a.Dk, bf, cur());
+      srl::delta::launch_delta_head_sum(p + hk, dk.data_ptr(), rows, a.Hv / a.Hk, a.Dk, bf, cur());
+    }
+    launched("gated_delta backward");
+    g[0] = dq, g[1] = dk, g[2] = dv, g[3] = dg, g[4] = db;
+    once(g, "gated_delta");
+    return g;
+  }
+};
+
+// The recurrent form over all T steps; the state after them goes to `after` (which may be `state`)
+Tensor delta_steps(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& decay, const Tensor& beta, const Tensor& state,
+                   const Tensor& first, const Tensor& lengths, const DeltaOpts& opt, const Tensor& after) {
+  auto a = delta_args(q, k, v, decay, beta, first, lengths, opt);
+  a.state = fp(state);
   const c10::DeviceGuard guard(q.device());
-  on(state_out, q, "gated_delta state");
-  shape(state_out, {a.B, a.Hv, a.Dk, a.Dv}, "gated_delta state");
-  TORCH_CHECK(state_out.scalar_type() == torch::kFloat32, "gated_delta: state fp32");
-  TORCH_CHECK((state_out.stride(3) == 1 || a.Dv == 1) && (state_out.stride(2) == a.Dv || a.Dk == 1), "gated_delta: state [B, Hv, Dk, Dv] with contiguous [Dk, Dv]");
-  if (a.state) TORCH_CHECK(state->strides() == state_out.strides(), "gated_delta: the states before and after have the same strides");
   auto out = torch::empty({a.T, a.B, a.Hv, a.Dv}, v.options());
-  srl::delta::launch_delta_steps(a, out.data_ptr(), state_out.data_ptr<float>(), state_out.stride(0), state_out.stride(1),
+  srl::delta::launch_delta_steps(a, out.data_ptr(), after.data_ptr<float>(), after.stride(0), after.stride(1),
                                  q.scalar_type() == torch::kBFloat16, cur());
-  launched("gated_delta_steps");
+  launched("gated_delta");
   return out;
 }
 
-// ------------------------------------------------------------------ gated residual norms
-const float* par(const OptT& t, const Tensor& x, const char* name) {
-  if (!has(t)) return nullptr;
-  on(*t, x, name);
-  TORCH_CHECK(t->scalar_type() == torch::kFloat32 && t->is_contiguous() && t->dim() == 1 && t->size(0) == x.size(1), name,
-              ": fp32 [", x.size(1), "], contiguous");
-  return t->data_ptr<float>();
+// Up to this many steps without a gradient the recurrent kernel is taken.
+constexpr int RECURRENT_MAX_STEPS = 16;
+
+std::pair<Tensor, Tensor> gated_delta(Tensor q, Tensor k, Tensor v, Tensor decay, Tensor beta, OptT state_, OptT first_, OptT lengths_,
+                                      c10::optional<double> scale, bool normalize, double eps) {
+  Tensor state = val(state_);
+  delta_check(q, k, v, decay, beta, state, 2);
+  const int64_t T = v.size(0), B = v.size(1);
+  const Tensor first = delta_first(first_, {T, B}, v), lengths = delta_lengths(lengths_, B, v);
+  const DeltaOpts opt{scale.has_value() ? *scale : 1.0 / std::sqrt((double)q.size(3)), eps, normalize};
+  q = unit_last(q), k = unit_last(k), v = unit_last(v), decay = f32(decay), beta = f32(beta);
+  if (state.defined()) state = state.contiguous();
+  if (at::GradMode::is_enabled() && (wants(q) || wants(k) || wants(v) || wants(decay) || wants(beta) || wants(state))) {
+    auto r = GatedDeltaFn::apply(q, k, v, decay, beta, opt_of(state), opt_of(first), opt_of(lengths), opt.scale, normalize, eps, wants(state));
+    return {r[0], r[1]};
+  }
+  if (T <= RECURRENT_MAX_STEPS) {
+    auto last = torch::empty({B, v.size(2), q.size(3), v.size(3)}, decay.options());
+    auto out = delta_steps(q, k, v, decay, beta, state, first, lengths, opt, last);
+    return {out, last};
+  }
+  return delta_forward(q, k, v, decay, beta, state, first, lengths, opt, nullptr);
 }
 
-// rows [R, D] with unit last stride; clears `vec` if 16 bytes at a time cannot be read
-void rows_of(const Tensor& t, const Tensor& x, const char* name, const void** p, long* stride, bool* vec) {
-  on(t, x, name);
-  TORCH_CHECK(t.scalar_type() == x.scalar_type() && t.sizes() == x.sizes() && (t.stride(1) == 1 || t.size(1) == 1), name,
-              ": rows like x with unit last stride");
+Tensor gated_delta_step(Tensor q, Tensor k, Tensor v, Tensor decay, Tensor beta, Tensor state, OptT first_, c10::optional<double> scale,
+                        bool normalize, double eps) {
+  delta_check(q, k, v, decay, beta, state, 1);
+  TORCH_CHECK(!at::GradMode::is_enabled() ||
+                  !(wants(q) || wants(k) || wants(v) || wants(decay) || wants(beta) || wants(state)),
+              "gated_delta_step updates the state in place and has no gradient: use gated_delta, or torch.no_grad()");
+  const int64_t B = state.size(0), Hv = state.size(1), Dk = state.size(2), Dv = state.size(3);
+  const Tensor first = delta_first(first_, {B}, v);
+  TORCH_CHECK_VALUE((Dv == 1 || state.stride(3) == 1) && (Dk == 1 || state.stride(2) == Dv),
+                    "each [Dk, Dv] of the state must be contiguous, got strides ", state.strides());
+  int64_t d0 = 0, d1 = 1;
+  if (B > 1 && Hv > 1 && state.stride(0) < state.stride(1)) std::swap(d0, d1);
+  // d1 the inner of the two leading axes
+  if (B == 1) std::swap(d0, d1);
+  int64_t least = Dk * Dv;
+  for (int64_t d : {d1, d0}) {
+    if (state.size(d) <= 1) continue;
+    TORCH_CHECK_VALUE(state.stride(d) >= least, "the states must not overlap, got strides ", state.strides());
+    least = state.stride(d) * state.size(d);
+  }
+  const DeltaOpts opt{scale.has_value() ? *scale : 1.0 / std::sqrt((double)Dk), eps, normalize};
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
+  return delta_steps(unit_last(q).unsqueeze(0), unit_last(k).unsqueeze(0), unit_last(v).unsqueeze(0), f32(decay).unsqueeze(0),
+                     f32(beta).unsqueeze(0), state, first.defined() ? first.unsqueeze(0) : first, Tensor(), opt, state)
+      .squeeze(0);
+}
+
+// ------------------------------------------------------------------ gated residual norms
+// rows of the last axis with unit stride, by a view where there is one
+Tensor rows2d(const Tensor& t) {
+  const int64_t D = t.size(-1);
+  if (t.dim() == 2) return unit_last(t);
+  if (t.is_contiguous()) return t.view({-1, D});
+  return unit_last(t.reshape({-1, D}));
+}
+
+// clears `vec` if 16 bytes at a time cannot be read
+void rows_of(const Tensor& t, const void** p, long* stride, bool* vec) {
   const int n = 16 / (int)t.element_size();
   *p = t.data_ptr();
   *stride = t.stride(0);
-  *vec = *vec && x.size(1) % n == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && t.stride(0) % n == 0;
+  *vec = *vec && t.size(1) % n == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && t.stride(0) % n == 0;
 }
 
-srl::rnorm::Args norm_args(const Tensor& x, const Tensor& h, const OptT& gate, const OptT& scale, const OptT& pw, const OptT& pb,
-                           const OptT& rw, const OptT& rb, bool layer, int64_t act, double eps, double s1, bool* vec) {
-  TORCH_CHECK(x.dim() == 2 && (x.scalar_type() == torch::kFloat32 || x.scalar_type() == torch::kBFloat16),
-              "gated_residual_norm: rows [R, D] in fp32 or bf16");
-  TORCH_CHECK(x.size(1) >= 1 && x.size(1) <= srl::rnorm::MAXD, "gated_residual_norm: 1..", srl::rnorm::MAXD, " columns");
-  TORCH_CHECK(x.size(0) >= 1 && x.size(0) < (1ll << 31) - 64, "gated_residual_norm: 1..2^31 rows");
+struct NormOpts {
+  bool layer;
+  int64_t act;
+  double eps, s1;
+};
+
+// x, h, gate as rows; the weights fp32 [D], contiguous, or undefined
+srl::rnorm::Args norm_args(const Tensor& x, const Tensor& h, const Tensor& gate, const Tensor& scale, const Tensor& pw, const Tensor& pb,
+                           const Tensor& rw, const Tensor& rb, const NormOpts& o, bool* vec) {
   srl::rnorm::Args a{};
   *vec = true;
-  rows_of(x, x, "gated_residual_norm x", &a.x, &a.xs, vec);
-  rows_of(h, x, "gated_residual_norm h", &a.h, &a.hs, vec);
-  if (has(gate)) rows_of(*gate, x, "gated_residual_norm gate", &a.gate, &a.gs, vec);
-  a.scale = par(scale, x, "gated_residual_norm scale");
-  a.pw = par(pw, x, "gated_residual_norm post_weight"), a.pb = par(pb, x, "gated_residual_norm post_bias");
-  a.rw = par(rw, x, "gated_residual_norm pre_weight"), a.rb = par(rb, x, "gated_residual_norm pre_bias");
-  a.rows = (int)x.size(0), a.D = (int)x.size(1), a.layer = layer, a.act = (int)act;
-  a.eps = (float)eps, a.inv_d = 1.f / (float)x.size(1), a.s1 = (float)s1;
+  rows_of(x, &a.x, &a.xs, vec);
+  rows_of(h, &a.h, &a.hs, vec);
+  if (gate.defined()) rows_of(gate, &a.gate, &a.gs, vec);
+  a.scale = fp(scale), a.pw = fp(pw), a.pb = fp(pb), a.rw = fp(rw), a.rb = fp(rb);
+  a.rows = (int)x.size(0), a.D = (int)x.size(1), a.layer = o.layer, a.act = (int)o.act;
+  a.eps = (float)o.eps, a.inv_d = 1.f / (float)x.size(1), a.s1 = (float)o.s1;
   return a;
 }
 
-std::vector<Tensor> residual_norm_fwd(Tensor x, Tensor h, OptT gate, OptT scale, OptT pw, OptT pb, OptT rw, OptT rb, bool layer,
-                                      int64_t act, double eps, double s1) {
+std::pair<Tensor, Tensor> norm_forward(const Tensor& x, const Tensor& h, const Tensor& gate, const Tensor& scale, const Tensor& pw,
+                                       const Tensor& pb, const Tensor& rw, const Tensor& rb, const NormOpts& o) {
   bool vec;
-  auto a = norm_args(x, h, gate, scale, pw, pb, rw, rb, layer, act, eps, s1, &vec);
+  const Tensor x2 = rows2d(x), h2 = rows2d(h), g2 = gate.defined() ? rows2d(gate) : gate;
+  auto a = norm_args(x2, h2, g2, scale, pw, pb, rw, rb, o, &vec);
   const c10::DeviceGuard guard(x.device());
-  auto y = torch::empty({x.size(0), x.size(1)}, x.options()), u = torch::empty_like(y);
+  auto y = torch::empty(x.sizes(), x.options()), u = torch::empty(x.sizes(), x.options());
   a.y = y.data_ptr(), a.u = u.data_ptr();
   srl::rnorm::launch_residual_norm_fwd(a, x.scalar_type() == torch::kBFloat16, vec, cur());
-  launched("residual_norm_fwd");
+  launched("gated_residual_norm");
   return {y, u};
 }
 
-// -> {dx, dh, dgate (empty without a gate), sums [5, D]: dscale, dpost_weight, dpost_bias, dpre_weight, dpre_bias}
-std::vector<Tensor> residual_norm_bwd(Tensor x, Tensor h, OptT gate, OptT scale, OptT pw, OptT pb, OptT rw, OptT rb, bool layer,
-                                      int64_t act, double eps, double s1, OptT dy, OptT du) {
-  bool vec;
-  auto a = norm_args(x, h, gate, scale, pw, pb, rw, rb, layer, act, eps, s1, &vec);
-  const c10::DeviceGuard guard(x.device());
-  srl::rnorm::BwdArgs o{};
-  if (has(dy)) rows_of(*dy, x, "gated_residual_norm dy", &o.dy, &o.dys, &vec);
-  if (has(du)) rows_of(*du, x, "gated_residual_norm du", &o.du, &o.dus, &vec);
-  auto dx = torch::empty({x.size(0), x.size(1)}, x.options()), dh = torch::empty_like(dx);
-  auto dg = has(gate) ? torch::empty_like(dx) : torch::empty({0}, x.options());
-  auto f = x.options().dtype(torch::kFloat32);
-  auto sums = torch::empty({5, x.size(1)}, f);
-  auto part = torch::empty({srl::rnorm::residual_norm_groups(a.rows, a.D), 4, x.size(1)}, f);
-  o.dx = dx.data_ptr(), o.dh = dh.data_ptr(), o.dgate = has(gate) ? dg.data_ptr() : nullptr, o.part = part.data_ptr<float>();
-  srl::rnorm::launch_residual_norm_bwd(a, o, sums.data_ptr<float>(), x.scalar_type() == torch::kBFloat16, vec, cur());
-  launched("residual_norm_bwd");
-  return {dx, dh, dg, sums};
+struct ResidualNormFn : public torch::autograd::Function<ResidualNormFn> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, Tensor x, Tensor h, OptT gate_, OptT scale_, OptT pw_,
+                                                OptT pb_, OptT rw_, OptT rb_, bool layer, int64_t act, double eps, double s1,
+                                                int64_t want) {
+    const Tensor gate = val(gate_), scale = val(scale_), pw = val(pw_), pb = val(pb_), rw = val(rw_), rb = val(rb_);
+    auto r = norm_forward(x, h, gate, scale, pw, pb, rw, rb, NormOpts{layer, act, eps, s1});
+    ctx->save_for_backward({x, h, gate, scale, pw, pb, rw, rb});
+    ctx->saved_data["layer"] = layer;
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["s1"] = s1;
+    ctx->saved_data["want"] = want;
+    ctx->set_materialize_grads(false);
+    return {r.first, r.second};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    torch::autograd::variable_list g(13);
+    if (!grads[0].defined() && !grads[1].defined()) return g;
+    const int64_t want = ctx->saved_data["want"].toInt();
+    const auto s = ctx->get_saved_variables();
+    const Tensor &x = s[0], &gate = s[2];
+    bool vec;
+    const Tensor x2 = rows2d(x), h2 = rows2d(s[1]), g2 = gate.defined() ? rows2d(gate) : gate;
+    auto a = norm_args(x2, h2, g2, s[3], s[4], s[5], s[6], s[7],
+                       NormOpts{ctx->saved_data["layer"].toBool(), ctx->saved_data["act"].toInt(), ctx->saved_data["eps"].toDouble(),
+                                ctx->saved_data["s1"].toDouble()},
+                       &vec);
+    const c10::DeviceGuard guard(x.device());
+    srl::rnorm::BwdArgs o{};
+    Tensor dy, du;
+    if (grads[0].defined()) {
+      dy = rows2d(grads[0]);
+      rows_of(dy, &o.dy, &o.dys, &vec);
+    }
+    if (grads[1].defined()) {
+      du = rows2d(grads[1]);
+      rows_of(du, &o.du, &o.dus, &vec);
+    }
+    g[0] = torch::empty(x.sizes(), x.options());
+    g[1] = torch::empty(x.sizes(), x.options());
+    if (want & 1) g[2] = torch::empty(x.sizes(), x.options());
+    const auto f = x.options().dtype(torch::kFloat32);
+    const Tensor sums = torch::empty({5, a.D}, f), part = torch::empty({srl::rnorm::residual_norm_groups(a.rows, a.D), 4, a.D}, f);
+    o.dx = g[0].data_ptr(), o.dh = g[1].data_ptr(), o.dgate = g[2].defined() ? g[2].data_ptr() : nullptr, o.part = part.data_ptr<float>();
+    srl::rnorm::launch_residual_norm_bwd(a, o, sums.data_ptr<float>(), x.scalar_type() == torch::kBFloat16, vec, cur());
+    launched("gated_residual_norm backward");
+    for (int i = 0; i < 5; ++i)
+      if (want >> (i + 1) & 1) g[3 + i] = sums.select(0, i);
+    once(g, "gated_residual_norm");
+    return g;
+  }
+};
+
+std::pair<Tensor, Tensor> gated_residual_norm(Tensor x, Tensor h, OptT gate_, OptT scale_, OptT pw_, OptT pb_, OptT rw_, OptT rb_, bool layer,
+                                              int64_t act, double eps, double s1) {
+  TORCH_CHECK_VALUE(x.dim() >= 1 && h.sizes() == x.sizes(), "x and h must have one shape, got ", x.sizes(), " and ", h.sizes());
+  const int64_t D = x.size(-1);
+  TORCH_CHECK_VALUE(D >= 1 && D <= srl::rnorm::MAXD, "the last axis must be 1..", srl::rnorm::MAXD, " wide, got ", D);
+  TORCH_CHECK_VALUE(two_types(x), "x must be float32 or bfloat16, got ", x.scalar_type());
+  TORCH_CHECK_VALUE(x.numel() / D < (1ll << 31) - 64, "at most 2^31 rows, got ", x.sizes());
+  auto operand = [&](const Tensor& t) {
+    TORCH_CHECK_VALUE(t.device() == x.device() && t.is_floating_point(), "every operand must be floating point on ", x.device(), ", got ",
+                      t.scalar_type(), " on ", t.device());
+  };
+  operand(h);
+  if (h.scalar_type() != x.scalar_type()) h = h.to(x.scalar_type());
+  Tensor gate = val(gate_);
+  if (gate.defined()) {
+    operand(gate);
+    if (gate.scalar_type() != x.scalar_type()) gate = gate.to(x.scalar_type());
+    if (gate.sizes() != x.sizes()) gate = gate.expand(x.sizes());
+  }
+  const char* names[5] = {"scale", "post_weight", "post_bias", "pre_weight", "pre_bias"};
+  Tensor w[5] = {val(scale_), val(pw_), val(pb_), val(rw_), val(rb_)};
+  bool any = wants(x) || wants(h) || wants(gate);
+  int64_t want = wants(gate);  // and a bit for each weight: the gradients that are made
+  for (int i = 0; i < 5; ++i) {
+    if (!w[i].defined()) continue;
+    if (i == 0 && w[0].dim() == 0) w[0] = w[0].expand({D});
+    shape(w[i], {D}, names[i]);
+    operand(w[i]);
+    w[i] = f32(w[i]).contiguous();
+    any = any || wants(w[i]);
+    want |= (int64_t)wants(w[i]) << (i + 1);
+  }
+  if (at::GradMode::is_enabled() && any) {
+    auto r = ResidualNormFn::apply(x, h, opt_of(gate), opt_of(w[0]), opt_of(w[1]), opt_of(w[2]), opt_of(w[3]), opt_of(w[4]), layer, act, eps, s1, want);
+    return {r[0], r[1]};
+  }
+  return norm_forward(x, h, gate, w[0], w[1], w[2], w[3], w[4], NormOpts{layer, act, eps, s1});
 }
 
 }  // namespace
 
 void register_delta(pybind11::module& m) {
-  m.def("gated_delta_fwd", &gated_delta_fwd);
-  m.def("gated_delta_bwd", &gated_delta_bwd);
-  m.def("gated_delta_steps", &gated_delta_steps);
-  m.def("residual_norm_fwd", &residual_norm_fwd);
-  m.def("residual_norm_bwd", &residual_norm_bwd);
+  m.def("gated_delta", &gated_delta);
+  m.def("gated_delta_step", &gated_delta_step);
+  m.def("gated_residual_norm", &gated_residual_norm);
 }

@@ -481,9 +481,8 @@ __global__ void delta_head_sum_kernel(const float* x, T* y, long n, int rep, int
 template <typename T, int DKT, int C, bool MAP>
 static void launch_state(const Args& a, const BwdArgs& o, hipStream_t st) {
   const size_t lds = strip_lds<DKT, C>(true);
-  auto* f = delta_bwd_state_kernel<T, DKT, C, MAP>;
-  (void)hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-  f<<<a.B * a.Hv * a.nseg, 64 * ((a.Dv + 15) / 16), lds, st>>>(a, o);
+  allow_lds<delta_bwd_state_kernel<T, DKT, C, MAP>>((int)lds);
+  delta_bwd_state_kernel<T, DKT, C, MAP><<<a.B * a.Hv * a.nseg, 64 * ((a.Dv + 15) / 16), lds, st>>>(a, o);
 }
 
 template <typename T, int DKT, int C>
@@ -495,10 +494,9 @@ static void launch_c(const Args& a, const BwdArgs& o, bool per_value_head, hipSt
     }
   }
   launch_state<T, DKT, C, false>(a, o, st);
-  auto* f = delta_bwd_pair_kernel<T, DKT, C>;
   const int lds = (int)sizeof(PairLds<DKT, C>);
-  (void)hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  f<<<a.B * a.Hv * a.N, 64 * DKT, lds, st>>>(a, o, per_value_head ? 1 : 0);
+  allow_lds<delta_bwd_pair_kernel<T, DKT, C>>(lds);
+  delta_bwd_pair_kernel<T, DKT, C><<<a.B * a.Hv * a.N, 64 * DKT, lds, st>>>(a, o, per_value_head ? 1 : 0);
 }
 
 template <typename T>

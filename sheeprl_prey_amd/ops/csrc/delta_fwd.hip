@@ -227,10 +227,9 @@ __global__ void __launch_bounds__(64) delta_scan_kernel(const float* first, cons
 template <typename T, int DKT, int C, bool MAP>
 static void launch_one(const Args& a, const FwdOut& o, hipStream_t st) {
   const size_t lds = strip_lds<DKT, C>(!MAP);
-  auto* f = delta_fwd_kernel<T, DKT, C, MAP>;
-  (void)hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  allow_lds<delta_fwd_kernel<T, DKT, C, MAP>>((int)lds);
   const int nvs = (a.Dv + 15) / 16;
-  f<<<a.B * a.Hv * a.nseg, 64 * (nvs + (MAP ? DKT : 0)), lds, st>>>(a, o);
+  delta_fwd_kernel<T, DKT, C, MAP><<<a.B * a.Hv * a.nseg, 64 * (nvs + (MAP ? DKT : 0)), lds, st>>>(a, o);
 }
 
 template <typename T, int DKT>

@@ -17,7 +17,6 @@ from torch import Tensor
 from sheeprl_prey_amd.ops import reference as ref
 
 MAX_HEAD_DIM = 128
-RECURRENT_MAX_STEPS = 16  # no gradient: up to this many steps the recurrent kernel is used
 
 
 def _check(q: Tensor, k: Tensor, v: Tensor, decay: Tensor, beta: Tensor, state: Optional[Tensor], lead: Tuple[str, ...]) -> None:
@@ -74,43 +73,18 @@ def _lengths(x: Optional[Tensor], B: int, device) -> Optional[Tensor]:
     return x.to(torch.int32).contiguous()
 
 
-def _unit_last(x: Tensor) -> Tensor:
-    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+def _ext():
+    from sheeprl_prey_amd import ops
 
-
-class _GatedDelta(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, decay, beta, state, first, lengths, scale, normalize, eps):
-        from sheeprl_prey_amd.ops import _ext
-
-        ctx.set_materialize_grads(False)
-        out, last, Sc, U, P = _ext().gated_delta_fwd(q, k, v, decay, beta, state, first, lengths, scale, normalize, eps, True)
-        ctx.save_for_backward(q, k, v, decay, beta, first, lengths, Sc, U, P)
-        ctx.meta = (scale, normalize, eps)
-        return out, last
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, d_out, d_last):
-        from sheeprl_prey_amd.ops import _ext
-
-        if d_out is None and d_last is None:
-            return (None,) * 11
-        q, k, v, decay, beta, first, lengths, Sc, U, P = ctx.saved_tensors
-        d_out = None if d_out is None else _unit_last(d_out)
-        d_last = None if d_last is None else d_last.contiguous()
-        dq, dk, dv, dg, db, ds = _ext().gated_delta_bwd(q, k, v, decay, beta, None, first, lengths, *ctx.meta, Sc, U, P, d_out, d_last)
-        return dq, dk, dv, dg, db, ds if ctx.needs_input_grad[5] else None, None, None, None, None, None
+    return ops._ext()  # loud failure if missing
 
 
 def _fused(t: Tensor) -> bool:
-    """The kernels take fp32 and bf16 as they come, so autocast regions use them too."""
+    """The kernels take fp32 and bf16 as they come, so autocast regions use them too.  They check their operands as
+    ``_check`` and its neighbours do here for the eager form."""
     from sheeprl_prey_amd import ops
 
-    if t.is_cuda and ops._FUSED:
-        ops._ext()  # loud failure if missing
-        return True
-    return False
+    return t.is_cuda and ops._FUSED
 
 
 def gated_delta(
@@ -130,24 +104,14 @@ def gated_delta(
 
     Differentiable in ``q``, ``k``, ``v``, ``decay``, ``beta`` and ``state`` (once).  The sums, decays and states are fp32;
     outputs and gradients are rounded once to the operand's type, those of shared key heads after their sum."""
+    if _fused(v) and v.numel() and q.numel():
+        return _ext().gated_delta(q, k, v, decay, beta, state, is_first, lengths, scale, normalize, eps)
     _check(q, k, v, decay, beta, state, ("T", "B"))
     T, B = v.shape[:2]
     first = _flags(is_first, (T, B), "is_first", v.device)
     lens = _lengths(lengths, B, v.device)
     scale = float(q.shape[-1]) ** -0.5 if scale is None else float(scale)
-    if not _fused(v) or T == 0 or B == 0:
-        return ref.gated_delta(q, k, v, decay, beta, state, first, lens, scale, normalize, eps)
-    from sheeprl_prey_amd.ops import _ext
-
-    args = (_unit_last(q), _unit_last(k), _unit_last(v), decay.float(), beta.float(), None if state is None else state.contiguous(),
-            first, lens, scale, bool(normalize), float(eps))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, decay, beta, state)):
-        return _GatedDelta.apply(*args)
-    if T <= RECURRENT_MAX_STEPS:
-        last = torch.empty(B, v.shape[2], q.shape[3], v.shape[3], device=v.device, dtype=torch.float32)
-        return _ext().gated_delta_steps(*args, last), last
-    out, last, *_ = _ext().gated_delta_fwd(*args, False)
-    return out, last
+    return ref.gated_delta(q, k, v, decay, beta, state, first, lens, scale, normalize, eps)
 
 
 def gated_delta_step(
@@ -159,6 +123,8 @@ def gated_delta_step(
     ``q``, ``k`` ``[B, Hk, Dk]``, ``v [B, Hv, Dv]``, ``decay``, ``beta`` ``[B, Hv]``, ``is_first [B(, 1)]`` as in
     :func:`gated_delta`; ``state`` fp32 ``[B, Hv, Dk, Dv]``, each ``[Dk, Dv]`` contiguous and none overlapping (a slice of a larger
     store of states is fine).  No gradient; a captured graph replays it on the same state."""
+    if _fused(v) and v.numel() and q.numel():
+        return _ext().gated_delta_step(q, k, v, decay, beta, state, is_first, scale, normalize, eps)
     _check(q, k, v, decay, beta, state, ("B",))
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, decay, beta, state)):
         raise RuntimeError("gated_delta_step updates the state in place and has no gradient: use gated_delta, or torch.no_grad()")
@@ -174,12 +140,7 @@ def gated_delta_step(
         least = stride * n
     if B == 0:
         return torch.empty_like(v)
-    if not _fused(v):
-        out, last = ref.gated_delta(*(t[None] for t in (q, k, v, decay, beta)), state, None if first is None else first[None], None, scale,
-                                    normalize, eps)
-        state.copy_(last)
-        return out[0]
-    from sheeprl_prey_amd.ops import _ext
-
-    return _ext().gated_delta_steps(*(_unit_last(t)[None] for t in (q, k, v)), decay.float()[None], beta.float()[None], state,
-                                    None if first is None else first[None], None, scale, bool(normalize), float(eps), state)[0]
+    out, last = ref.gated_delta(*(t[None] for t in (q, k, v, decay, beta)), state, None if first is None else first[None], None, scale,
+                                normalize, eps)
+    state.copy_(last)
+    return out[0]

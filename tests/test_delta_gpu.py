@@ -354,3 +354,50 @@ def test_operands_on_two_devices_are_refused():
     x = delta_inputs(4, 2, 1, 1, 8, 8, device="cuda")
     with pytest.raises(ValueError, match="every operand must be on"):
         ops.gated_delta(**{**x, "beta": x["beta"].cpu()})
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(k=torch.zeros(4, 2, 1, 7)), "one shape"),
+    (dict(v=torch.zeros(4, 2, 3, 8)), "multiple of the key heads"),
+    (dict(q=torch.zeros(4, 2, 2, 129), k=torch.zeros(4, 2, 2, 129)), "1..128"),
+    (dict(v=torch.zeros(4, 2, 2, 8, dtype=torch.bfloat16)), "one type"),
+    (dict(q=torch.zeros(4, 2, 2, 8).half(), k=torch.zeros(4, 2, 2, 8).half(), v=torch.zeros(4, 2, 2, 8).half()), "float32 or bfloat16"),
+    (dict(decay=torch.zeros(4, 2)), "decay and beta"),
+    (dict(beta=torch.zeros(4, 2, 2, dtype=torch.int64)), "floating point"),
+    (dict(state=torch.zeros(2, 2, 8, 7)), "state must be"),
+    (dict(state=torch.zeros(2, 2, 8, 8, dtype=torch.bfloat16)), "state must be"),
+    (dict(is_first=torch.zeros(2, 4, dtype=torch.bool)), "is_first must be"),
+    (dict(lengths=torch.zeros(2)), "lengths must be"),
+    (dict(lengths=torch.zeros(3, dtype=torch.int32)), "lengths must be"),
+    (dict(q=torch.zeros(4, 2, 8)), "heads, dim"),
+])
+def test_refusals(change, match):
+    x = delta_inputs(4, 2, 2, 2, 8, 8, device="cuda")
+    with pytest.raises(ValueError, match=match):
+        ops.gated_delta(**{**x, **{n: t.cuda() for n, t in change.items()}})
+
+
+def test_step_refusals():
+    x = {k: t if k == "state" else t[0] for k, t in delta_inputs(1, 2, 1, 2, 8, 8, device="cuda").items()}
+    before = x["state"].clone()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        ops.gated_delta_step(**{**x, "q": x["q"].clone().requires_grad_()})
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.gated_delta_step(**{**x, "state": x["state"].transpose(2, 3)})
+    for bad in (x["state"][:1].expand(2, 2, 8, 8), x["state"][:, :1].expand(2, 2, 8, 8), x["state"].as_strided((2, 2, 8, 8), (128, 60, 8, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.gated_delta_step(**{**x, "state": bad})
+    with pytest.raises(ValueError, match="heads, dim"):
+        ops.gated_delta_step(**{**x, "q": x["q"][None]})
+    assert torch.equal(before, x["state"])
+    heads_first = x["state"].transpose(0, 1).contiguous().transpose(0, 1)
+    a, b = ops.gated_delta_step(**x), ops.gated_delta_step(**{**x, "state": heads_first})
+    assert torch.equal(a, b) and torch.equal(x["state"], heads_first)
+
+
+def test_a_second_differentiation_is_refused():
+    x = {n: t.requires_grad_() for n, t in delta_inputs(20, 1, 1, 1, 16, 16, device="cuda").items()}
+    out, _ = ops.gated_delta(**x)
+    (g,) = torch.autograd.grad(out.square().sum(), x["v"], create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        g.sum().backward()

@@ -137,3 +137,29 @@ def test_captured_training_replays():
         want = (y, u, *torch.autograd.grad((y, u), list(b.values()), (dy, du)))
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(norm="batch"), "norm must be"), (dict(act="relu"), "act must be"), (dict(h=torch.zeros(4, 5)), "one shape"),
+    (dict(scale=torch.zeros(5)), "scale must be"), (dict(pre_bias=torch.zeros(4, 6)), "pre_bias must be"),
+    (dict(x=torch.zeros(1, 8193), h=torch.zeros(1, 8193)), "1..8192"), (dict(x=torch.zeros(4, 6).half()), "float32 or bfloat16"),
+    (dict(post_weight=torch.zeros(6, dtype=torch.int32)), "floating point"),
+])
+def test_refusals(kw, match):
+    args = {**dict(x=torch.zeros(4, 6), h=torch.zeros(4, 6)), **kw}
+    with pytest.raises(ValueError, match=match):
+        ops.gated_residual_norm(**{n: t.cuda() if isinstance(t, torch.Tensor) else t for n, t in args.items()})
+    with pytest.raises(ValueError, match="floating point on"):
+        ops.gated_residual_norm(torch.zeros(4, 6, device="cuda"), torch.zeros(4, 6, device="cuda"), torch.zeros(4, 6))
+
+
+def test_mixed_types_and_a_second_differentiation():
+    a = inputs(8, 32, torch.bfloat16)
+    want = ops.gated_residual_norm(**a)
+    got = ops.gated_residual_norm(**{**a, "h": a["h"].float(), "gate": a["gate"].float(), "scale": a["scale"].double()})
+    assert all(torch.equal(p, q) for p, q in zip(want, got))
+    x = a["x"].float().requires_grad_()
+    y, _ = ops.gated_residual_norm(x, a["h"])
+    (g,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        g.sum().backward()
