@@ -230,6 +230,100 @@ __device__ __forceinline__ void diag_inverse(const float* A, float* Td) {
   for (int i = 0; i < 16; ++i) Td[(16 * q + i) * LT + c] = x[i];
 }
 
+// A barrier for what goes through LDS: __syncthreads() would also wait for every store to memory on its way.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// A chunk of 64 steps on its way from memory to LDS for the strip kernels: K (and Q) as they lie in memory, the pair tiles,
+// the gates.  fetch() starts the reads for the next chunk, commit() writes what has arrived to LDS: the reads have the whole
+// walk over the present chunk to arrive in.
+constexpr int TS = 320, TL = 20;  // a tile in LDS: 16 rows of 20: reads of rows and of columns are free of bank conflicts
+template <typename T, int DKT, int NWT, bool QP>
+struct Stage {
+  static constexpr int LD = 16 * DKT + 4, NE = DKT, RR = 16 / NWT, TH = 64 * NWT;
+  static constexpr int NB = NE * (int)sizeof(T) / 4, TILES = QP ? PAIR_TILES : 14, NT4 = (TILES * 64 + TH - 1) / TH;
+  static constexpr int FLOATS = (QP ? 2 : 1) * 64 * LD + TILES * TS + 3 * 64;
+  float *K, *Q, *tile, *gates;  // gates: beta, gam, e
+  uint32_t rk_[RR][NB], rq_[QP ? RR : 1][NB];
+  float nk[RR], nq[RR];
+  f4 tl[NT4], ga;
+
+  __device__ __forceinline__ explicit Stage(float* lds) : K(lds), Q(lds + 64 * LD), tile(lds + (QP ? 2 : 1) * 64 * LD), gates(tile + TILES * TS) {}
+  // tile x of A (x = 0..9 by rows), P and T
+  __device__ __forceinline__ const float* A(int ti, int tj) const { return tile + (ti * (ti + 1) / 2 + tj) * TS; }
+  __device__ __forceinline__ const float* P(int ti, int tj) const { return tile + (10 + ti * (ti + 1) / 2 + tj) * TS; }
+  __device__ __forceinline__ const float* Ti(int ti) const { return tile + ((QP ? 20 : 10) + ti) * TS; }
+
+  __device__ __forceinline__ void row(uint32_t* w, const T* p, int D, bool ok, bool vec) {
+    const int c0 = (threadIdx.x & 15) * NE;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) w[j] = 0;
+    if (!ok || c0 >= D) return;
+    if (vec) {
+      if constexpr (NB >= 4) {
+#pragma unroll
+        for (int j = 0; j < NB; j += 4) {
+          const uint4 x = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p + c0) + j);
+          w[j] = x.x, w[j + 1] = x.y, w[j + 2] = x.z, w[j + 3] = x.w;
+        }
+      } else if constexpr (NB == 2) {
+        const uint2 x = *reinterpret_cast<const uint2*>(p + c0);
+        w[0] = x.x, w[1] = x.y;
+      } else {
+        w[0] = *reinterpret_cast<const uint32_t*>(p + c0);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NE; ++j)
+        if (c0 + j < D) {
+          if constexpr (sizeof(T) == 4) w[j] = __builtin_bit_cast(uint32_t, p[c0 + j]);
+          else w[j / 2] |= (uint32_t)p[c0 + j].x << (16 * (j & 1));
+        }
+    }
+  }
+  __device__ __forceinline__ void fetch(const Args& a, const T* qp, const T* kp, const float* pair, int t0, int len) {
+#pragma unroll
+    for (int r = 0; r < RR; ++r) {
+      const int i = (threadIdx.x >> 4) + r * 4 * NWT;
+      row(rk_[r], kp + (long)(t0 + i) * a.kt, a.Dk, t0 + i < len, a.veck);
+      nk[r] = pair[PAIR_TILES * 256 + 256 + i];
+      if constexpr (QP) {
+        row(rq_[r], qp + (long)(t0 + i) * a.qt, a.Dk, t0 + i < len, a.vecq);
+        nq[r] = pair[PAIR_TILES * 256 + 192 + i];
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < NT4; ++x) {
+      const int at = threadIdx.x + x * TH;  // 16 bytes each
+      if (at < TILES * 64) tl[x] = row4(pair + 4 * (QP || at < 640 ? at : at + 640));
+    }
+    if (threadIdx.x < 48) ga = row4(pair + PAIR_TILES * 256 + 4 * threadIdx.x);
+  }
+  __device__ __forceinline__ void put(float* d, const uint32_t* w, float n) {
+#pragma unroll
+    for (int j = 0; j < NE; ++j) {
+      float x;
+      if constexpr (sizeof(T) == 4) x = __builtin_bit_cast(float, w[j]);
+      else x = __builtin_bit_cast(float, j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+      d[j] = x * n;
+    }
+  }
+  __device__ __forceinline__ void commit() {
+    const int c0 = (threadIdx.x & 15) * NE;
+#pragma unroll
+    for (int r = 0; r < RR; ++r) {
+      const int i = (threadIdx.x >> 4) + r * 4 * NWT;
+      put(K + i * LD + c0, rk_[r], nk[r]);
+      if constexpr (QP) put(Q + i * LD + c0, rq_[r], nq[r]);
+    }
+#pragma unroll
+    for (int x = 0; x < NT4; ++x) {
+      const int at = threadIdx.x + x * TH;
+      if (at < TILES * 64) *reinterpret_cast<f4*>(tile + (at >> 6) * TS + ((at >> 2) & 15) * TL + 4 * (at & 3)) = tl[x];
+    }
+    if (threadIdx.x < 48) *reinterpret_cast<f4*>(gates + 4 * threadIdx.x) = ga;
+  }
+};
+
 // More than 64 KB of LDS has to be asked for, once for each kernel and device.
 template <auto F>
 static void allow_lds(int bytes) {

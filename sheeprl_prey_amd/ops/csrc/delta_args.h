@@ -23,13 +23,18 @@ struct Args {
   int N, nseg, cps;
 };
 
+// What all value columns of a chunk of 64 steps share, from delta_pairs_kernel: the lower 16 x 16 tiles of A and P (10
+// each, by rows) and the inverses of the diagonal blocks of I + A (4), row-major; then beta, gam, e, 1 / |q| and 1 / |k|.
+constexpr int PAIR_TILES = 24, PAIR_A = 0, PAIR_P = 10, PAIR_T = 20, PAIR_FLOATS = PAIR_TILES * 256 + 5 * 64;
+
 struct FwdOut {
+  float* pairs;     // [BH, N, PAIR_FLOATS] (chunks of 64)
   void* out;        // [T, B, Hv, Dv] contiguous
   float* last;      // [B, Hv, Dk, Dv]
   float* Sc;        // [BH, N, DKp, Dvp] each chunk's first state, or null
   float* U;         // [BH, N, C, Dvp], or null
-  float* Sseg;      // [BH, nseg, DKp, Dvp] each segment's first state (nseg > 1)
-  float* Rseg;      // [BH, nseg, DKp, Dvp] a segment's last state from a zero first state
+  float* Sseg;      // [BH, nseg, Dvp / 16, DKp / 16, 64, 4] each segment's first state (nseg > 1), as the registers hold it
+  float* Rseg;      // the same: a segment's last state from a zero first state
   float* Pseg;      // [BH, nseg, DKp, DKp] the map from a segment's first to its last state
 };
 
@@ -37,11 +42,11 @@ struct BwdArgs {
   const void* dout;  // [T, B, Hv, Dv] by strides, or null
   long ot, ob, oh;
   const float* dlast;  // [B, Hv, Dk, Dv] contiguous, or null
-  const float *Sc, *U, *Pseg;
+  const float *Sc, *U, *Pseg, *pairs;
   float* dSc;   // [BH, N, DKp, Dvp] gradient of each chunk's last state
   float* dR;    // [BH, N, C, Dvp]
-  float* Xseg;  // [BH, nseg, DKp, Dvp]
-  float* dSseg; // [BH, nseg, DKp, Dvp]
+  float* Xseg;   // as Rseg: the gradient of a segment's first state where that of its last is zero
+  float* dSseg;  // as Sseg: the gradient of each segment's last state
   void *dq, *dk;  // [T, B, H?, Dk] contiguous: per key head in the input's type (Hv == Hk), else per value head in fp32
   void* dv;
   float *dg, *db, *dstate;

@@ -159,15 +159,16 @@ struct Workspace {
   Tensor make(const Tensor& like) const { return torch::empty({n}, like.options().dtype(torch::kFloat32)); }
 };
 
-// What a forward pass leaves for the backward pass, in one workspace: Sc, U, Pseg
+// What a forward pass leaves for the backward pass, in one workspace: Sc, U, Pseg, pairs
 struct DeltaSaved {
-  int64_t Sc, U, P, n;
+  int64_t Sc, U, P, pairs, n;
   DeltaSaved(const srl::delta::Args& a, int C) {
     const int64_t BH = (int64_t)a.B * a.Hv, DKp = dkp(a.Dk), Dvp = (a.Dv + 15) / 16 * 16;
     Workspace w;
     Sc = w.add(BH * a.N * DKp * Dvp);
     U = w.add(BH * a.N * C * Dvp);
     P = w.add(a.nseg > 1 ? BH * a.nseg * DKp * DKp : 0);
+    pairs = w.add(C == 64 ? BH * a.N * srl::delta::PAIR_FLOATS : 0);
     n = w.n;
   }
 };
@@ -189,16 +190,17 @@ std::pair<Tensor, Tensor> delta_forward(const Tensor& q, const Tensor& k, const 
   if (saved) {
     *saved = torch::empty({at.n}, decay.options());
     float* p = saved->data_ptr<float>();
-    o.Sc = p + at.Sc, o.U = p + at.U, o.Pseg = p + at.P;
+    o.Sc = p + at.Sc, o.U = p + at.U, o.Pseg = p + at.P, o.pairs = p + at.pairs;
   }
   Tensor ws;
-  if (a.nseg > 1) {
+  if (a.nseg > 1 || !saved) {
     Workspace w;
-    const int64_t s = w.add(BH * a.nseg * DKp * Dvp), r = w.add(BH * a.nseg * DKp * Dvp), m = saved ? 0 : w.add(BH * a.nseg * DKp * DKp);
+    const int64_t segs = a.nseg > 1 ? BH * a.nseg * DKp : 0, s = w.add(segs * Dvp), r = w.add(segs * Dvp);
+    const int64_t m = w.add(saved ? 0 : segs * DKp), pr = w.add(!saved && C == 64 ? BH * a.N * srl::delta::PAIR_FLOATS : 0);
     ws = w.make(q);
     float* p = ws.data_ptr<float>();
     o.Sseg = p + s, o.Rseg = p + r;
-    if (!saved) o.Pseg = p + m;
+    if (!saved) o.Pseg = p + m, o.pairs = p + pr;
   }
   srl::delta::launch_delta_fwd(a, o, C, q.scalar_type() == torch::kBFloat16, cur());
   launched("gated_delta");
@@ -245,7 +247,7 @@ struct GatedDeltaFn : public torch::autograd::Function<GatedDeltaFn> {
     const DeltaSaved at(a, C);
     TORCH_CHECK(s[7].numel() == at.n, "gated_delta: the plan changed between the passes");
     const float* sp = s[7].data_ptr<float>();
-    o.Sc = sp + at.Sc, o.U = sp + at.U, o.Pseg = sp + at.P;
+    o.Sc = sp + at.Sc, o.U = sp + at.U, o.Pseg = sp + at.P, o.pairs = sp + at.pairs;
     const bool shared = a.Hk != a.Hv, bf = q.scalar_type() == torch::kBFloat16;
     Workspace w;
     const int64_t segs = a.nseg > 1 ? BH * a.nseg * DKp * Dvp : 0, heads = shared ? (int64_t)a.T * BH * a.Dk : 0;

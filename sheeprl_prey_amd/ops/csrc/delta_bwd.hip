@@ -3,7 +3,7 @@
 // With dS the gradient of a chunk's last state, dO that of its outputs, and T = (I + A)^-1:
 //   dU = P^T dO + diag(e) K dS,   dR = T^T dU,   dV = diag(beta) dR,
 //   dS0 = gam_C dS + scale Q^T diag(gam) dO - K^T diag(beta gam) dR:
-// again nothing mixes the value columns, so delta_bwd_state_kernel walks the chunks backwards with one wave a strip of 16
+// again nothing mixes the value columns, so delta_bwd_walk_kernel walks the chunks backwards with one wave a strip of 16
 // of them, dS in registers, split into segments over a long axis as the forward walk is (the map of dS over a segment
 // is the transpose of Pseg).  What sums over the value columns is left to delta_bwd_pair_kernel, one workgroup a chunk
 // and no order among them:
@@ -19,9 +19,9 @@
 namespace srl {
 namespace delta {
 
-template <typename T, int DKT, int C, bool MAP>
-__global__ void __launch_bounds__(512) delta_bwd_state_kernel(Args a, BwdArgs o) {
-  constexpr int LD = 16 * DKT + 4, LC = C + 4, NT = C / 16, DKp = 16 * DKT;
+template <typename T, int DKT>
+__global__ void __launch_bounds__(512) delta_bwd_short_kernel(Args a, BwdArgs o) {
+  constexpr int C = 16, LD = 16 * DKT + 4, LC = C + 4, DKp = 16 * DKT;
   extern __shared__ __align__(16) unsigned char lds[];
   Gates<C>& s = *reinterpret_cast<Gates<C>*>(lds);
   float* K = reinterpret_cast<float*>(lds + sizeof(Gates<C>));
@@ -31,87 +31,158 @@ __global__ void __launch_bounds__(512) delta_bwd_state_kernel(Args a, BwdArgs o)
   float* Td = P + C * LC;
 
   const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
-  const int BH = a.B * a.Hv, bh = blockIdx.x % BH, seg = blockIdx.x / BH;
-  const int b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
+  const int BH = a.B * a.Hv, bh = blockIdx.x, b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
   const int Dvp = 16 * ((a.Dv + 15) >> 4), dv = 16 * wave + l16;
   const int len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
   const T* qp = reinterpret_cast<const T*>(a.q) + (long)b * a.qb + (long)hk * a.qh;
   const T* kp = reinterpret_cast<const T*>(a.k) + (long)b * a.kb + (long)hk * a.kh;
   const T* gp = o.dout ? reinterpret_cast<const T*>(o.dout) + (long)b * o.ob + (long)h * o.oh : nullptr;
 
-  f4 S[DKT];  // the gradient of the state
+  load_rows<T, DKT, C>(K, s.rk, kp, a.kt, a.Dk, 0, len, a.veck, a.normalize, a.eps);
+  load_rows<T, DKT, C>(Q, s.rq, qp, a.qt, a.Dk, 0, len, a.vecq, a.normalize, a.eps);
+  if (wave == 0) chunk_gates<C>(a, s, b, h, 0, len, lane);
+  f4 S[DKT], dy;  // the gradient of the state, and of the outputs
 #pragma unroll
   for (int m = 0; m < DKT; ++m)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int d = 16 * m + 4 * kq + r;
-      if (MAP) S[m][r] = 0.f;
-      else if (a.nseg > 1) S[m][r] = o.dSseg[(((long)bh * a.nseg + seg) * DKp + d) * Dvp + dv];
-      else S[m][r] = (o.dlast && d < a.Dk && dv < a.Dv) ? o.dlast[((long)bh * a.Dk + d) * a.Dv + dv] : 0.f;
+      S[m][r] = (o.dlast && d < a.Dk && dv < a.Dv) ? o.dlast[((long)bh * a.Dk + d) * a.Dv + dv] : 0.f;
+      o.dSc[((long)bh * DKp + d) * Dvp + dv] = S[m][r];
     }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) dy[r] = (gp && 4 * kq + r < len && dv < a.Dv) ? ld1(gp + (long)(4 * kq + r) * o.ot + dv) : 0.f;
+  lds_barrier();
+  pair_tiles<DKT, C>(K, Q, A, P, s, a.scale, wave, nw);
+  f4 u = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int m = 0; m < DKT; ++m) u = mm16(row4(K + l16 * LD + 16 * m + 4 * kq), S[m], u);
+  lds_barrier();
+  if (wave == 0) diag_inverse<C>(A, Td);
+  lds_barrier();
+  const f4 be = row4(s.beta + 4 * kq), ga = row4(s.gam + 4 * kq);
+  u = mm16(col4(P + 4 * kq * LC + l16, LC), dy, u * row4(s.e + 4 * kq));
+  u = mm16(col4(Td + 4 * kq * LT + l16, LT), u, f4{0.f, 0.f, 0.f, 0.f});
+  T* vp = reinterpret_cast<T*>(o.dv) + (long)bh * a.Dv + dv;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int t = 4 * kq + r;
+    o.dR[((long)bh * C + t) * Dvp + dv] = u[r];
+    if (t < a.T && dv < a.Dv) st1(vp + (long)t * BH * a.Dv, t < len ? be[r] * u[r] : 0.f);
+  }
+  if (!o.dstate) return;
+  const float gc = s.gam[C - 1];
+  const f4 w = dy * (a.scale * ga), z = -(u * ga * be);
+#pragma unroll
+  for (int m = 0; m < DKT; ++m) {
+    S[m] = mm16(col4(Q + 4 * kq * LD + 16 * m + l16, LD), w, S[m] * gc);
+    S[m] = mm16(col4(K + 4 * kq * LD + 16 * m + l16, LD), z, S[m]);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int d = 16 * m + 4 * kq + r;
+      if (d < a.Dk && dv < a.Dv) o.dstate[((long)bh * a.Dk + d) * a.Dv + dv] = S[m][r];
+    }
+  }
+}
 
-  for (int n = min(a.N, (seg + 1) * a.cps) - 1; n >= seg * a.cps; --n) {
-    const int t0 = n * C;
-    if (t0 >= len) {
-      if (!MAP && dv < a.Dv) {
-        T* p = reinterpret_cast<T*>(o.dv) + (long)bh * a.Dv + dv;
-        for (int i = kq; i < C && t0 + i < a.T; i += 4) st1(p + (long)(t0 + i) * BH * a.Dv, 0.f);
-      }
-      continue;
+template <typename T, int DKT, int NWT, bool MAP>
+__global__ void __launch_bounds__(64 * NWT) delta_bwd_walk_kernel(Args a, BwdArgs o) {
+  using St = Stage<T, DKT, NWT, true>;
+  constexpr int C = 64, LD = St::LD, NT = 4, DKp = 16 * DKT;
+  extern __shared__ __align__(16) float flds[];
+  St st(flds);
+
+  const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4, wave = threadIdx.x >> 6;
+  const int BH = a.B * a.Hv, bh = blockIdx.x % BH, seg = blockIdx.x / BH;
+  const int b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
+  const int nvs = (a.Dv + 15) >> 4, Dvp = 16 * nvs, dv = 16 * wave + l16;
+  const bool works = wave < nvs;
+  const int len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
+  const T* qp = reinterpret_cast<const T*>(a.q) + (long)b * a.qb + (long)hk * a.qh;
+  const T* kp = reinterpret_cast<const T*>(a.k) + (long)b * a.kb + (long)hk * a.kh;
+  const T* gp = o.dout ? reinterpret_cast<const T*>(o.dout) + (long)b * o.ob + (long)h * o.oh : nullptr;
+  const float* pairs = o.pairs + (long)bh * a.N * PAIR_FLOATS;
+
+  const f4 zero = {0.f, 0.f, 0.f, 0.f};
+  f4 S[DKT], dn[NT];  // the gradient of the state; the next chunk's of the outputs
+#pragma unroll
+  for (int m = 0; m < DKT; ++m) S[m] = zero;
+  if (!MAP && works) {
+    if (a.nseg > 1) {
+      const float* p = o.dSseg + ((((long)bh * a.nseg + seg) * nvs + wave) * DKT * 64 + lane) * 4;
+#pragma unroll
+      for (int m = 0; m < DKT; ++m) S[m] = row4(p + m * 256);
+    } else if (o.dlast) {
+#pragma unroll
+      for (int m = 0; m < DKT; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int d = 16 * m + 4 * kq + r;
+          if (d < a.Dk && dv < a.Dv) S[m][r] = o.dlast[((long)bh * a.Dk + d) * a.Dv + dv];
+        }
     }
-    if (!MAP) {
+  }
+  auto load_dy = [&](int t0) {
+#pragma unroll
+    for (int ti = 0; ti < NT; ++ti)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int t = t0 + 16 * ti + 4 * kq + r;
+        dn[ti][r] = (gp && works && t < len && dv < a.Dv) ? ld1(gp + (long)t * o.ot + dv) : 0.f;
+      }
+  };
+
+  const int n0 = seg * a.cps, n1 = min(a.N, n0 + a.cps), live = min(n1, (len + C - 1) / C);
+  if (n0 < live) {
+    st.fetch(a, qp, kp, pairs + (long)(live - 1) * PAIR_FLOATS, (live - 1) * C, len);
+    load_dy((live - 1) * C);
+  }
+  for (int n = live - 1; n >= n0; --n) {
+    const int t0 = n * C;
+    if (!MAP && works) {
       float* p = o.dSc + ((long)bh * a.N + n) * DKp * Dvp + dv;
 #pragma unroll
       for (int m = 0; m < DKT; ++m)
 #pragma unroll
         for (int r = 0; r < 4; ++r) p[(16 * m + 4 * kq + r) * Dvp] = S[m][r];
     }
-    __syncthreads();
-    load_rows<T, DKT, C>(K, s.rk, kp, a.kt, a.Dk, t0, len, a.veck, a.normalize, a.eps);
-    load_rows<T, DKT, C>(Q, s.rq, qp, a.qt, a.Dk, t0, len, a.vecq, a.normalize, a.eps);
-    if (wave == 0) chunk_gates<C>(a, s, b, h, t0, len, lane);
-    f4 dy[NT];
+    lds_barrier();
+    st.commit();
+    lds_barrier();
+    f4 dy[NT], u[NT];
 #pragma unroll
-    for (int ti = 0; ti < NT; ++ti)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int t = t0 + 16 * ti + 4 * kq + r;
-        dy[ti][r] = (gp && t < len && dv < a.Dv) ? ld1(gp + (long)t * o.ot + dv) : 0.f;
-      }
-    __syncthreads();
-    pair_tiles<DKT, C>(K, Q, A, P, s, a.scale, wave, nw);
-    f4 u[NT];
-#pragma unroll
-    for (int ti = 0; ti < NT; ++ti) u[ti] = f4{0.f, 0.f, 0.f, 0.f};
+    for (int ti = 0; ti < NT; ++ti) dy[ti] = dn[ti], u[ti] = zero;
+    if (n > n0) {
+      st.fetch(a, qp, kp, pairs + (long)(n - 1) * PAIR_FLOATS, t0 - C, len);
+      load_dy(t0 - C);
+    }
+    if (!works) continue;
 #pragma unroll
     for (int m = 0; m < DKT; ++m) {
       f4 x[NT];
 #pragma unroll
-      for (int ti = 0; ti < NT; ++ti) x[ti] = row4(K + (16 * ti + l16) * LD + 16 * m + 4 * kq);
+      for (int ti = 0; ti < NT; ++ti) x[ti] = row4(st.K + (16 * ti + l16) * LD + 16 * m + 4 * kq);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int ti = 0; ti < NT; ++ti) u[ti] = mfma4(x[ti][j], S[m][j], u[ti]);
     }
-    __syncthreads();
-    if (wave == 0) diag_inverse<C>(A, Td);
-    __syncthreads();
     // dR: backward substitution by blocks of 16 steps
 #pragma unroll
     for (int ti = NT - 1; ti >= 0; --ti) {
-      f4 r = u[ti] * row4(s.e + 16 * ti + 4 * kq);
+      f4 r = u[ti] * row4(st.gates + 128 + 16 * ti + 4 * kq);
 #pragma unroll
-      for (int tr = ti; tr < NT; ++tr) r = mm16(col4(P + (16 * tr + 4 * kq) * LC + 16 * ti + l16, LC), dy[tr], r);
+      for (int tr = ti; tr < NT; ++tr) r = mm16(col4(st.P(tr, ti) + 4 * kq * TL + l16, TL), dy[tr], r);
 #pragma unroll
-      for (int tr = ti + 1; tr < NT; ++tr) r = mm16(-col4(A + (16 * tr + 4 * kq) * LC + 16 * ti + l16, LC), u[tr], r);
-      u[ti] = mm16(col4(Td + (16 * ti + 4 * kq) * LT + l16, LT), r, f4{0.f, 0.f, 0.f, 0.f});
+      for (int tr = ti + 1; tr < NT; ++tr) r = mm16(-col4(st.A(tr, ti) + 4 * kq * TL + l16, TL), u[tr], r);
+      u[ti] = mm16(col4(st.Ti(ti) + 4 * kq * TL + l16, TL), r, zero);
     }
     if (!MAP) {
       float* p = o.dR + ((long)bh * a.N + n) * C * Dvp + dv;
       T* vp = reinterpret_cast<T*>(o.dv) + (long)bh * a.Dv + dv;
 #pragma unroll
       for (int ti = 0; ti < NT; ++ti) {
-        const f4 g = u[ti] * row4(s.beta + 16 * ti + 4 * kq);
+        const f4 g = u[ti] * row4(st.gates + 16 * ti + 4 * kq);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int i = 16 * ti + 4 * kq + r;
@@ -120,36 +191,39 @@ __global__ void __launch_bounds__(512) delta_bwd_state_kernel(Args a, BwdArgs o)
         }
       }
     }
-    const float gc = s.gam[C - 1];
+    const float gc = st.gates[64 + C - 1];
 #pragma unroll
     for (int m = 0; m < DKT; ++m) S[m] *= gc;
 #pragma unroll
     for (int ti = 0; ti < NT; ++ti) {
-      const f4 ga = row4(s.gam + 16 * ti + 4 * kq);
-      const f4 w = dy[ti] * (a.scale * ga), z = -(u[ti] * ga * row4(s.beta + 16 * ti + 4 * kq));
-      f4 x[DKT], y[DKT];
+      const f4 ga = row4(st.gates + 64 + 16 * ti + 4 * kq);
+      const f4 w = dy[ti] * (a.scale * ga), z = -(u[ti] * ga * row4(st.gates + 16 * ti + 4 * kq));
+      f4 x[DKT];
 #pragma unroll
-      for (int m = 0; m < DKT; ++m) {
-        x[m] = col4(Q + (16 * ti + 4 * kq) * LD + 16 * m + l16, LD);
-        y[m] = col4(K + (16 * ti + 4 * kq) * LD + 16 * m + l16, LD);
-      }
+      for (int m = 0; m < DKT; ++m) x[m] = col4(st.Q + (16 * ti + 4 * kq) * LD + 16 * m + l16, LD);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int m = 0; m < DKT; ++m) S[m] = mfma4(x[m][j], w[j], S[m]);
 #pragma unroll
+      for (int m = 0; m < DKT; ++m) x[m] = col4(st.K + (16 * ti + 4 * kq) * LD + 16 * m + l16, LD);
+#pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int m = 0; m < DKT; ++m) S[m] = mfma4(y[m][j], z[j], S[m]);
+        for (int m = 0; m < DKT; ++m) S[m] = mfma4(x[m][j], z[j], S[m]);
     }
   }
+  if (!works) return;
   if (MAP) {
-    float* p = o.Xseg + ((long)bh * a.nseg + seg) * DKp * Dvp + dv;
+    float* p = o.Xseg + ((((long)bh * a.nseg + seg) * nvs + wave) * DKT * 64 + lane) * 4;
 #pragma unroll
-    for (int m = 0; m < DKT; ++m)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) p[(16 * m + 4 * kq + r) * Dvp] = S[m][r];
-  } else if (seg == 0 && o.dstate && dv < a.Dv) {
+    for (int m = 0; m < DKT; ++m) *reinterpret_cast<f4*>(p + m * 256) = S[m];
+    return;
+  }
+  if (dv >= a.Dv) return;
+  T* vp = reinterpret_cast<T*>(o.dv) + (long)bh * a.Dv + dv;  // behind the sequence's end: zeros
+  for (int t = max(n0, live) * C + kq; t < min(a.T, n1 * C); t += 4) st1(vp + (long)t * BH * a.Dv, 0.f);
+  if (seg == 0 && o.dstate) {
 #pragma unroll
     for (int m = 0; m < DKT; ++m)
 #pragma unroll
@@ -478,25 +552,30 @@ __global__ void delta_head_sum_kernel(const float* x, T* y, long n, int rep, int
   st1(y + i, v);
 }
 
-template <typename T, int DKT, int C, bool MAP>
-static void launch_state(const Args& a, const BwdArgs& o, hipStream_t st) {
-  const size_t lds = strip_lds<DKT, C>(true);
-  allow_lds<delta_bwd_state_kernel<T, DKT, C, MAP>>((int)lds);
-  delta_bwd_state_kernel<T, DKT, C, MAP><<<a.B * a.Hv * a.nseg, 64 * ((a.Dv + 15) / 16), lds, st>>>(a, o);
+template <typename T, int DKT, int NWT, bool MAP>
+static void launch_walk(const Args& a, const BwdArgs& o, hipStream_t st) {
+  const int lds = Stage<T, DKT, NWT, true>::FLOATS * (int)sizeof(float);
+  allow_lds<delta_bwd_walk_kernel<T, DKT, NWT, MAP>>(lds);
+  delta_bwd_walk_kernel<T, DKT, NWT, MAP><<<a.B * a.Hv * a.nseg, 64 * NWT, lds, st>>>(a, o);
 }
 
 template <typename T, int DKT, int C>
 static void launch_c(const Args& a, const BwdArgs& o, bool per_value_head, hipStream_t st) {
-  if constexpr (C == 64) {
+  const int nvs = (a.Dv + 15) / 16, BH = a.B * a.Hv;
+  if constexpr (C == 16) {
+    delta_bwd_short_kernel<T, DKT><<<BH, 64 * nvs, strip_lds<DKT, 16>(true), st>>>(a, o);
+  } else {
     if (a.nseg > 1) {
-      launch_state<T, DKT, C, true>(a, o, st);
-      launch_delta_scan_rev(o.dlast, o.Pseg, o.Xseg, o.dSseg, a.B * a.Hv, a.nseg, a.Dk, a.Dv, st);
+      if (nvs <= 4) launch_walk<T, DKT, 4, true>(a, o, st);
+      else launch_walk<T, DKT, 8, true>(a, o, st);
+      launch_delta_scan_rev(o.dlast, o.Pseg, o.Xseg, o.dSseg, BH, a.nseg, a.Dk, a.Dv, st);
     }
+    if (nvs <= 4) launch_walk<T, DKT, 4, false>(a, o, st);
+    else launch_walk<T, DKT, 8, false>(a, o, st);
   }
-  launch_state<T, DKT, C, false>(a, o, st);
   const int lds = (int)sizeof(PairLds<DKT, C>);
   allow_lds<delta_bwd_pair_kernel<T, DKT, C>>(lds);
-  delta_bwd_pair_kernel<T, DKT, C><<<a.B * a.Hv * a.N, 64 * DKT, lds, st>>>(a, o, per_value_head ? 1 : 0);
+  delta_bwd_pair_kernel<T, DKT, C><<<BH * a.N, 64 * DKT, lds, st>>>(a, o, per_value_head ? 1 : 0);
 }
 
 template <typename T>

@@ -1,81 +1,206 @@
 // The gated delta rule, chunked form, forward (the mathematics and the layout: delta.h).
 //
-// delta_fwd_kernel<MAP = false>: one workgroup walks the chunks of one segment of one (sequence, value head), one wave
-// per 16 value columns.  With few heads the chip would wait for the walk, so a long axis is split into segments: the
-// walk is affine in its first state, S_last = Pseg S_first + Rseg, and <MAP = true> finds both for every segment at
-// once, Rseg as the walk from zero and Pseg as the walk of the identity's columns with v = 0; delta_scan_kernel joins
-// the segments; then every segment walks again from its first state and writes the outputs.
+// Chunks of 64 steps: delta_pairs_kernel finds A, P, the inverses of the diagonal blocks of I + A and the gates of every
+// chunk, all chunks at once, for the forward and the backward walk.  delta_walk_kernel<MAP = false> walks the chunks of
+// one segment of one (sequence, value head), one wave per 16 value columns, the next chunk's operands on their way while it
+// works on this one.  With few heads the chip would wait for the walk, so a long axis is split into segments: the walk is
+// affine in its first state, S_last = Pseg S_first + Rseg, and <MAP = true> finds both for every segment at once, Rseg as the
+// walk from zero and Pseg as the walk of the identity's columns with v = 0; delta_scan_kernel joins the segments; then
+// every segment walks again from its first state and writes the outputs.
+//
+// Sequences of at most 16 steps are one chunk of 16: delta_short_kernel does all of it at once.
 #include "delta.h"
 
 namespace srl {
 namespace delta {
 
-template <typename T, int DKT, int C, bool MAP>
-__global__ void __launch_bounds__(MAP ? 1024 : 512) delta_fwd_kernel(Args a, FwdOut o) {
-  constexpr int LD = 16 * DKT + 4, LC = C + 4, NT = C / 16, DKp = 16 * DKT;
+template <typename T, int DKT>
+__global__ void __launch_bounds__(512) delta_short_kernel(Args a, FwdOut o) {
+  constexpr int C = 16, LD = 16 * DKT + 4, LC = C + 4, DKp = 16 * DKT;
   extern __shared__ __align__(16) unsigned char lds[];
   Gates<C>& s = *reinterpret_cast<Gates<C>*>(lds);
   float* K = reinterpret_cast<float*>(lds + sizeof(Gates<C>));
-  float* Q = K + (MAP ? 0 : C * LD);
+  float* Q = K + C * LD;
   float* A = Q + C * LD;
-  float* P = A + (MAP ? 0 : C * LC);
+  float* P = A + C * LC;
   float* Td = P + C * LC;
 
   const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
-  const int BH = a.B * a.Hv, bh = blockIdx.x % BH, seg = blockIdx.x / BH;
-  const int b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
-  const int nvs = (a.Dv + 15) >> 4, Dvp = 16 * nvs;
+  const int BH = a.B * a.Hv, bh = blockIdx.x, b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
+  const int Dvp = 16 * ((a.Dv + 15) >> 4), dv = 16 * wave + l16;
   const int len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
-  const bool vstrip = !MAP || wave < nvs;
-  const int dv = 16 * (vstrip ? wave : wave - nvs) + l16;
   const T* qp = reinterpret_cast<const T*>(a.q) + (long)b * a.qb + (long)hk * a.qh;
   const T* kp = reinterpret_cast<const T*>(a.k) + (long)b * a.kb + (long)hk * a.kh;
   const T* vp = reinterpret_cast<const T*>(a.v) + (long)b * a.vb + (long)h * a.vh;
 
-  f4 S[DKT];
+  load_rows<T, DKT, C>(K, s.rk, kp, a.kt, a.Dk, 0, len, a.veck, a.normalize, a.eps);
+  load_rows<T, DKT, C>(Q, s.rq, qp, a.qt, a.Dk, 0, len, a.vecq, a.normalize, a.eps);
+  if (wave == 0) chunk_gates<C>(a, s, b, h, 0, len, lane);
+  f4 S[DKT], v;
+#pragma unroll
+  for (int m = 0; m < DKT; ++m)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int d = 16 * m + 4 * kq + r;
+      S[m][r] = (a.state && d < a.Dk && dv < a.Dv) ? a.state[((long)bh * a.Dk + d) * a.Dv + dv] : 0.f;
+      if (o.Sc) o.Sc[((long)bh * DKp + d) * Dvp + dv] = S[m][r];
+    }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) v[r] = (4 * kq + r < len && dv < a.Dv) ? ld1(vp + (long)(4 * kq + r) * a.vt + dv) : 0.f;
+  lds_barrier();
+  pair_tiles<DKT, C>(K, Q, A, P, s, a.scale, wave, nw);
+  f4 u = {0.f, 0.f, 0.f, 0.f}, y = u;
+#pragma unroll
+  for (int m = 0; m < DKT; ++m) {
+    u = mm16(row4(K + l16 * LD + 16 * m + 4 * kq), S[m], u);
+    y = mm16(row4(Q + l16 * LD + 16 * m + 4 * kq), S[m], y);
+  }
+  lds_barrier();
+  if (wave == 0) diag_inverse<C>(A, Td);
+  lds_barrier();
+  const f4 ga = row4(s.gam + 4 * kq);
+  u = mm16(row4(Td + l16 * LT + 4 * kq), row4(s.beta + 4 * kq) * (v - ga * u), f4{0.f, 0.f, 0.f, 0.f});
+  y = mm16(row4(P + l16 * LC + 4 * kq), u, y * (a.scale * ga));
+  T* op = reinterpret_cast<T*>(o.out) + (long)bh * a.Dv + dv;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int t = 4 * kq + r;
+    if (o.U) o.U[((long)bh * C + t) * Dvp + dv] = u[r];
+    if (t < a.T && dv < a.Dv) st1(op + (long)t * BH * a.Dv, t < len ? y[r] : 0.f);
+  }
+  const float gc = s.gam[C - 1];
+  const f4 w = u * row4(s.e + 4 * kq);
+#pragma unroll
+  for (int m = 0; m < DKT; ++m) {
+    S[m] = mm16(col4(K + 4 * kq * LD + 16 * m + l16, LD), w, S[m] * gc);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int d = 16 * m + 4 * kq + r;
+      if (d < a.Dk && dv < a.Dv) o.last[((long)bh * a.Dk + d) * a.Dv + dv] = S[m][r];
+    }
+  }
+}
+
+template <typename T, int DKT>
+__global__ void __launch_bounds__(256) delta_pairs_kernel(Args a, float* pairs) {
+  constexpr int C = 64, LD = 16 * DKT + 4, NT = 4;
+  extern __shared__ __align__(16) unsigned char lds[];
+  Gates<C>& s = *reinterpret_cast<Gates<C>*>(lds);
+  float* K = reinterpret_cast<float*>(lds + sizeof(Gates<C>));
+  float* Q = K + C * LD;
+  float* A = Q + C * LD;  // the four diagonal tiles
+
+  const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4, wave = threadIdx.x >> 6;
+  const int BH = a.B * a.Hv, bh = blockIdx.x % BH, n = blockIdx.x / BH, t0 = n * C;
+  const int b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
+  const int len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
+  if (t0 >= len) return;
+  float* out = pairs + ((long)bh * a.N + n) * PAIR_FLOATS;
+  if (wave == 3) chunk_gates<C>(a, s, b, h, t0, len, lane);
+  load_rows<T, DKT, C>(K, s.rk, reinterpret_cast<const T*>(a.k) + (long)b * a.kb + (long)hk * a.kh, a.kt, a.Dk, t0, len, a.veck,
+                       a.normalize, a.eps);
+  load_rows<T, DKT, C>(Q, s.rq, reinterpret_cast<const T*>(a.q) + (long)b * a.qb + (long)hk * a.qh, a.qt, a.Dk, t0, len, a.vecq,
+                       a.normalize, a.eps);
+  lds_barrier();
+  // the diagonal tiles first: their inverses follow while the others are still made
+  for (int x = wave; x < 10; x += 4) {
+    const int ti = x < 4 ? x : x < 7 ? x - 3 : x < 9 ? x - 5 : 3, tj = x < 4 ? x : x < 7 ? x - 4 : x < 9 ? x - 7 : 0;
+    const int xi = (16 * ti + l16) * LD + 4 * kq;
+    const float* kj = K + (16 * tj + l16) * LD + 4 * kq;
+    f4 dk = {0.f, 0.f, 0.f, 0.f}, dq = dk;
+#pragma unroll
+    for (int m = 0; m < DKT; ++m) {
+      const f4 k = row4(kj + 16 * m), ki = row4(K + xi + 16 * m), qi = row4(Q + xi + 16 * m);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        dk = mfma4(k[j], ki[j], dk);
+        dq = mfma4(k[j], qi[j], dq);
+      }
+    }
+    const int i = 16 * ti + l16, j0 = 16 * tj + 4 * kq, t = ti * (ti + 1) / 2 + tj;
+    const double Gi = s.G[i];
+    const int segi = s.seg[i];
+    const float be = s.beta[i];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float m = pair_decay<C>(s, i, j0 + r, Gi, segi);
+      dk[r] = j0 + r < i ? be * m * dk[r] : 0.f;
+      dq[r] = a.scale * m * dq[r];
+    }
+    *reinterpret_cast<f4*>(out + (PAIR_A + t) * 256 + l16 * 16 + 4 * kq) = dk;
+    *reinterpret_cast<f4*>(out + (PAIR_P + t) * 256 + l16 * 16 + 4 * kq) = dq;
+    if (ti == tj) {  // this wave's own tile: no barrier between its writes and its reads
+      float* d = A + ti * TS;
+      *reinterpret_cast<f4*>(d + l16 * TL + 4 * kq) = dk;
+      __builtin_amdgcn_wave_barrier();
+      float c[16];
+#pragma unroll
+      for (int i2 = 0; i2 < 16; ++i2) {
+        float v = i2 == l16 ? 1.f : 0.f;
+#pragma unroll
+        for (int m4 = 0; m4 < i2; m4 += 4) {
+          const f4 r = row4(d + i2 * TL + m4);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (m4 + j < i2) v = fmaf(-r[j], c[m4 + j], v);
+        }
+        c[i2] = v;
+      }
+#pragma unroll
+      for (int i2 = 0; i2 < 16; ++i2)
+        if ((i2 >> 2) == kq) out[(PAIR_T + ti) * 256 + i2 * 16 + l16] = c[i2];
+    }
+  }
+  float* g = out + PAIR_TILES * 256;
+  const int i = threadIdx.x & 63;
+  g[threadIdx.x] = wave == 0 ? s.beta[i] : wave == 1 ? s.gam[i] : wave == 2 ? s.e[i] : s.rq[i];
+  if (wave == 0) g[256 + i] = s.rk[i];
+}
+
+template <typename T, int DKT, int NWT, bool MAP>
+__global__ void __launch_bounds__(64 * NWT) delta_walk_kernel(Args a, FwdOut o) {
+  using St = Stage<T, DKT, NWT, !MAP>;
+  constexpr int C = 64, LD = St::LD, NT = 4, DKp = 16 * DKT;
+  extern __shared__ __align__(16) float flds[];
+  St st(flds);
+
+  const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4, wave = threadIdx.x >> 6;
+  const int BH = a.B * a.Hv, bh = blockIdx.x % BH, seg = blockIdx.x / BH;
+  const int b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
+  const int nvs = (a.Dv + 15) >> 4, Dvp = 16 * nvs;
+  const int len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
+  const bool vstrip = wave < nvs, works = wave < nvs + (MAP ? DKT : 0);  // the other waves only move operands
+  const int dv = 16 * (vstrip ? wave : wave - nvs) + l16;
+  const T* qp = reinterpret_cast<const T*>(a.q) + (long)b * a.qb + (long)hk * a.qh;
+  const T* kp = reinterpret_cast<const T*>(a.k) + (long)b * a.kb + (long)hk * a.kh;
+  const T* vp = reinterpret_cast<const T*>(a.v) + (long)b * a.vb + (long)h * a.vh;
+  const float* pairs = o.pairs + (long)bh * a.N * PAIR_FLOATS;
+
+  f4 S[DKT], v[NT];
+  const f4 zero = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int m = 0; m < DKT; ++m) S[m] = zero;
   if (MAP) {
+    if (!vstrip) {
 #pragma unroll
-    for (int m = 0; m < DKT; ++m)
+      for (int m = 0; m < DKT; ++m)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) S[m][r] = (!vstrip && 16 * m + 4 * kq + r == dv) ? 1.f : 0.f;
-  } else if (a.nseg > 1) {
-    const float* p = o.Sseg + ((long)bh * a.nseg + seg) * DKp * Dvp + dv;
+        for (int r = 0; r < 4; ++r) S[m][r] = 16 * m + 4 * kq + r == dv ? 1.f : 0.f;
+    }
+  } else if (works && a.nseg > 1) {
+    const float* p = o.Sseg + ((((long)bh * a.nseg + seg) * nvs + wave) * DKT * 64 + lane) * 4;
 #pragma unroll
-    for (int m = 0; m < DKT; ++m)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) S[m][r] = p[(16 * m + 4 * kq + r) * Dvp];
-  } else {
+    for (int m = 0; m < DKT; ++m) S[m] = row4(p + m * 256);
+  } else if (works && a.state) {
 #pragma unroll
     for (int m = 0; m < DKT; ++m)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int d = 16 * m + 4 * kq + r;
-        S[m][r] = (a.state && d < a.Dk && dv < a.Dv) ? a.state[((long)bh * a.Dk + d) * a.Dv + dv] : 0.f;
+        if (d < a.Dk && dv < a.Dv) S[m][r] = a.state[((long)bh * a.Dk + d) * a.Dv + dv];
       }
   }
-
-  const int n1 = min(a.N, (seg + 1) * a.cps);
-  for (int n = seg * a.cps; n < n1; ++n) {
-    const int t0 = n * C;
-    if (!MAP && o.Sc) {
-      float* p = o.Sc + ((long)bh * a.N + n) * DKp * Dvp + dv;
-#pragma unroll
-      for (int m = 0; m < DKT; ++m)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) p[(16 * m + 4 * kq + r) * Dvp] = S[m][r];
-    }
-    if (t0 >= len) {  // behind the sequence's end: the state stays, the outputs are zero
-      if (!MAP && dv < a.Dv) {
-        T* op = reinterpret_cast<T*>(o.out) + (long)bh * a.Dv + dv;
-        for (int i = kq; i < C && t0 + i < a.T; i += 4) st1(op + (long)(t0 + i) * BH * a.Dv, 0.f);
-      }
-      continue;
-    }
-    __syncthreads();  // the chunk before is done with LDS
-    load_rows<T, DKT, C>(K, s.rk, kp, a.kt, a.Dk, t0, len, a.veck, a.normalize, a.eps);
-    if (!MAP) load_rows<T, DKT, C>(Q, s.rq, qp, a.qt, a.Dk, t0, len, a.vecq, a.normalize, a.eps);
-    if (wave == 0) chunk_gates<C>(a, s, b, h, t0, len, lane);
-    f4 v[NT];
+  auto load_v = [&](int t0) {
 #pragma unroll
     for (int ti = 0; ti < NT; ++ti)
 #pragma unroll
@@ -83,33 +208,56 @@ __global__ void __launch_bounds__(MAP ? 1024 : 512) delta_fwd_kernel(Args a, Fwd
         const int t = t0 + 16 * ti + 4 * kq + r;
         v[ti][r] = (vstrip && t < len && dv < a.Dv) ? ld1(vp + (long)t * a.vt + dv) : 0.f;
       }
-    __syncthreads();
-    pair_tiles<DKT, C>(K, MAP ? nullptr : Q, A, P, s, a.scale, wave, nw);
-    // K S0 while the other waves finish their tiles
+  };
+
+  const int n0 = seg * a.cps, n1 = min(a.N, n0 + a.cps), live = min(n1, (len + C - 1) / C);
+  if (n0 < live) {
+    st.fetch(a, qp, kp, pairs + (long)n0 * PAIR_FLOATS, n0 * C, len);
+    load_v(n0 * C);
+  }
+  for (int n = n0; n < live; ++n) {
+    const int t0 = n * C;
+    if (!MAP && o.Sc && works) {
+      float* p = o.Sc + ((long)bh * a.N + n) * DKp * Dvp + dv;
+#pragma unroll
+      for (int m = 0; m < DKT; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) p[(16 * m + 4 * kq + r) * Dvp] = S[m][r];
+    }
+    lds_barrier();  // the chunk before is done with LDS
+    st.commit();
+    lds_barrier();
     f4 u[NT];
 #pragma unroll
-    for (int ti = 0; ti < NT; ++ti) u[ti] = f4{0.f, 0.f, 0.f, 0.f};
+    for (int ti = 0; ti < NT; ++ti) u[ti] = row4(st.gates + 16 * ti + 4 * kq) * v[ti];
+    if (n + 1 < live) {
+      st.fetch(a, qp, kp, pairs + (long)(n + 1) * PAIR_FLOATS, t0 + C, len);
+      load_v(t0 + C);
+    }
+    if (!works) continue;
+    // beta (V - gam K S0)
+    f4 x4[NT];
+#pragma unroll
+    for (int ti = 0; ti < NT; ++ti) x4[ti] = zero;
 #pragma unroll
     for (int m = 0; m < DKT; ++m) {
       f4 x[NT];
 #pragma unroll
-      for (int ti = 0; ti < NT; ++ti) x[ti] = row4(K + (16 * ti + l16) * LD + 16 * m + 4 * kq);
+      for (int ti = 0; ti < NT; ++ti) x[ti] = row4(st.K + (16 * ti + l16) * LD + 16 * m + 4 * kq);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int ti = 0; ti < NT; ++ti) u[ti] = mfma4(x[ti][j], S[m][j], u[ti]);
+        for (int ti = 0; ti < NT; ++ti) x4[ti] = mfma4(x[ti][j], S[m][j], x4[ti]);
     }
-    __syncthreads();
-    if (wave == 0) diag_inverse<C>(A, Td);
-    __syncthreads();
+#pragma unroll
+    for (int ti = 0; ti < NT; ++ti) u[ti] -= row4(st.gates + 16 * ti + 4 * kq) * row4(st.gates + 64 + 16 * ti + 4 * kq) * x4[ti];
     // U: forward substitution by blocks of 16 steps
 #pragma unroll
     for (int ti = 0; ti < NT; ++ti) {
-      const f4 be = row4(s.beta + 16 * ti + 4 * kq), ga = row4(s.gam + 16 * ti + 4 * kq);
-      f4 r = be * (v[ti] - ga * u[ti]);
+      f4 r = u[ti];
 #pragma unroll
-      for (int tc = 0; tc < ti; ++tc) r = mm16(-row4(A + (16 * ti + l16) * LC + 16 * tc + 4 * kq), u[tc], r);
-      u[ti] = mm16(row4(Td + (16 * ti + l16) * LT + 4 * kq), r, f4{0.f, 0.f, 0.f, 0.f});
+      for (int tc = 0; tc < ti; ++tc) r = mm16(-row4(st.A(ti, tc) + l16 * TL + 4 * kq), u[tc], r);
+      u[ti] = mm16(row4(st.Ti(ti) + l16 * TL + 4 * kq), r, zero);
     }
     if (!MAP) {
       if (o.U) {
@@ -121,12 +269,12 @@ __global__ void __launch_bounds__(MAP ? 1024 : 512) delta_fwd_kernel(Args a, Fwd
       }
       f4 y[NT];
 #pragma unroll
-      for (int ti = 0; ti < NT; ++ti) y[ti] = f4{0.f, 0.f, 0.f, 0.f};
+      for (int ti = 0; ti < NT; ++ti) y[ti] = zero;
 #pragma unroll
       for (int m = 0; m < DKT; ++m) {
         f4 x[NT];
 #pragma unroll
-        for (int ti = 0; ti < NT; ++ti) x[ti] = row4(Q + (16 * ti + l16) * LD + 16 * m + 4 * kq);
+        for (int ti = 0; ti < NT; ++ti) x[ti] = row4(st.Q + (16 * ti + l16) * LD + 16 * m + 4 * kq);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -135,9 +283,9 @@ __global__ void __launch_bounds__(MAP ? 1024 : 512) delta_fwd_kernel(Args a, Fwd
       T* op = reinterpret_cast<T*>(o.out) + (long)bh * a.Dv + dv;
 #pragma unroll
       for (int ti = 0; ti < NT; ++ti) {
-        f4 w = y[ti] * (a.scale * row4(s.gam + 16 * ti + 4 * kq));
+        f4 w = y[ti] * (a.scale * row4(st.gates + 64 + 16 * ti + 4 * kq));
 #pragma unroll
-        for (int tj = 0; tj <= ti; ++tj) w = mm16(row4(P + (16 * ti + l16) * LC + 16 * tj + 4 * kq), u[tj], w);
+        for (int tj = 0; tj <= ti; ++tj) w = mm16(row4(st.P(ti, tj) + l16 * TL + 4 * kq), u[tj], w);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int t = t0 + 16 * ti + 4 * kq + r;
@@ -146,29 +294,40 @@ __global__ void __launch_bounds__(MAP ? 1024 : 512) delta_fwd_kernel(Args a, Fwd
       }
     }
     // S' = gam_C S + K^T diag(e) U
-    const float gc = s.gam[C - 1];
+    const float gc = st.gates[64 + C - 1];
 #pragma unroll
     for (int m = 0; m < DKT; ++m) S[m] *= gc;
 #pragma unroll
     for (int ti = 0; ti < NT; ++ti) {
-      const f4 w = u[ti] * row4(s.e + 16 * ti + 4 * kq);
+      const f4 w = u[ti] * row4(st.gates + 128 + 16 * ti + 4 * kq);
       f4 x[DKT];
 #pragma unroll
-      for (int m = 0; m < DKT; ++m) x[m] = col4(K + (16 * ti + 4 * kq) * LD + 16 * m + l16, LD);
+      for (int m = 0; m < DKT; ++m) x[m] = col4(st.K + (16 * ti + 4 * kq) * LD + 16 * m + l16, LD);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int m = 0; m < DKT; ++m) S[m] = mfma4(x[m][j], w[j], S[m]);
     }
   }
+  if (!works) return;
   if (MAP) {
-    const int ld = vstrip ? Dvp : DKp;
-    float* p = (vstrip ? o.Rseg : o.Pseg) + ((long)bh * a.nseg + seg) * DKp * ld + dv;
+    if (vstrip) {
+      float* p = o.Rseg + ((((long)bh * a.nseg + seg) * nvs + wave) * DKT * 64 + lane) * 4;
 #pragma unroll
-    for (int m = 0; m < DKT; ++m)
+      for (int m = 0; m < DKT; ++m) *reinterpret_cast<f4*>(p + m * 256) = S[m];
+    } else {
+      float* p = o.Pseg + ((long)bh * a.nseg + seg) * DKp * DKp + dv;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) p[(16 * m + 4 * kq + r) * ld] = S[m][r];
-  } else if (seg == a.nseg - 1 && dv < a.Dv) {
+      for (int m = 0; m < DKT; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) p[(16 * m + 4 * kq + r) * DKp] = S[m][r];
+    }
+    return;
+  }
+  if (dv >= a.Dv) return;
+  T* op = reinterpret_cast<T*>(o.out) + (long)bh * a.Dv + dv;  // behind the sequence's end: zeros
+  for (int t = max(n0, live) * C + kq; t < min(a.T, n1 * C); t += 4) st1(op + (long)t * BH * a.Dv, 0.f);
+  if (seg == a.nseg - 1) {
 #pragma unroll
     for (int m = 0; m < DKT; ++m)
 #pragma unroll
@@ -179,70 +338,73 @@ __global__ void __launch_bounds__(MAP ? 1024 : 512) delta_fwd_kernel(Args a, Fwd
   }
 }
 
-// Joins the segments: S_{s+1} = Pseg_s S_s + Rseg_s (REV: dS_s = Pseg_s^T dS_{s+1} + Xseg_s), one wave per 16 columns.
+// Joins the segments: S_{s+1} = Pseg_s S_s + Rseg_s (REV: dS_s = Pseg_s^T dS_{s+1} + Xseg_s).  One workgroup per 16
+// columns, one wave per 16 rows; the state goes through LDS, the next segment's map is on its way meanwhile.
 template <int DKT, bool REV>
-__global__ void __launch_bounds__(64) delta_scan_kernel(const float* first, const float* P, const float* R, float* out, int nseg,
-                                                        int Dk, int Dv) {
-  constexpr int DKp = 16 * DKT;
-  const int lane = threadIdx.x, l16 = lane & 15, kq = lane >> 4;
-  const int nvs = (Dv + 15) >> 4, Dvp = 16 * nvs, bh = blockIdx.x / nvs, dv = 16 * (blockIdx.x % nvs) + l16;
-  f4 S[DKT];
+__global__ void __launch_bounds__(64 * DKT) delta_scan_kernel(const float* first, const float* P, const float* R, float* out, int nseg,
+                                                              int Dk, int Dv) {
+  constexpr int DKp = 16 * DKT, LD = DKp + 4;
+  __shared__ __align__(16) float S[2][16 * LD];
+  const int lane = threadIdx.x & 63, m = threadIdx.x >> 6, l16 = lane & 15, kq = lane >> 4;
+  const int nvs = (Dv + 15) >> 4, bh = blockIdx.x / nvs, strip = blockIdx.x % nvs, dv = 16 * strip + l16;
+  f4 s, x[DKT], r;
 #pragma unroll
-  for (int m = 0; m < DKT; ++m)
+  for (int j = 0; j < 4; ++j) {
+    const int d = 16 * m + 4 * kq + j;
+    s[j] = (first && d < Dk && dv < Dv) ? first[((long)bh * Dk + d) * Dv + dv] : 0.f;
+  }
+  auto at = [&](int i) { return (long)bh * nseg + (REV ? nseg - 1 - i : i); };
+  auto native = [&](long g) { return ((g * nvs + strip) * DKT + m) * 256 + lane * 4; };
+  auto fetch = [&](int i) {
+    const float* p = P + at(i) * DKp * DKp;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int d = 16 * m + 4 * kq + r;
-      S[m][r] = (first && d < Dk && dv < Dv) ? first[((long)bh * Dk + d) * Dv + dv] : 0.f;
-    }
+    for (int k = 0; k < DKT; ++k)
+      x[k] = REV ? col4(p + (16 * k + 4 * kq) * DKp + 16 * m + l16, DKp) : row4(p + (16 * m + l16) * DKp + 16 * k + 4 * kq);
+    r = row4(R + native(at(i)));
+  };
+  if (nseg > 1) fetch(0);
   for (int i = 0; i < nseg; ++i) {
-    const int s = REV ? nseg - 1 - i : i;
-    const long at = ((long)bh * nseg + s) * DKp;
-    f4 n[DKT];
-#pragma unroll
-    for (int m = 0; m < DKT; ++m)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) out[(at + 16 * m + 4 * kq + r) * Dvp + dv] = S[m][r];
+    *reinterpret_cast<f4*>(out + native(at(i))) = s;
     if (i == nseg - 1) break;
+    float* l = S[i & 1];
+    *reinterpret_cast<f4*>(l + l16 * LD + 16 * m + 4 * kq) = s;
+    lds_barrier();  // two buffers: the one before is free once every wave is here
+    f4 n0 = r, n1 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int m = 0; m < DKT; ++m)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) n[m][r] = R[(at + 16 * m + 4 * kq + r) * Dvp + dv];
-    const float* p = P + at * DKp;
-#pragma unroll
-    for (int mk = 0; mk < DKT; ++mk) {
-      f4 x[DKT];
-#pragma unroll
-      for (int m = 0; m < DKT; ++m)
-        x[m] = REV ? col4(p + (16 * mk + 4 * kq) * DKp + 16 * m + l16, DKp) : row4(p + (16 * m + l16) * DKp + 16 * mk + 4 * kq);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int m = 0; m < DKT; ++m) n[m] = mfma4(x[m][j], S[mk][j], n[m]);
+    for (int k = 0; k < DKT; k += 2) {
+      n0 = mm16(x[k], row4(l + l16 * LD + 16 * k + 4 * kq), n0);
+      n1 = mm16(x[k + 1], row4(l + l16 * LD + 16 * k + 16 + 4 * kq), n1);
     }
-#pragma unroll
-    for (int m = 0; m < DKT; ++m) S[m] = n[m];
+    if (i + 2 < nseg) fetch(i + 1);
+    s = n0 + n1;
   }
 }
 
-template <typename T, int DKT, int C, bool MAP>
-static void launch_one(const Args& a, const FwdOut& o, hipStream_t st) {
-  const size_t lds = strip_lds<DKT, C>(!MAP);
-  allow_lds<delta_fwd_kernel<T, DKT, C, MAP>>((int)lds);
-  const int nvs = (a.Dv + 15) / 16;
-  delta_fwd_kernel<T, DKT, C, MAP><<<a.B * a.Hv * a.nseg, 64 * (nvs + (MAP ? DKT : 0)), lds, st>>>(a, o);
+template <typename T, int DKT, int NWT, bool MAP>
+static void launch_walk(const Args& a, const FwdOut& o, hipStream_t st) {
+  const int lds = Stage<T, DKT, NWT, !MAP>::FLOATS * (int)sizeof(float);
+  allow_lds<delta_walk_kernel<T, DKT, NWT, MAP>>(lds);
+  delta_walk_kernel<T, DKT, NWT, MAP><<<a.B * a.Hv * a.nseg, 64 * NWT, lds, st>>>(a, o);
 }
 
 template <typename T, int DKT>
 static void launch_dk(const Args& a, const FwdOut& o, int C, hipStream_t st) {
+  const int nvs = (a.Dv + 15) / 16, BH = a.B * a.Hv;
   if (C == 16) {
-    launch_one<T, DKT, 16, false>(a, o, st);
+    const int lds = (int)strip_lds<DKT, 16>(true);
+    delta_short_kernel<T, DKT><<<BH, 64 * nvs, lds, st>>>(a, o);
     return;
   }
+  const int lds = (int)sizeof(Gates<64>) + (2 * 64 * (16 * DKT + 4) + 4 * TS) * (int)sizeof(float);
+  allow_lds<delta_pairs_kernel<T, DKT>>(lds);
+  delta_pairs_kernel<T, DKT><<<BH * a.N, 256, lds, st>>>(a, o.pairs);
   if (a.nseg > 1) {
-    launch_one<T, DKT, 64, true>(a, o, st);
-    delta_scan_kernel<DKT, false><<<a.B * a.Hv * ((a.Dv + 15) / 16), 64, 0, st>>>(a.state, o.Pseg, o.Rseg, o.Sseg, a.nseg, a.Dk, a.Dv);
+    if (nvs + DKT <= 8) launch_walk<T, DKT, 8, true>(a, o, st);
+    else launch_walk<T, DKT, 16, true>(a, o, st);
+    delta_scan_kernel<DKT, false><<<BH * nvs, 64 * DKT, 0, st>>>(a.state, o.Pseg, o.Rseg, o.Sseg, a.nseg, a.Dk, a.Dv);
   }
-  launch_one<T, DKT, 64, false>(a, o, st);
+  if (nvs <= 4) launch_walk<T, DKT, 4, false>(a, o, st);
+  else launch_walk<T, DKT, 8, false>(a, o, st);
 }
 
 template <typename T>
@@ -260,9 +422,9 @@ void launch_delta_fwd(const Args& a, const FwdOut& o, int C, bool is_bf16, hipSt
 void launch_delta_scan_rev(const float* dlast, const float* P, const float* X, float* dS, int BH, int nseg, int Dk, int Dv,
                            hipStream_t st) {
   const int g = BH * ((Dv + 15) / 16);
-  if (Dk <= 32) delta_scan_kernel<2, true><<<g, 64, 0, st>>>(dlast, P, X, dS, nseg, Dk, Dv);
-  else if (Dk <= 64) delta_scan_kernel<4, true><<<g, 64, 0, st>>>(dlast, P, X, dS, nseg, Dk, Dv);
-  else delta_scan_kernel<8, true><<<g, 64, 0, st>>>(dlast, P, X, dS, nseg, Dk, Dv);
+  if (Dk <= 32) delta_scan_kernel<2, true><<<g, 128, 0, st>>>(dlast, P, X, dS, nseg, Dk, Dv);
+  else if (Dk <= 64) delta_scan_kernel<4, true><<<g, 256, 0, st>>>(dlast, P, X, dS, nseg, Dk, Dv);
+  else delta_scan_kernel<8, true><<<g, 512, 0, st>>>(dlast, P, X, dS, nseg, Dk, Dv);
 }
 
 }  // namespace delta
