@@ -14,6 +14,7 @@
 // products chain from registers to registers, and only K, Q, A and P, which all strips share, go through LDS.
 #pragma once
 #include <atomic>
+#include <type_traits>
 
 #include "common.h"
 #include "delta_args.h"
@@ -126,40 +127,75 @@ __device__ __forceinline__ void chunk_gates(const Args& a, Gates<C>& s, int b, i
   }
 }
 
-// Rows t0.. of one head into LDS as fp32 [C][16 DKT + 4], scaled to unit length; 16 lanes a row.
-template <typename T, int DKT, int C>
+// A uniform value that the compiler does not carry over from one turn of a loop to the next: addresses that it would work out
+// once and hold in registers through the whole walk (32 of 64 bits each, to no end but spills) are worked out again instead.
+__device__ __forceinline__ long afresh(long x) {
+  asm volatile("" : "+s"(x));
+  return x;
+}
+
+// Reads that a wave has on their way must not hide behind branches or selects of their results (each would be waited for by
+// itself): rows behind the end and columns past the width are read from the nearest that is there, and zeroed afterwards.
+// There is a first step in any case.
+
+// Rows t0.. of one head into LDS as fp32 [C][16 DKT + 4], scaled to unit length; 16 lanes a row, R rows a thread.
+template <typename T, int DKT, int C, int R>
 __device__ __forceinline__ void load_rows(float* dst, float* rn, const T* src, long st, int D, int t0, int len, bool vec,
                                           bool normalize, float eps) {
   constexpr int LD = 16 * DKT + 4, NE = DKT;
   const int sub = threadIdx.x & 15, c0 = sub * NE;
-  for (int i = threadIdx.x >> 4; i < C; i += blockDim.x >> 4) {
-    const bool ok = t0 + i < len;
-    float x[NE];
+  float x[R][NE];
+  const T* p[R];
 #pragma unroll
-    for (int j = 0; j < NE; ++j) x[j] = 0.f;
-    if (ok) {
-      const T* p = src + (long)(t0 + i) * st + c0;
-      if (vec) {
-        if (c0 < D) ldv<NE>(p, x);
-      } else {
+  for (int r = 0; r < R; ++r) {
+    const int i = (threadIdx.x >> 4) + r * (blockDim.x >> 4);
+    p[r] = src + (long)max(0, min(t0 + i, len - 1)) * st;
+  }
+  if (vec) {
 #pragma unroll
-        for (int j = 0; j < NE; ++j)
-          if (c0 + j < D) x[j] = ld1(p + j);
-      }
+    for (int r = 0; r < R; ++r) ldv<NE>(p[r] + min(c0, D - NE), x[r]);
+  } else {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int j = 0; j < NE; ++j) x[r][j] = ld1(p[r] + min(c0 + j, D - 1));
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int i = (threadIdx.x >> 4) + r * (blockDim.x >> 4);
+    float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < NE; ++j) {
+      x[r][j] = (t0 + i < len && c0 + j < D) ? x[r][j] : 0.f;
+      ss = fmaf(x[r][j], x[r][j], ss);
     }
-    float r = 1.f;
-    if (normalize) {
-      float ss = 0.f;
+    const float n = normalize ? 1.f / sqrtf(row16_sum(ss) + eps) : 1.f;
+    if (i < C) {
+      float* d = dst + i * LD + c0;
 #pragma unroll
-      for (int j = 0; j < NE; ++j) ss = fmaf(x[j], x[j], ss);
-      r = 1.f / sqrtf(row16_sum(ss) + eps);
+      for (int j = 0; j < NE; ++j) d[j] = x[r][j] * n;
+      if (sub == 0) rn[i] = n;
     }
-    float* d = dst + i * LD + c0;
-#pragma unroll
-    for (int j = 0; j < NE; ++j) d[j] = x[j] * r;
-    if (sub == 0) rn[i] = r;
   }
 }
+
+// A strip's values at the 64 (NT = 4) or 16 steps from t0 on: as they lie in memory, and as numbers
+template <typename T, int NT>
+struct Column {
+  T raw[NT][4];
+  __device__ __forceinline__ void fetch(const T* p, long st, int t0, int len, int kq) {
+#pragma unroll
+    for (int ti = 0; ti < NT; ++ti)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) raw[ti][r] = p[(long)min(t0 + 16 * ti + 4 * kq + r, len - 1) * st];
+  }
+  __device__ __forceinline__ f4 get(int ti, int t0, int len, int kq, bool on) const {
+    f4 v;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = (on && t0 + 16 * ti + 4 * kq + r < len) ? ld1(&raw[ti][r]) : 0.f;
+    return v;
+  }
+};
 
 template <int C>
 __device__ __forceinline__ float pair_decay(const Gates<C>& s, int i, int j, double Gi, int segi) {
@@ -233,96 +269,346 @@ __device__ __forceinline__ void diag_inverse(const float* A, float* Td) {
 // A barrier for what goes through LDS: __syncthreads() would also wait for every store to memory on its way.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// ---------------------------------------------------------------- products of the strip kernels
+// fp32 operands (K, Q, dO in fp32) take v_mfma_f32_16x16x4_f32: 64 operations a cycle and SIMD.  Where K, Q and dO are
+// bf16 they are exact operands of v_mfma_f32_16x16x32_bf16 (1024 a cycle), and everything else is cut into three bf16 parts,
+// x = p0 + p1 + p2 (8 bits each, so all 24 of x): an exact operand takes three products, two cut operands the six whose
+// parts are not below 2^-24 of the largest.  fp32 sums throughout, so both forms round alike; two parts would be 2^-17 off.
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));  // not HIP's uint2: its union keeps operands out of registers
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+
+template <bool SP>
+struct Op16;  // an operand over 16 contraction indexes, 4 a lane
+template <>
+struct Op16<false> {
+  f4 x;
+};
+template <>
+struct Op16<true> {
+  u2 p0, p1, p2;
+};
+__device__ __forceinline__ u2 part(f4 x) { return u2{f2bf2(x[0], x[1]), f2bf2(x[2], x[3])}; }
+__device__ __forceinline__ f4 rest(f4 x, u2 p) {
+  return f4{x[0] - __builtin_bit_cast(float, p.x << 16), x[1] - __builtin_bit_cast(float, p.x & 0xffff0000u),
+            x[2] - __builtin_bit_cast(float, p.y << 16), x[3] - __builtin_bit_cast(float, p.y & 0xffff0000u)};
+}
+__device__ __forceinline__ Op16<true> cut3(f4 x) {
+  const u2 p0 = part(x);
+  const f4 r = rest(x, p0);
+  const u2 p1 = part(r);
+  return {p0, p1, part(rest(r, p1))};
+}
+template <bool SP>
+__device__ __forceinline__ Op16<SP> cut(f4 x) {
+  if constexpr (SP) return cut3(x);
+  else return Op16<false>{x};
+}
+template <bool SP>
+struct Exact32;  // a K, Q or dO operand over 32 contraction indexes, 8 a lane
+template <>
+struct Exact32<false> {
+  f4 a, b;
+};
+template <>
+struct Exact32<true> {
+  u4 x;
+};
+__device__ __forceinline__ b8 join(u2 a, u2 b) { return __builtin_bit_cast(b8, __builtin_shufflevector(a, b, 0, 1, 2, 3)); }
+__device__ __forceinline__ f4 mfma32(b8 a, b8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f4 mm32(const Exact32<false>& a, const Op16<false>& b0, const Op16<false>& b1, f4 c) {
+  return mm16(a.b, b1.x, mm16(a.a, b0.x, c));
+}
+__device__ __forceinline__ f4 mm32(const Exact32<true>& a, const Op16<true>& b0, const Op16<true>& b1, f4 c) {
+  const b8 x = __builtin_bit_cast(b8, a.x);
+  c = mfma32(x, join(b0.p2, b1.p2), c);
+  c = mfma32(x, join(b0.p1, b1.p1), c);
+  c = mfma32(x, join(b0.p0, b1.p0), c);
+  return c;
+}
+// two cut operands over 32 indexes, and over 16
+__device__ __forceinline__ f4 mm32(const Op16<false>& a0, const Op16<false>& a1, const Op16<false>& b0, const Op16<false>& b1, f4 c) {
+  return mm16(a1.x, b1.x, mm16(a0.x, b0.x, c));
+}
+__device__ __forceinline__ f4 mm32(const Op16<true>& a0, const Op16<true>& a1, const Op16<true>& b0, const Op16<true>& b1, f4 c) {
+  const b8 x0 = join(a0.p0, a1.p0), x1 = join(a0.p1, a1.p1), y0 = join(b0.p0, b1.p0), y1 = join(b0.p1, b1.p1);
+  c = mfma32(join(a0.p2, a1.p2), y0, c);
+  c = mfma32(x1, y1, c);
+  c = mfma32(x0, join(b0.p2, b1.p2), c);
+  c = mfma32(x1, y0, c);
+  c = mfma32(x0, y1, c);
+  c = mfma32(x0, y0, c);
+  return c;
+}
+// c + a b over 16 indexes.  Cut operands are summed from zero and added to c by plain additions: the 16 x 16 x 16 product must
+// not take over an accumulator that a 16 x 16 x 32 product has just written (the wait that this needs is not put in by the
+// compiler, and the first two rows of each four came out wrong).
+__device__ __forceinline__ f4 mm16o(const Op16<false>& a, const Op16<false>& b, f4 c) { return mm16(a.x, b.x, c); }
+__device__ __forceinline__ f4 mm16o(const Op16<true>& a, const Op16<true>& b, f4 c) {
+  const s4 x0 = __builtin_bit_cast(s4, a.p0), x1 = __builtin_bit_cast(s4, a.p1), y0 = __builtin_bit_cast(s4, b.p0), y1 = __builtin_bit_cast(s4, b.p1);
+  f4 d = {0.f, 0.f, 0.f, 0.f};
+  d = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s4, a.p2), y0, d, 0, 0, 0);
+  d = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(x1, y1, d, 0, 0, 0);
+  d = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(x0, __builtin_bit_cast(s4, b.p2), d, 0, 0, 0);
+  d = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(x1, y0, d, 0, 0, 0);
+  d = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(x0, y1, d, 0, 0, 0);
+  d = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(x0, y0, d, 0, 0, 0);
+  return c + d;
+}
+
 // A chunk of 64 steps on its way from memory to LDS for the strip kernels: K (and Q) as they lie in memory, the pair tiles,
 // the gates.  fetch() starts the reads for the next chunk, commit() writes what has arrived to LDS: the reads have the whole
-// walk over the present chunk to arrive in.
-constexpr int TS = 320, TL = 20;  // a tile in LDS: 16 rows of 20: reads of rows and of columns are free of bank conflicts
-template <typename T, int DKT, int NWT, bool QP>
-struct Stage {
-  static constexpr int LD = 16 * DKT + 4, NE = DKT, RR = 16 / NWT, TH = 64 * NWT;
-  static constexpr int NB = NE * (int)sizeof(T) / 4, TILES = QP ? PAIR_TILES : 14, NT4 = (TILES * 64 + TH - 1) / TH;
-  static constexpr int FLOATS = (QP ? 2 : 1) * 64 * LD + TILES * TS + 3 * 64;
+// walk over the present chunk to arrive in.  MODE: 0 forward, 1 forward without Q and P (maps), 2 backward.
+// What the kernels read: k(ti, m2), q(ti, m2): rows of steps against 32 key columns; kt(m, t2), qt(m, t2): rows of key columns
+// against 32 steps; A (negated), P, Ti: tiles, transposed in the backward mode; rk4, rq4: factors that are not in k and q yet.
+constexpr int TS = 320, TL = 20;  // a fp32 tile in LDS: 16 rows of 20: reads of rows and of columns are free of bank conflicts
+template <typename T, int DKT, int NWT, int MODE>
+struct Stage;
+
+template <int MODE>
+struct TileIndex {
+  static constexpr int N = MODE == 1 ? 14 : 24;
+  static __device__ __forceinline__ int A(int ti, int tj) { return ti * (ti + 1) / 2 + tj; }
+  static __device__ __forceinline__ int P(int ti, int tj) { return 10 + ti * (ti + 1) / 2 + tj; }
+  static __device__ __forceinline__ int Ti(int ti) { return (MODE == 1 ? 10 : 20) + ti; }
+  static __device__ __forceinline__ int source(int x) { return MODE == 1 && x >= 10 ? x + 10 : x; }  // in the pair data
+};
+
+template <int DKT, int NWT, int MODE>
+struct Stage<float, DKT, NWT, MODE> {
+  using TI = TileIndex<MODE>;
+  static constexpr bool SP = false, HQ = MODE != 1;
+  static constexpr int LD = 16 * DKT + 4, NE = DKT, RR = 16 / NWT, TH = 64 * NWT, NT4 = (TI::N * 64 + TH - 1) / TH;
+  static constexpr int BYTES = 4 * ((HQ ? 2 : 1) * 64 * LD + TI::N * TS + 3 * 64);
   float *K, *Q, *tile, *gates;  // gates: beta, gam, e
-  uint32_t rk_[RR][NB], rq_[QP ? RR : 1][NB];
+  float rk_[RR][NE], rq_[HQ ? RR : 1][NE];
   float nk[RR], nq[RR];
   f4 tl[NT4], ga;
+  int l16, kq;
 
-  __device__ __forceinline__ explicit Stage(float* lds) : K(lds), Q(lds + 64 * LD), tile(lds + (QP ? 2 : 1) * 64 * LD), gates(tile + TILES * TS) {}
-  // tile x of A (x = 0..9 by rows), P and T
-  __device__ __forceinline__ const float* A(int ti, int tj) const { return tile + (ti * (ti + 1) / 2 + tj) * TS; }
-  __device__ __forceinline__ const float* P(int ti, int tj) const { return tile + (10 + ti * (ti + 1) / 2 + tj) * TS; }
-  __device__ __forceinline__ const float* Ti(int ti) const { return tile + ((QP ? 20 : 10) + ti) * TS; }
+  __device__ __forceinline__ explicit Stage(void* lds)
+      : K((float*)lds), Q(K + 64 * LD), tile(K + (HQ ? 2 : 1) * 64 * LD), gates(tile + TI::N * TS), l16(threadIdx.x & 15),
+        kq((threadIdx.x >> 4) & 3) {}
+  __device__ __forceinline__ Exact32<false> rows(const float* M, int ti, int m2) const {
+    const float* p = M + (16 * ti + l16) * LD + 32 * m2 + 4 * kq;
+    return {row4(p), row4(p + 16)};
+  }
+  __device__ __forceinline__ Exact32<false> cols(const float* M, int m, int t2) const {
+    const float* p = M + (32 * t2 + 4 * kq) * LD + 16 * m + l16;
+    return {col4(p, LD), col4(p + 16 * LD, LD)};
+  }
+  __device__ __forceinline__ Exact32<false> k(int ti, int m2) const { return rows(K, ti, m2); }
+  __device__ __forceinline__ Exact32<false> q(int ti, int m2) const { return rows(Q, ti, m2); }
+  __device__ __forceinline__ Exact32<false> kt(int m, int t2) const { return cols(K, m, t2); }
+  __device__ __forceinline__ Exact32<false> qt(int m, int t2) const { return cols(Q, m, t2); }
+  __device__ __forceinline__ Op16<false> tl_(int x) const {
+    const float* p = tile + x * TS;
+    return {MODE == 2 ? col4(p + 4 * kq * TL + l16, TL) : row4(p + l16 * TL + 4 * kq)};
+  }
+  __device__ __forceinline__ Op16<false> A(int ti, int tj) const { return tl_(TI::A(ti, tj)); }
+  __device__ __forceinline__ Op16<false> P(int ti, int tj) const { return tl_(TI::P(ti, tj)); }
+  __device__ __forceinline__ Op16<false> Ti(int ti) const { return tl_(TI::Ti(ti)); }
+  __device__ __forceinline__ f4 beta(int ti) const { return row4(gates + 16 * ti + 4 * kq); }
+  __device__ __forceinline__ f4 gam(int ti) const { return row4(gates + 64 + 16 * ti + 4 * kq); }
+  __device__ __forceinline__ f4 e(int ti) const { return row4(gates + 128 + 16 * ti + 4 * kq); }
+  __device__ __forceinline__ float gam_last() const { return gates[127]; }
+  __device__ __forceinline__ f4 rk4(int) const { return f4{1.f, 1.f, 1.f, 1.f}; }
+  __device__ __forceinline__ f4 rq4(int) const { return f4{1.f, 1.f, 1.f, 1.f}; }
 
-  __device__ __forceinline__ void row(uint32_t* w, const T* p, int D, bool ok, bool vec) {
+  __device__ __forceinline__ void rows_(float (*w)[NE], const float* src, long st, int D, int t0, int len, bool vec) {
     const int c0 = (threadIdx.x & 15) * NE;
+    const float* p[RR];
 #pragma unroll
-    for (int j = 0; j < NB; ++j) w[j] = 0;
-    if (!ok || c0 >= D) return;
+    for (int r = 0; r < RR; ++r) p[r] = src + (long)min(t0 + (int)(threadIdx.x >> 4) + r * 4 * NWT, len - 1) * st;
     if (vec) {
-      if constexpr (NB >= 4) {
 #pragma unroll
-        for (int j = 0; j < NB; j += 4) {
-          const uint4 x = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p + c0) + j);
-          w[j] = x.x, w[j + 1] = x.y, w[j + 2] = x.z, w[j + 3] = x.w;
-        }
-      } else if constexpr (NB == 2) {
-        const uint2 x = *reinterpret_cast<const uint2*>(p + c0);
-        w[0] = x.x, w[1] = x.y;
-      } else {
-        w[0] = *reinterpret_cast<const uint32_t*>(p + c0);
-      }
+      for (int r = 0; r < RR; ++r) ldv<NE>(p[r] + min(c0, D - NE), w[r]);
     } else {
 #pragma unroll
-      for (int j = 0; j < NE; ++j)
-        if (c0 + j < D) {
-          if constexpr (sizeof(T) == 4) w[j] = __builtin_bit_cast(uint32_t, p[c0 + j]);
-          else w[j / 2] |= (uint32_t)p[c0 + j].x << (16 * (j & 1));
-        }
+      for (int r = 0; r < RR; ++r)
+#pragma unroll
+        for (int j = 0; j < NE; ++j) w[r][j] = p[r][min(c0 + j, D - 1)];
     }
   }
-  __device__ __forceinline__ void fetch(const Args& a, const T* qp, const T* kp, const float* pair, int t0, int len) {
+  __device__ __forceinline__ void fetch(const Args& a, const float* qp, const float* kp, const float* pair, int t0, int len) {
+    rows_(rk_, kp, a.kt, a.Dk, t0, len, a.veck);
+    if constexpr (HQ) rows_(rq_, qp, a.qt, a.Dk, t0, len, a.vecq);
 #pragma unroll
     for (int r = 0; r < RR; ++r) {
-      const int i = (threadIdx.x >> 4) + r * 4 * NWT;
-      row(rk_[r], kp + (long)(t0 + i) * a.kt, a.Dk, t0 + i < len, a.veck);
-      nk[r] = pair[PAIR_TILES * 256 + 256 + i];
-      if constexpr (QP) {
-        row(rq_[r], qp + (long)(t0 + i) * a.qt, a.Dk, t0 + i < len, a.vecq);
-        nq[r] = pair[PAIR_TILES * 256 + 192 + i];
-      }
+      const float* n = pair + PAIR_TILES * 256 + (threadIdx.x >> 4) + r * 4 * NWT;
+      nk[r] = n[256];
+      if constexpr (HQ) nq[r] = n[192];
     }
 #pragma unroll
     for (int x = 0; x < NT4; ++x) {
-      const int at = threadIdx.x + x * TH;  // 16 bytes each
-      if (at < TILES * 64) tl[x] = row4(pair + 4 * (QP || at < 640 ? at : at + 640));
+      const int at = min((int)threadIdx.x + x * TH, TI::N * 64 - 1);  // 16 bytes each
+      tl[x] = row4(pair + 256 * TI::source(at >> 6) + 4 * (at & 63));
     }
-    if (threadIdx.x < 48) ga = row4(pair + PAIR_TILES * 256 + 4 * threadIdx.x);
+    ga = row4(pair + PAIR_TILES * 256 + 4 * min((int)threadIdx.x, 47));
   }
-  __device__ __forceinline__ void put(float* d, const uint32_t* w, float n) {
-#pragma unroll
-    for (int j = 0; j < NE; ++j) {
-      float x;
-      if constexpr (sizeof(T) == 4) x = __builtin_bit_cast(float, w[j]);
-      else x = __builtin_bit_cast(float, j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
-      d[j] = x * n;
-    }
-  }
-  __device__ __forceinline__ void commit() {
+  __device__ __forceinline__ void commit(int t0, int len, int D) {
     const int c0 = (threadIdx.x & 15) * NE;
 #pragma unroll
     for (int r = 0; r < RR; ++r) {
       const int i = (threadIdx.x >> 4) + r * 4 * NWT;
-      put(K + i * LD + c0, rk_[r], nk[r]);
-      if constexpr (QP) put(Q + i * LD + c0, rq_[r], nq[r]);
+#pragma unroll
+      for (int j = 0; j < NE; ++j) {
+        const bool in = t0 + i < len && c0 + j < D;
+        K[i * LD + c0 + j] = in ? rk_[r][j] * nk[r] : 0.f;
+        if constexpr (HQ) Q[i * LD + c0 + j] = in ? rq_[r][j] * nq[r] : 0.f;
+      }
     }
 #pragma unroll
     for (int x = 0; x < NT4; ++x) {
       const int at = threadIdx.x + x * TH;
-      if (at < TILES * 64) *reinterpret_cast<f4*>(tile + (at >> 6) * TS + ((at >> 2) & 15) * TL + 4 * (at & 3)) = tl[x];
+      if (at < TI::N * 64) *reinterpret_cast<f4*>(tile + (at >> 6) * TS + ((at >> 2) & 15) * TL + 4 * (at & 3)) = (at >> 6) < 10 ? -tl[x] : tl[x];
     }
     if (threadIdx.x < 48) *reinterpret_cast<f4*>(gates + 4 * threadIdx.x) = ga;
   }
 };
+
+// The place of contraction index c among a row's: the 8 that a lane takes of 32 lie together (16 m + 4 (l/16) + j, two m).
+__device__ __forceinline__ int place(int c) { return (c & ~31) | ((c & 12) << 1) | ((c & 16) >> 2) | (c & 3); }
+
+template <int DKT, int NWT, int MODE>
+struct Stage<bf16, DKT, NWT, MODE> {
+  using TI = TileIndex<MODE>;
+  static constexpr bool SP = true, HQ = MODE != 1, QT = MODE == 2;
+  static constexpr int LR = 16 * DKT + 8, LC = 64 + 8, TH = 64 * NWT, NT4 = (TI::N * 64 + TH - 1) / TH;
+  static constexpr int CP = 8 * DKT, RG = TH / CP < 16 ? TH / CP : 16, NG = 16 / RG;  // pairs of columns, groups of four rows at once, of a thread
+  static constexpr int ROWS = 64 * LR, COLS = 16 * DKT * LC;
+  static constexpr int BYTES = 2 * (ROWS + COLS + (HQ ? (QT ? COLS : ROWS) : 0)) + TI::N * 1536 + 5 * 64 * 4;
+  uint16_t *Kr, *Kc, *Qx;
+  u2* tile;   // [tile][part][lane]
+  float* gates;  // beta, gam, e, rq, rk
+  uint32_t rk_[NG][4], rq_[HQ ? NG : 1][4];
+  f4 tl[NT4], ga;
+  int l16, kq;
+
+  __device__ __forceinline__ explicit Stage(void* lds)
+      : Kr((uint16_t*)lds), Kc(Kr + ROWS), Qx(Kc + COLS), tile((u2*)(Qx + (HQ ? (QT ? COLS : ROWS) : 0))),
+        gates((float*)(tile + TI::N * 192)), l16(threadIdx.x & 15), kq((threadIdx.x >> 4) & 3) {}
+  __device__ __forceinline__ Exact32<true> rows(const uint16_t* M, int ti, int m2) const {
+    return {*reinterpret_cast<const u4*>(M + (16 * ti + l16) * LR + 32 * m2 + 8 * kq)};
+  }
+  __device__ __forceinline__ Exact32<true> cols(const uint16_t* M, int m, int t2) const {
+    return {*reinterpret_cast<const u4*>(M + (16 * m + l16) * LC + 32 * t2 + 8 * kq)};
+  }
+  __device__ __forceinline__ Exact32<true> k(int ti, int m2) const { return rows(Kr, ti, m2); }
+  __device__ __forceinline__ Exact32<true> q(int ti, int m2) const { return rows(Qx, ti, m2); }
+  __device__ __forceinline__ Exact32<true> kt(int m, int t2) const { return cols(Kc, m, t2); }
+  __device__ __forceinline__ Exact32<true> qt(int m, int t2) const { return cols(Qx, m, t2); }
+  __device__ __forceinline__ Op16<true> tl_(int x) const {
+    const u2* p = tile + x * 192 + (threadIdx.x & 63);
+    return {p[0], p[64], p[128]};
+  }
+  __device__ __forceinline__ Op16<true> A(int ti, int tj) const { return tl_(TI::A(ti, tj)); }
+  __device__ __forceinline__ Op16<true> P(int ti, int tj) const { return tl_(TI::P(ti, tj)); }
+  __device__ __forceinline__ Op16<true> Ti(int ti) const { return tl_(TI::Ti(ti)); }
+  __device__ __forceinline__ f4 beta(int ti) const { return row4(gates + 16 * ti + 4 * kq); }
+  __device__ __forceinline__ f4 gam(int ti) const { return row4(gates + 64 + 16 * ti + 4 * kq); }
+  __device__ __forceinline__ f4 e(int ti) const { return row4(gates + 128 + 16 * ti + 4 * kq); }
+  __device__ __forceinline__ float gam_last() const { return gates[127]; }
+  __device__ __forceinline__ f4 rq4(int ti) const { return row4(gates + 192 + 16 * ti + 4 * kq); }
+  __device__ __forceinline__ f4 rk4(int ti) const { return row4(gates + 256 + 16 * ti + 4 * kq); }
+
+  __device__ __forceinline__ void rows4(uint32_t (*w)[4], const bf16* src, long st, int D, int t0, int len, bool vec) {
+    const int c = 2 * (threadIdx.x % CP), i0 = 4 * (threadIdx.x / CP < 16 ? threadIdx.x / CP : 0);
+    const bf16* p[NG][4];
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) p[g][r] = src + (long)min(t0 + i0 + 4 * g * RG + r, len - 1) * st;
+    if (vec) {
+      const int x = min(c, D - 2);
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) w[g][r] = *reinterpret_cast<const uint32_t*>(p[g][r] + x);
+    } else {
+      const int x = min(c, D - 1), y = min(c + 1, D - 1);
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) w[g][r] = (uint32_t)p[g][r][x].x | (uint32_t)p[g][r][y].x << 16;
+    }
+  }
+  __device__ __forceinline__ void fetch(const Args& a, const bf16* qp, const bf16* kp, const float* pair, int t0, int len) {
+    rows4(rk_, kp, a.kt, a.Dk, t0, len, a.veck);
+    if constexpr (HQ) rows4(rq_, qp, a.qt, a.Dk, t0, len, a.vecq);
+#pragma unroll
+    for (int x = 0; x < NT4; ++x) {
+      const int at = min((int)threadIdx.x + x * TH, TI::N * 64 - 64 + (int)(threadIdx.x & 63));  // 64 divides TH: at & 63 is the lane
+      const float* p = pair + 256 * TI::source(at >> 6);
+      tl[x] = MODE == 2 ? col4(p + 4 * kq * 16 + l16, 16) : row4(p + 16 * l16 + 4 * kq);
+    }
+    ga = row4(pair + PAIR_TILES * 256 + 4 * min((int)threadIdx.x, 79));
+  }
+  __device__ __forceinline__ void put_rows(uint16_t* M, const uint32_t* w, int i) {
+    const int c = place(2 * (threadIdx.x % CP));
+#pragma unroll
+    for (int r = 0; r < 4; ++r) *reinterpret_cast<uint32_t*>(M + (i + r) * LR + c) = w[r];
+  }
+  __device__ __forceinline__ void put_cols(uint16_t* M, const uint32_t* w, int i) {
+    uint16_t* p = M + 2 * (threadIdx.x % CP) * LC + place(i);
+    *reinterpret_cast<u2*>(p) = u2{(w[0] & 0xffffu) | (w[1] << 16), (w[2] & 0xffffu) | (w[3] << 16)};
+    *reinterpret_cast<u2*>(p + LC) = u2{(w[0] >> 16) | (w[1] & 0xffff0000u), (w[2] >> 16) | (w[3] & 0xffff0000u)};
+  }
+  __device__ __forceinline__ void commit(int t0, int len, int D) {
+    const int g0 = threadIdx.x / CP, c = 2 * (threadIdx.x % CP);
+    const uint32_t cm = c + 1 < D ? ~0u : c < D ? 0xffffu : 0u;
+    if (g0 < 16) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const int i = 4 * (g0 + g * RG);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const uint32_t m = t0 + i + r < len ? cm : 0u;
+          rk_[g][r] &= m;
+          if constexpr (HQ) rq_[g][r] &= m;
+        }
+        put_rows(Kr, rk_[g], i);
+        put_cols(Kc, rk_[g], i);
+        if constexpr (HQ) {
+          if constexpr (QT) put_cols(Qx, rq_[g], i);
+          else put_rows(Qx, rq_[g], i);
+        }
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < NT4; ++x) {
+      const int at = threadIdx.x + x * TH;
+      if (at < TI::N * 64) {
+        const Op16<true> o = cut3((at >> 6) < 10 ? -tl[x] : tl[x]);
+        u2* p = tile + (at >> 6) * 192 + (at & 63);
+        p[0] = o.p0, p[64] = o.p1, p[128] = o.p2;
+      }
+    }
+    if (threadIdx.x < 80) *reinterpret_cast<f4*>(gates + 4 * threadIdx.x) = ga;
+  }
+};
+
+// f(0), ..., f(N - 1) with compile-time indexes: arrays of operands stay in registers
+template <int I, int N, typename F>
+__device__ __forceinline__ void each(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    each<I + 1, N>(f);
+  }
+}
+// c + sum over x = X..N-1 of tile(x) operand(x): pairs of tiles where there are two
+template <int X, int N, typename FA, typename FB>
+__device__ __forceinline__ f4 mm_tiles(FA&& tile, FB&& operand, f4 c) {
+  if constexpr (X + 1 < N) {
+    c = mm32(tile(X), tile(X + 1), operand(std::integral_constant<int, X>{}), operand(std::integral_constant<int, X + 1>{}), c);
+    return mm_tiles<X + 2, N>(tile, operand, c);
+  } else if constexpr (X < N) {
+    return mm16o(tile(X), operand(std::integral_constant<int, X>{}), c);
+  } else {
+    return c;
+  }
+}
 
 // More than 64 KB of LDS has to be asked for, once for each kernel and device.
 template <auto F>

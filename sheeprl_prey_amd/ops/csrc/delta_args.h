@@ -7,6 +7,7 @@ namespace srl {
 namespace delta {
 
 constexpr int MAXD = 128;        // head dimensions
+inline __host__ __device__ int pitch(int Dv) { return Dv <= 64 ? 64 : 128; }  // of a row of value columns in the workspaces: Dvp below
 constexpr float GONE = -104.0f;  // exp(g) rounds to zero in fp32 below this: the step forgets all that was before it
 
 struct Args {
@@ -33,7 +34,7 @@ struct FwdOut {
   float* last;      // [B, Hv, Dk, Dv]
   float* Sc;        // [BH, N, DKp, Dvp] each chunk's first state, or null
   float* U;         // [BH, N, C, Dvp], or null
-  float* Sseg;      // [BH, nseg, Dvp / 16, DKp / 16, 64, 4] each segment's first state (nseg > 1), as the registers hold it
+  float* Sseg;      // [BH, nseg, ceil(Dv / 16), DKp / 16, 64, 4] each segment's first state (nseg > 1), as the registers hold it
   float* Rseg;      // the same: a segment's last state from a zero first state
   float* Pseg;      // [BH, nseg, DKp, DKp] the map from a segment's first to its last state
 };

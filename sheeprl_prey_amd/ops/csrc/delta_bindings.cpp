@@ -163,7 +163,7 @@ struct Workspace {
 struct DeltaSaved {
   int64_t Sc, U, P, pairs, n;
   DeltaSaved(const srl::delta::Args& a, int C) {
-    const int64_t BH = (int64_t)a.B * a.Hv, DKp = dkp(a.Dk), Dvp = (a.Dv + 15) / 16 * 16;
+    const int64_t BH = (int64_t)a.B * a.Hv, DKp = dkp(a.Dk), Dvp = srl::delta::pitch(a.Dv);
     Workspace w;
     Sc = w.add(BH * a.N * DKp * Dvp);
     U = w.add(BH * a.N * C * Dvp);
@@ -181,7 +181,7 @@ std::pair<Tensor, Tensor> delta_forward(const Tensor& q, const Tensor& k, const 
   a.state = fp(state);
   const c10::DeviceGuard guard(q.device());
   const int C = delta_plan(a);
-  const int64_t BH = (int64_t)a.B * a.Hv, DKp = dkp(a.Dk), Dvp = (a.Dv + 15) / 16 * 16;
+  const int64_t BH = (int64_t)a.B * a.Hv, DKp = dkp(a.Dk), Dvp = srl::delta::pitch(a.Dv);
   auto out = torch::empty({a.T, a.B, a.Hv, a.Dv}, v.options());
   auto last = torch::empty({a.B, a.Hv, a.Dk, a.Dv}, decay.options());
   srl::delta::FwdOut o{};
@@ -233,7 +233,7 @@ struct GatedDeltaFn : public torch::autograd::Function<GatedDeltaFn> {
                         DeltaOpts{ctx->saved_data["scale"].toDouble(), ctx->saved_data["eps"].toDouble(), ctx->saved_data["normalize"].toBool()});
     const c10::DeviceGuard guard(q.device());
     const int C = delta_plan(a);
-    const int64_t BH = (int64_t)a.B * a.Hv, DKp = dkp(a.Dk), Dvp = (a.Dv + 15) / 16 * 16;
+    const int64_t BH = (int64_t)a.B * a.Hv, DKp = dkp(a.Dk), Dvp = srl::delta::pitch(a.Dv);
     srl::delta::BwdArgs o{};
     if (dout.defined()) {
       dout = unit_last(dout);

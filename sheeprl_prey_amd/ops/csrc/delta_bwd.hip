@@ -32,16 +32,18 @@ __global__ void __launch_bounds__(512) delta_bwd_short_kernel(Args a, BwdArgs o)
 
   const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
   const int BH = a.B * a.Hv, bh = blockIdx.x, b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
-  const int Dvp = 16 * ((a.Dv + 15) >> 4), dv = 16 * wave + l16;
+  const int Dvp = pitch(a.Dv), dv = 16 * wave + l16;
   const int len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
   const T* qp = reinterpret_cast<const T*>(a.q) + (long)b * a.qb + (long)hk * a.qh;
   const T* kp = reinterpret_cast<const T*>(a.k) + (long)b * a.kb + (long)hk * a.kh;
   const T* gp = o.dout ? reinterpret_cast<const T*>(o.dout) + (long)b * o.ob + (long)h * o.oh : nullptr;
 
-  load_rows<T, DKT, C>(K, s.rk, kp, a.kt, a.Dk, 0, len, a.veck, a.normalize, a.eps);
-  load_rows<T, DKT, C>(Q, s.rq, qp, a.qt, a.Dk, 0, len, a.vecq, a.normalize, a.eps);
+  Column<T, 1> dc;
+  if (gp) dc.fetch(gp + min(dv, a.Dv - 1), o.ot, 0, max(len, 1), kq);
+  load_rows<T, DKT, C, 4>(K, s.rk, kp, a.kt, a.Dk, 0, len, a.veck, a.normalize, a.eps);
+  load_rows<T, DKT, C, 4>(Q, s.rq, qp, a.qt, a.Dk, 0, len, a.vecq, a.normalize, a.eps);
   if (wave == 0) chunk_gates<C>(a, s, b, h, 0, len, lane);
-  f4 S[DKT], dy;  // the gradient of the state, and of the outputs
+  f4 S[DKT];  // the gradient of the state
 #pragma unroll
   for (int m = 0; m < DKT; ++m)
 #pragma unroll
@@ -50,9 +52,8 @@ __global__ void __launch_bounds__(512) delta_bwd_short_kernel(Args a, BwdArgs o)
       S[m][r] = (o.dlast && d < a.Dk && dv < a.Dv) ? o.dlast[((long)bh * a.Dk + d) * a.Dv + dv] : 0.f;
       o.dSc[((long)bh * DKp + d) * Dvp + dv] = S[m][r];
     }
-#pragma unroll
-  for (int r = 0; r < 4; ++r) dy[r] = (gp && 4 * kq + r < len && dv < a.Dv) ? ld1(gp + (long)(4 * kq + r) * o.ot + dv) : 0.f;
   lds_barrier();
+  const f4 dy = dc.get(0, 0, len, kq, gp && dv < a.Dv);
   pair_tiles<DKT, C>(K, Q, A, P, s, a.scale, wave, nw);
   f4 u = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -87,15 +88,16 @@ __global__ void __launch_bounds__(512) delta_bwd_short_kernel(Args a, BwdArgs o)
 
 template <typename T, int DKT, int NWT, bool MAP>
 __global__ void __launch_bounds__(64 * NWT) delta_bwd_walk_kernel(Args a, BwdArgs o) {
-  using St = Stage<T, DKT, NWT, true>;
-  constexpr int C = 64, LD = St::LD, NT = 4, DKp = 16 * DKT;
-  extern __shared__ __align__(16) float flds[];
-  St st(flds);
+  using St = Stage<T, DKT, NWT, 2>;
+  constexpr bool SP = St::SP;
+  constexpr int C = 64, NT = 4, DKp = 16 * DKT, Dvp = NWT == 4 ? 64 : 128;
+  extern __shared__ __align__(16) unsigned char lds[];
+  St st(lds);
 
   const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4, wave = threadIdx.x >> 6;
   const int BH = a.B * a.Hv, bh = blockIdx.x % BH, seg = blockIdx.x / BH;
   const int b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
-  const int nvs = (a.Dv + 15) >> 4, Dvp = 16 * nvs, dv = 16 * wave + l16;
+  const int nvs = (a.Dv + 15) >> 4, dv = 16 * wave + l16;
   const bool works = wave < nvs;
   const int len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
   const T* qp = reinterpret_cast<const T*>(a.q) + (long)b * a.qb + (long)hk * a.qh;
@@ -104,7 +106,9 @@ __global__ void __launch_bounds__(64 * NWT) delta_bwd_walk_kernel(Args a, BwdArg
   const float* pairs = o.pairs + (long)bh * a.N * PAIR_FLOATS;
 
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
-  f4 S[DKT], dn[NT];  // the gradient of the state; the next chunk's of the outputs
+  f4 S[DKT];          // the gradient of the state
+  Column<T, NT> dn;   // the next chunk's of the outputs
+  const T* gcol = gp + min(dv, a.Dv - 1);
 #pragma unroll
   for (int m = 0; m < DKT; ++m) S[m] = zero;
   if (!MAP && works) {
@@ -122,95 +126,81 @@ __global__ void __launch_bounds__(64 * NWT) delta_bwd_walk_kernel(Args a, BwdArg
         }
     }
   }
-  auto load_dy = [&](int t0) {
-#pragma unroll
-    for (int ti = 0; ti < NT; ++ti)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int t = t0 + 16 * ti + 4 * kq + r;
-        dn[ti][r] = (gp && works && t < len && dv < a.Dv) ? ld1(gp + (long)t * o.ot + dv) : 0.f;
-      }
-  };
-
   const int n0 = seg * a.cps, n1 = min(a.N, n0 + a.cps), live = min(n1, (len + C - 1) / C);
   if (n0 < live) {
     st.fetch(a, qp, kp, pairs + (long)(live - 1) * PAIR_FLOATS, (live - 1) * C, len);
-    load_dy((live - 1) * C);
+    if (gp) dn.fetch(gcol, o.ot, (live - 1) * C, len, kq);
   }
   for (int n = live - 1; n >= n0; --n) {
     const int t0 = n * C;
     if (!MAP && works) {
-      float* p = o.dSc + ((long)bh * a.N + n) * DKp * Dvp + dv;
+      float* p = o.dSc + ((long)bh * a.N + n) * DKp * Dvp + 4 * kq * Dvp + dv;
 #pragma unroll
       for (int m = 0; m < DKT; ++m)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) p[(16 * m + 4 * kq + r) * Dvp] = S[m][r];
+        for (int r = 0; r < 4; ++r) p[(16 * m + r) * Dvp] = S[m][r];
     }
     lds_barrier();
-    st.commit();
+    st.commit(t0, len, a.Dk);
     lds_barrier();
     f4 dy[NT], u[NT];
 #pragma unroll
-    for (int ti = 0; ti < NT; ++ti) dy[ti] = dn[ti], u[ti] = zero;
+    for (int ti = 0; ti < NT; ++ti) dy[ti] = dn.get(ti, t0, len, kq, gp && dv < a.Dv), u[ti] = zero;
     if (n > n0) {
       st.fetch(a, qp, kp, pairs + (long)(n - 1) * PAIR_FLOATS, t0 - C, len);
-      load_dy(t0 - C);
+      if (gp) dn.fetch(gcol, o.ot, t0 - C, len, kq);
     }
     if (!works) continue;
 #pragma unroll
-    for (int m = 0; m < DKT; ++m) {
-      f4 x[NT];
+    for (int m2 = 0; m2 < DKT / 2; ++m2) {
+      const Op16<SP> s0 = cut<SP>(S[2 * m2]), s1 = cut<SP>(S[2 * m2 + 1]);
 #pragma unroll
-      for (int ti = 0; ti < NT; ++ti) x[ti] = row4(st.K + (16 * ti + l16) * LD + 16 * m + 4 * kq);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int ti = 0; ti < NT; ++ti) u[ti] = mfma4(x[ti][j], S[m][j], u[ti]);
+      for (int ti = 0; ti < NT; ++ti) u[ti] = mm32(st.k(ti, m2), s0, s1, u[ti]);
     }
     // dR: backward substitution by blocks of 16 steps
-#pragma unroll
-    for (int ti = NT - 1; ti >= 0; --ti) {
-      f4 r = u[ti] * row4(st.gates + 128 + 16 * ti + 4 * kq);
-#pragma unroll
-      for (int tr = ti; tr < NT; ++tr) r = mm16(col4(st.P(tr, ti) + 4 * kq * TL + l16, TL), dy[tr], r);
-#pragma unroll
-      for (int tr = ti + 1; tr < NT; ++tr) r = mm16(-col4(st.A(tr, ti) + 4 * kq * TL + l16, TL), u[tr], r);
-      u[ti] = mm16(col4(st.Ti(ti) + 4 * kq * TL + l16, TL), r, zero);
-    }
+    Op16<SP> ub[NT], db[NT];
+    each<0, NT>([&](auto I) {
+      constexpr int ti = NT - 1 - I;
+      db[ti] = cut<SP>(dy[ti]);
+      f4 r = u[ti] * st.e(ti) * st.rk4(ti);
+      r = mm_tiles<ti, NT>([&](int x) { return st.P(x, ti); }, [&](auto x) { return db[decltype(x)::value]; }, r);
+      r = mm_tiles<ti + 1, NT>([&](int x) { return st.A(x, ti); }, [&](auto x) { return ub[decltype(x)::value]; }, r);
+      u[ti] = mm16o(st.Ti(ti), cut<SP>(r), zero);
+      ub[ti] = cut<SP>(u[ti]);
+    });
     if (!MAP) {
-      float* p = o.dR + ((long)bh * a.N + n) * C * Dvp + dv;
-      T* vp = reinterpret_cast<T*>(o.dv) + (long)bh * a.Dv + dv;
+      const long vstep = afresh((long)BH * a.Dv);
+      float* p = o.dR + ((long)bh * a.N + n) * C * Dvp + 4 * kq * Dvp + dv;
+      T* vp = reinterpret_cast<T*>(o.dv) + (long)bh * a.Dv + dv + (t0 + 4 * kq) * vstep;
 #pragma unroll
       for (int ti = 0; ti < NT; ++ti) {
-        const f4 g = u[ti] * row4(st.gates + 16 * ti + 4 * kq);
+        const f4 g = u[ti] * st.beta(ti);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int i = 16 * ti + 4 * kq + r;
-          p[i * Dvp] = u[ti][r];
-          if (t0 + i < a.T && dv < a.Dv) st1(vp + (long)(t0 + i) * BH * a.Dv, t0 + i < len ? g[r] : 0.f);
+          const int t = t0 + 16 * ti + 4 * kq + r;
+          p[(16 * ti + r) * Dvp] = u[ti][r];
+          if (t < a.T && dv < a.Dv) st1(vp + (16 * ti + r) * vstep, t < len ? g[r] : 0.f);
         }
       }
     }
-    const float gc = st.gates[64 + C - 1];
+    const float gc = st.gam_last();
 #pragma unroll
     for (int m = 0; m < DKT; ++m) S[m] *= gc;
 #pragma unroll
-    for (int ti = 0; ti < NT; ++ti) {
-      const f4 ga = row4(st.gates + 64 + 16 * ti + 4 * kq);
-      const f4 w = dy[ti] * (a.scale * ga), z = -(u[ti] * ga * row4(st.gates + 16 * ti + 4 * kq));
-      f4 x[DKT];
+    for (int t2 = 0; t2 < NT / 2; ++t2) {
+      Op16<SP> w[2], z[2];
 #pragma unroll
-      for (int m = 0; m < DKT; ++m) x[m] = col4(st.Q + (16 * ti + 4 * kq) * LD + 16 * m + l16, LD);
+      for (int x = 0; x < 2; ++x) {
+        const int ti = 2 * t2 + x;
+        const f4 ga = st.gam(ti);
+        w[x] = cut<SP>(dy[ti] * (a.scale * ga * st.rq4(ti)));
+        z[x] = cut<SP>(-(u[ti] * ga * st.beta(ti) * st.rk4(ti)));
+      }
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int m = 0; m < DKT; ++m) S[m] = mfma4(x[m][j], w[j], S[m]);
-#pragma unroll
-      for (int m = 0; m < DKT; ++m) x[m] = col4(st.K + (16 * ti + 4 * kq) * LD + 16 * m + l16, LD);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int m = 0; m < DKT; ++m) S[m] = mfma4(x[m][j], z[j], S[m]);
+      for (int m = 0; m < DKT; ++m) {
+        S[m] = mm32(st.qt(m, t2), w[0], w[1], S[m]);
+        S[m] = mm32(st.kt(m, t2), z[0], z[1], S[m]);
+      }
     }
   }
   if (!works) return;
@@ -258,7 +248,7 @@ __global__ void __launch_bounds__(64 * DKT) delta_bwd_pair_kernel(Args a, BwdArg
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, kq = lane >> 4, wave = tid >> 6;
   const int BH = a.B * a.Hv, bh = blockIdx.x % BH, n = blockIdx.x / BH, t0 = n * C;
   const int b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
-  const int Dvp = 16 * ((a.Dv + 15) >> 4);
+  const int Dvp = pitch(a.Dv), Dve = 16 * ((a.Dv + 15) >> 4);
   const int len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
   const int Ho = per_value_head ? a.Hv : a.Hk, ho = per_value_head ? h : hk;
   const bool same = per_value_head == 0;  // the outputs have the inputs' type
@@ -282,9 +272,10 @@ __global__ void __launch_bounds__(64 * DKT) delta_bwd_pair_kernel(Args a, BwdArg
     return;
   }
 
-  load_rows<T, DKT, C>(l.K, s.rk, reinterpret_cast<const T*>(a.k) + (long)b * a.kb + (long)hk * a.kh, a.kt, a.Dk, t0, len, a.veck,
+  constexpr int RL = C * 16 / (64 * NW) > 0 ? C * 16 / (64 * NW) : 1;
+  load_rows<T, DKT, C, RL>(l.K, s.rk, reinterpret_cast<const T*>(a.k) + (long)b * a.kb + (long)hk * a.kh, a.kt, a.Dk, t0, len, a.veck,
                        a.normalize, a.eps);
-  load_rows<T, DKT, C>(l.Q, s.rq, reinterpret_cast<const T*>(a.q) + (long)b * a.qb + (long)hk * a.qh, a.qt, a.Dk, t0, len, a.vecq,
+  load_rows<T, DKT, C, RL>(l.Q, s.rq, reinterpret_cast<const T*>(a.q) + (long)b * a.qb + (long)hk * a.qh, a.qt, a.Dk, t0, len, a.vecq,
                        a.normalize, a.eps);
   if (wave == 0) chunk_gates<C>(a, s, b, h, t0, len, lane);
 
@@ -305,13 +296,13 @@ __global__ void __launch_bounds__(64 * DKT) delta_bwd_pair_kernel(Args a, BwdArg
 #pragma unroll
   for (int x = 0; x < RPT; ++x) dRv[x] = 0.f;
 
-  for (int c0 = 0; c0 < Dvp; c0 += DVB) {
+  for (int c0 = 0; c0 < Dve; c0 += DVB) {
 #pragma unroll
     for (int x = 0; x < RPT; ++x) {
       const int at = tid + x * 64 * NW, i = at / (DVB / 4), c = c0 + 4 * (at % (DVB / 4));
       if (i < C) {
         f4 g = zero, r = zero, u = zero;
-        if (c < Dvp) {
+        if (c < Dve) {
           r = row4(rp + i * Dvp + c);
           u = row4(up + i * Dvp + c);
           const int t = t0 + i;
@@ -334,7 +325,7 @@ __global__ void __launch_bounds__(64 * DKT) delta_bwd_pair_kernel(Args a, BwdArg
 #pragma unroll
     for (int m = 0; m < DVB / 16; ++m) {
       const int c = c0 + 16 * m;
-      if (c < Dvp) {
+      if (c < Dve) {
         const f4 x = row4(s0 + c + 4 * kq), y = row4(ds + c + 4 * kq);
 #pragma unroll
         for (int j = 0; j < 4; ++j) sdot = fmaf(x[j], y[j], sdot);
@@ -554,7 +545,7 @@ __global__ void delta_head_sum_kernel(const float* x, T* y, long n, int rep, int
 
 template <typename T, int DKT, int NWT, bool MAP>
 static void launch_walk(const Args& a, const BwdArgs& o, hipStream_t st) {
-  const int lds = Stage<T, DKT, NWT, true>::FLOATS * (int)sizeof(float);
+  const int lds = Stage<T, DKT, NWT, 2>::BYTES;
   allow_lds<delta_bwd_walk_kernel<T, DKT, NWT, MAP>>(lds);
   delta_bwd_walk_kernel<T, DKT, NWT, MAP><<<a.B * a.Hv * a.nseg, 64 * NWT, lds, st>>>(a, o);
 }

@@ -27,16 +27,19 @@ __global__ void __launch_bounds__(512) delta_short_kernel(Args a, FwdOut o) {
 
   const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
   const int BH = a.B * a.Hv, bh = blockIdx.x, b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
-  const int Dvp = 16 * ((a.Dv + 15) >> 4), dv = 16 * wave + l16;
+  const int Dvp = pitch(a.Dv), dv = 16 * wave + l16;
   const int len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
   const T* qp = reinterpret_cast<const T*>(a.q) + (long)b * a.qb + (long)hk * a.qh;
   const T* kp = reinterpret_cast<const T*>(a.k) + (long)b * a.kb + (long)hk * a.kh;
   const T* vp = reinterpret_cast<const T*>(a.v) + (long)b * a.vb + (long)h * a.vh;
 
-  load_rows<T, DKT, C>(K, s.rk, kp, a.kt, a.Dk, 0, len, a.veck, a.normalize, a.eps);
-  load_rows<T, DKT, C>(Q, s.rq, qp, a.qt, a.Dk, 0, len, a.vecq, a.normalize, a.eps);
+  // a sequence of no steps reads its first one, which is there, and counts none of it
+  Column<T, 1> vc;
+  vc.fetch(vp + min(dv, a.Dv - 1), a.vt, 0, max(len, 1), kq);
+  load_rows<T, DKT, C, 4>(K, s.rk, kp, a.kt, a.Dk, 0, len, a.veck, a.normalize, a.eps);
+  load_rows<T, DKT, C, 4>(Q, s.rq, qp, a.qt, a.Dk, 0, len, a.vecq, a.normalize, a.eps);
   if (wave == 0) chunk_gates<C>(a, s, b, h, 0, len, lane);
-  f4 S[DKT], v;
+  f4 S[DKT];
 #pragma unroll
   for (int m = 0; m < DKT; ++m)
 #pragma unroll
@@ -45,9 +48,8 @@ __global__ void __launch_bounds__(512) delta_short_kernel(Args a, FwdOut o) {
       S[m][r] = (a.state && d < a.Dk && dv < a.Dv) ? a.state[((long)bh * a.Dk + d) * a.Dv + dv] : 0.f;
       if (o.Sc) o.Sc[((long)bh * DKp + d) * Dvp + dv] = S[m][r];
     }
-#pragma unroll
-  for (int r = 0; r < 4; ++r) v[r] = (4 * kq + r < len && dv < a.Dv) ? ld1(vp + (long)(4 * kq + r) * a.vt + dv) : 0.f;
   lds_barrier();
+  const f4 v = vc.get(0, 0, len, kq, dv < a.Dv);
   pair_tiles<DKT, C>(K, Q, A, P, s, a.scale, wave, nw);
   f4 u = {0.f, 0.f, 0.f, 0.f}, y = u;
 #pragma unroll
@@ -97,9 +99,9 @@ __global__ void __launch_bounds__(256) delta_pairs_kernel(Args a, float* pairs) 
   if (t0 >= len) return;
   float* out = pairs + ((long)bh * a.N + n) * PAIR_FLOATS;
   if (wave == 3) chunk_gates<C>(a, s, b, h, t0, len, lane);
-  load_rows<T, DKT, C>(K, s.rk, reinterpret_cast<const T*>(a.k) + (long)b * a.kb + (long)hk * a.kh, a.kt, a.Dk, t0, len, a.veck,
+  load_rows<T, DKT, C, 4>(K, s.rk, reinterpret_cast<const T*>(a.k) + (long)b * a.kb + (long)hk * a.kh, a.kt, a.Dk, t0, len, a.veck,
                        a.normalize, a.eps);
-  load_rows<T, DKT, C>(Q, s.rq, reinterpret_cast<const T*>(a.q) + (long)b * a.qb + (long)hk * a.qh, a.qt, a.Dk, t0, len, a.vecq,
+  load_rows<T, DKT, C, 4>(Q, s.rq, reinterpret_cast<const T*>(a.q) + (long)b * a.qb + (long)hk * a.qh, a.qt, a.Dk, t0, len, a.vecq,
                        a.normalize, a.eps);
   lds_barrier();
   // the diagonal tiles first: their inverses follow while the others are still made
@@ -159,15 +161,16 @@ __global__ void __launch_bounds__(256) delta_pairs_kernel(Args a, float* pairs) 
 
 template <typename T, int DKT, int NWT, bool MAP>
 __global__ void __launch_bounds__(64 * NWT) delta_walk_kernel(Args a, FwdOut o) {
-  using St = Stage<T, DKT, NWT, !MAP>;
-  constexpr int C = 64, LD = St::LD, NT = 4, DKp = 16 * DKT;
-  extern __shared__ __align__(16) float flds[];
-  St st(flds);
+  using St = Stage<T, DKT, NWT, MAP ? 1 : 0>;
+  constexpr bool SP = St::SP;
+  constexpr int C = 64, NT = 4, DKp = 16 * DKT, Dvp = NWT == 4 ? 64 : 128;
+  extern __shared__ __align__(16) unsigned char lds[];
+  St st(lds);
 
   const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4, wave = threadIdx.x >> 6;
   const int BH = a.B * a.Hv, bh = blockIdx.x % BH, seg = blockIdx.x / BH;
   const int b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
-  const int nvs = (a.Dv + 15) >> 4, Dvp = 16 * nvs;
+  const int nvs = (a.Dv + 15) >> 4;
   const int len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
   const bool vstrip = wave < nvs, works = wave < nvs + (MAP ? DKT : 0);  // the other waves only move operands
   const int dv = 16 * (vstrip ? wave : wave - nvs) + l16;
@@ -176,7 +179,7 @@ __global__ void __launch_bounds__(64 * NWT) delta_walk_kernel(Args a, FwdOut o) 
   const T* vp = reinterpret_cast<const T*>(a.v) + (long)b * a.vb + (long)h * a.vh;
   const float* pairs = o.pairs + (long)bh * a.N * PAIR_FLOATS;
 
-  f4 S[DKT], v[NT];
+  f4 S[DKT];
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int m = 0; m < DKT; ++m) S[m] = zero;
@@ -200,113 +203,85 @@ __global__ void __launch_bounds__(64 * NWT) delta_walk_kernel(Args a, FwdOut o) 
         if (d < a.Dk && dv < a.Dv) S[m][r] = a.state[((long)bh * a.Dk + d) * a.Dv + dv];
       }
   }
-  auto load_v = [&](int t0) {
-#pragma unroll
-    for (int ti = 0; ti < NT; ++ti)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int t = t0 + 16 * ti + 4 * kq + r;
-        v[ti][r] = (vstrip && t < len && dv < a.Dv) ? ld1(vp + (long)t * a.vt + dv) : 0.f;
-      }
-  };
-
+  Column<T, NT> v;
+  const T* vcol = vp + min(dv, a.Dv - 1);
   const int n0 = seg * a.cps, n1 = min(a.N, n0 + a.cps), live = min(n1, (len + C - 1) / C);
   if (n0 < live) {
     st.fetch(a, qp, kp, pairs + (long)n0 * PAIR_FLOATS, n0 * C, len);
-    load_v(n0 * C);
+    v.fetch(vcol, a.vt, n0 * C, len, kq);
   }
   for (int n = n0; n < live; ++n) {
     const int t0 = n * C;
     if (!MAP && o.Sc && works) {
-      float* p = o.Sc + ((long)bh * a.N + n) * DKp * Dvp + dv;
+      float* p = o.Sc + ((long)bh * a.N + n) * DKp * Dvp + 4 * kq * Dvp + dv;
 #pragma unroll
       for (int m = 0; m < DKT; ++m)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) p[(16 * m + 4 * kq + r) * Dvp] = S[m][r];
+        for (int r = 0; r < 4; ++r) p[(16 * m + r) * Dvp] = S[m][r];
     }
     lds_barrier();  // the chunk before is done with LDS
-    st.commit();
+    st.commit(t0, len, a.Dk);
     lds_barrier();
     f4 u[NT];
 #pragma unroll
-    for (int ti = 0; ti < NT; ++ti) u[ti] = row4(st.gates + 16 * ti + 4 * kq) * v[ti];
+    for (int ti = 0; ti < NT; ++ti) u[ti] = st.beta(ti) * v.get(ti, t0, len, kq, vstrip && dv < a.Dv);
     if (n + 1 < live) {
       st.fetch(a, qp, kp, pairs + (long)(n + 1) * PAIR_FLOATS, t0 + C, len);
-      load_v(t0 + C);
+      v.fetch(vcol, a.vt, t0 + C, len, kq);
     }
     if (!works) continue;
-    // beta (V - gam K S0)
-    f4 x4[NT];
+    // K S0 and Q S0
+    f4 ks[NT], y[NT];
 #pragma unroll
-    for (int ti = 0; ti < NT; ++ti) x4[ti] = zero;
+    for (int ti = 0; ti < NT; ++ti) ks[ti] = y[ti] = zero;
 #pragma unroll
-    for (int m = 0; m < DKT; ++m) {
-      f4 x[NT];
+    for (int m2 = 0; m2 < DKT / 2; ++m2) {
+      const Op16<SP> s0 = cut<SP>(S[2 * m2]), s1 = cut<SP>(S[2 * m2 + 1]);
 #pragma unroll
-      for (int ti = 0; ti < NT; ++ti) x[ti] = row4(st.K + (16 * ti + l16) * LD + 16 * m + 4 * kq);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int ti = 0; ti < NT; ++ti) x4[ti] = mfma4(x[ti][j], S[m][j], x4[ti]);
+      for (int ti = 0; ti < NT; ++ti) {
+        ks[ti] = mm32(st.k(ti, m2), s0, s1, ks[ti]);
+        if constexpr (!MAP) y[ti] = mm32(st.q(ti, m2), s0, s1, y[ti]);
+      }
     }
-#pragma unroll
-    for (int ti = 0; ti < NT; ++ti) u[ti] -= row4(st.gates + 16 * ti + 4 * kq) * row4(st.gates + 64 + 16 * ti + 4 * kq) * x4[ti];
     // U: forward substitution by blocks of 16 steps
-#pragma unroll
-    for (int ti = 0; ti < NT; ++ti) {
-      f4 r = u[ti];
-#pragma unroll
-      for (int tc = 0; tc < ti; ++tc) r = mm16(-row4(st.A(ti, tc) + l16 * TL + 4 * kq), u[tc], r);
-      u[ti] = mm16(row4(st.Ti(ti) + l16 * TL + 4 * kq), r, zero);
-    }
-    if (!MAP) {
+    Op16<SP> ub[NT];
+    each<0, NT>([&](auto I) {
+      constexpr int ti = I;
+      f4 r = u[ti] - st.beta(ti) * st.gam(ti) * st.rk4(ti) * ks[ti];
+      r = mm_tiles<0, ti>([&](int x) { return st.A(ti, x); }, [&](auto x) { return ub[decltype(x)::value]; }, r);
+      u[ti] = mm16o(st.Ti(ti), cut<SP>(r), zero);
+      ub[ti] = cut<SP>(u[ti]);
+    });
+    if constexpr (!MAP) {
       if (o.U) {
-        float* p = o.U + ((long)bh * a.N + n) * C * Dvp + dv;
+        float* p = o.U + ((long)bh * a.N + n) * C * Dvp + 4 * kq * Dvp + dv;
 #pragma unroll
         for (int ti = 0; ti < NT; ++ti)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) p[(16 * ti + 4 * kq + r) * Dvp] = u[ti][r];
+          for (int r = 0; r < 4; ++r) p[(16 * ti + r) * Dvp] = u[ti][r];
       }
-      f4 y[NT];
-#pragma unroll
-      for (int ti = 0; ti < NT; ++ti) y[ti] = zero;
-#pragma unroll
-      for (int m = 0; m < DKT; ++m) {
-        f4 x[NT];
-#pragma unroll
-        for (int ti = 0; ti < NT; ++ti) x[ti] = row4(st.Q + (16 * ti + l16) * LD + 16 * m + 4 * kq);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int ti = 0; ti < NT; ++ti) y[ti] = mfma4(x[ti][j], S[m][j], y[ti]);
-      }
-      T* op = reinterpret_cast<T*>(o.out) + (long)bh * a.Dv + dv;
-#pragma unroll
-      for (int ti = 0; ti < NT; ++ti) {
-        f4 w = y[ti] * (a.scale * row4(st.gates + 64 + 16 * ti + 4 * kq));
-#pragma unroll
-        for (int tj = 0; tj <= ti; ++tj) w = mm16(row4(st.P(ti, tj) + l16 * TL + 4 * kq), u[tj], w);
+      const long ostep = afresh((long)BH * a.Dv);
+      T* op = reinterpret_cast<T*>(o.out) + (long)bh * a.Dv + dv + (t0 + 4 * kq) * ostep;
+      each<0, NT>([&](auto I) {
+        constexpr int ti = I;
+        const f4 w = mm_tiles<0, ti + 1>([&](int x) { return st.P(ti, x); }, [&](auto x) { return ub[decltype(x)::value]; },
+                                         y[ti] * (a.scale * st.gam(ti) * st.rq4(ti)));
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int t = t0 + 16 * ti + 4 * kq + r;
-          if (t < a.T && dv < a.Dv) st1(op + (long)t * BH * a.Dv, t < len ? w[r] : 0.f);
+          if (t < a.T && dv < a.Dv) st1(op + (16 * ti + r) * ostep, t < len ? w[r] : 0.f);
         }
-      }
+      });
     }
     // S' = gam_C S + K^T diag(e) U
-    const float gc = st.gates[64 + C - 1];
+    const float gc = st.gam_last();
 #pragma unroll
     for (int m = 0; m < DKT; ++m) S[m] *= gc;
 #pragma unroll
-    for (int ti = 0; ti < NT; ++ti) {
-      const f4 w = u[ti] * row4(st.gates + 128 + 16 * ti + 4 * kq);
-      f4 x[DKT];
+    for (int t2 = 0; t2 < NT / 2; ++t2) {
+      const Op16<SP> w0 = cut<SP>(u[2 * t2] * st.e(2 * t2) * st.rk4(2 * t2)), w1 = cut<SP>(u[2 * t2 + 1] * st.e(2 * t2 + 1) * st.rk4(2 * t2 + 1));
 #pragma unroll
-      for (int m = 0; m < DKT; ++m) x[m] = col4(st.K + (16 * ti + 4 * kq) * LD + 16 * m + l16, LD);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int m = 0; m < DKT; ++m) S[m] = mfma4(x[m][j], w[j], S[m]);
+      for (int m = 0; m < DKT; ++m) S[m] = mm32(st.kt(m, t2), w0, w1, S[m]);
     }
   }
   if (!works) return;
@@ -382,7 +357,7 @@ __global__ void __launch_bounds__(64 * DKT) delta_scan_kernel(const float* first
 
 template <typename T, int DKT, int NWT, bool MAP>
 static void launch_walk(const Args& a, const FwdOut& o, hipStream_t st) {
-  const int lds = Stage<T, DKT, NWT, !MAP>::FLOATS * (int)sizeof(float);
+  const int lds = Stage<T, DKT, NWT, MAP ? 1 : 0>::BYTES;
   allow_lds<delta_walk_kernel<T, DKT, NWT, MAP>>(lds);
   delta_walk_kernel<T, DKT, NWT, MAP><<<a.B * a.Hv * a.nseg, 64 * NWT, lds, st>>>(a, o);
 }
