@@ -327,6 +327,21 @@ __device__ __forceinline__ f4 mm32(const Exact32<true>& a, const Op16<true>& b0,
   c = mfma32(x, join(b0.p0, b1.p0), c);
   return c;
 }
+// the exact operand on the right
+__device__ __forceinline__ f4 mm32r(const Op16<false>& a0, const Op16<false>& a1, const Exact32<false>& b, f4 c) {
+  return mm16(a1.x, b.b, mm16(a0.x, b.a, c));
+}
+__device__ __forceinline__ f4 mm32r(const Op16<true>& a0, const Op16<true>& a1, const Exact32<true>& b, f4 c) {
+  const b8 x = __builtin_bit_cast(b8, b.x);
+  c = mfma32(join(a0.p2, a1.p2), x, c);
+  c = mfma32(join(a0.p1, a1.p1), x, c);
+  c = mfma32(join(a0.p0, a1.p0), x, c);
+  return c;
+}
+__device__ __forceinline__ f4 mm32x(const Exact32<false>& a, const Exact32<false>& b, f4 c) { return mm16(a.b, b.b, mm16(a.a, b.a, c)); }
+__device__ __forceinline__ f4 mm32x(const Exact32<true>& a, const Exact32<true>& b, f4 c) {
+  return mfma32(__builtin_bit_cast(b8, a.x), __builtin_bit_cast(b8, b.x), c);
+}
 // two cut operands over 32 indexes, and over 16
 __device__ __forceinline__ f4 mm32(const Op16<false>& a0, const Op16<false>& a1, const Op16<false>& b0, const Op16<false>& b1, f4 c) {
   return mm16(a1.x, b1.x, mm16(a0.x, b0.x, c));
@@ -359,7 +374,8 @@ __device__ __forceinline__ f4 mm16o(const Op16<true>& a, const Op16<true>& b, f4
 
 // A chunk of 64 steps on its way from memory to LDS for the strip kernels: K (and Q) as they lie in memory, the pair tiles,
 // the gates.  fetch() starts the reads for the next chunk, commit() writes what has arrived to LDS: the reads have the whole
-// walk over the present chunk to arrive in.  MODE: 0 forward, 1 forward without Q and P (maps), 2 backward.
+// walk over the present chunk to arrive in.  MODE: 0 forward, 1 forward without Q and P (maps), 2 backward,
+// 3 without the tiles (gradients of q and k).
 // What the kernels read: k(ti, m2), q(ti, m2): rows of steps against 32 key columns; kt(m, t2), qt(m, t2): rows of key columns
 // against 32 steps; A (negated), P, Ti: tiles, transposed in the backward mode; rk4, rq4: factors that are not in k and q yet.
 constexpr int TS = 320, TL = 20;  // a fp32 tile in LDS: 16 rows of 20: reads of rows and of columns are free of bank conflicts
@@ -368,7 +384,7 @@ struct Stage;
 
 template <int MODE>
 struct TileIndex {
-  static constexpr int N = MODE == 1 ? 14 : 24;
+  static constexpr int N = MODE == 3 ? 0 : MODE == 1 ? 14 : 24;
   static __device__ __forceinline__ int A(int ti, int tj) { return ti * (ti + 1) / 2 + tj; }
   static __device__ __forceinline__ int P(int ti, int tj) { return 10 + ti * (ti + 1) / 2 + tj; }
   static __device__ __forceinline__ int Ti(int ti) { return (MODE == 1 ? 10 : 20) + ti; }
@@ -380,11 +396,11 @@ struct Stage<float, DKT, NWT, MODE> {
   using TI = TileIndex<MODE>;
   static constexpr bool SP = false, HQ = MODE != 1;
   static constexpr int LD = 16 * DKT + 4, NE = DKT, RR = 16 / NWT, TH = 64 * NWT, NT4 = (TI::N * 64 + TH - 1) / TH;
-  static constexpr int BYTES = 4 * ((HQ ? 2 : 1) * 64 * LD + TI::N * TS + 3 * 64);
-  float *K, *Q, *tile, *gates;  // gates: beta, gam, e
+  static constexpr int BYTES = 4 * ((HQ ? 2 : 1) * 64 * LD + TI::N * TS + 5 * 64);
+  float *K, *Q, *tile, *gates;  // gates: beta, gam, e, rq, rk
   float rk_[RR][NE], rq_[HQ ? RR : 1][NE];
   float nk[RR], nq[RR];
-  f4 tl[NT4], ga;
+  f4 tl[NT4 > 0 ? NT4 : 1], ga;
   int l16, kq;
 
   __device__ __forceinline__ explicit Stage(void* lds)
@@ -416,6 +432,9 @@ struct Stage<float, DKT, NWT, MODE> {
   __device__ __forceinline__ f4 rk4(int) const { return f4{1.f, 1.f, 1.f, 1.f}; }
   __device__ __forceinline__ f4 rq4(int) const { return f4{1.f, 1.f, 1.f, 1.f}; }
 
+  // four key columns from c on of step i, scaled to unit length
+  __device__ __forceinline__ f4 k_of(int i, int c) const { return row4(K + i * LD + c); }
+  __device__ __forceinline__ f4 q_of(int i, int c) const { return row4(Q + i * LD + c); }
   __device__ __forceinline__ void rows_(float (*w)[NE], const float* src, long st, int D, int t0, int len, bool vec) {
     const int c0 = (threadIdx.x & 15) * NE;
     const float* p[RR];
@@ -445,7 +464,7 @@ struct Stage<float, DKT, NWT, MODE> {
       const int at = min((int)threadIdx.x + x * TH, TI::N * 64 - 1);  // 16 bytes each
       tl[x] = row4(pair + 256 * TI::source(at >> 6) + 4 * (at & 63));
     }
-    ga = row4(pair + PAIR_TILES * 256 + 4 * min((int)threadIdx.x, 47));
+    ga = row4(pair + PAIR_TILES * 256 + 4 * min((int)threadIdx.x, 79));
   }
   __device__ __forceinline__ void commit(int t0, int len, int D) {
     const int c0 = (threadIdx.x & 15) * NE;
@@ -464,7 +483,7 @@ struct Stage<float, DKT, NWT, MODE> {
       const int at = threadIdx.x + x * TH;
       if (at < TI::N * 64) *reinterpret_cast<f4*>(tile + (at >> 6) * TS + ((at >> 2) & 15) * TL + 4 * (at & 3)) = (at >> 6) < 10 ? -tl[x] : tl[x];
     }
-    if (threadIdx.x < 48) *reinterpret_cast<f4*>(gates + 4 * threadIdx.x) = ga;
+    if (threadIdx.x < 80) *reinterpret_cast<f4*>(gates + 4 * threadIdx.x) = ga;
   }
 };
 
@@ -474,7 +493,7 @@ __device__ __forceinline__ int place(int c) { return (c & ~31) | ((c & 12) << 1)
 template <int DKT, int NWT, int MODE>
 struct Stage<bf16, DKT, NWT, MODE> {
   using TI = TileIndex<MODE>;
-  static constexpr bool SP = true, HQ = MODE != 1, QT = MODE == 2;
+  static constexpr bool SP = true, HQ = MODE != 1, QT = MODE >= 2;
   static constexpr int LR = 16 * DKT + 8, LC = 64 + 8, TH = 64 * NWT, NT4 = (TI::N * 64 + TH - 1) / TH;
   static constexpr int CP = 8 * DKT, RG = TH / CP < 16 ? TH / CP : 16, NG = 16 / RG;  // pairs of columns, groups of four rows at once, of a thread
   static constexpr int ROWS = 64 * LR, COLS = 16 * DKT * LC;
@@ -483,7 +502,7 @@ struct Stage<bf16, DKT, NWT, MODE> {
   u2* tile;   // [tile][part][lane]
   float* gates;  // beta, gam, e, rq, rk
   uint32_t rk_[NG][4], rq_[HQ ? NG : 1][4];
-  f4 tl[NT4], ga;
+  f4 tl[NT4 > 0 ? NT4 : 1], ga;
   int l16, kq;
 
   __device__ __forceinline__ explicit Stage(void* lds)
@@ -513,6 +532,17 @@ struct Stage<bf16, DKT, NWT, MODE> {
   __device__ __forceinline__ f4 rq4(int ti) const { return row4(gates + 192 + 16 * ti + 4 * kq); }
   __device__ __forceinline__ f4 rk4(int ti) const { return row4(gates + 256 + 16 * ti + 4 * kq); }
 
+  __device__ __forceinline__ f4 k_of(int i, int c) const {
+    const u2 w = *reinterpret_cast<const u2*>(Kr + i * LR + place(c));
+    const float n = gates[256 + i];
+    return f4{n * __builtin_bit_cast(float, w.x << 16), n * __builtin_bit_cast(float, w.x & 0xffff0000u), n * __builtin_bit_cast(float, w.y << 16),
+              n * __builtin_bit_cast(float, w.y & 0xffff0000u)};
+  }
+  __device__ __forceinline__ f4 q_of(int i, int c) const {  // Qx holds columns
+    const uint16_t* p = Qx + c * LC + place(i);
+    const float n = gates[192 + i];
+    return f4{n * bf2f(p[0]), n * bf2f(p[LC]), n * bf2f(p[2 * LC]), n * bf2f(p[3 * LC])};
+  }
   __device__ __forceinline__ void rows4(uint32_t (*w)[4], const bf16* src, long st, int D, int t0, int len, bool vec) {
     const int c = 2 * (threadIdx.x % CP), i0 = 4 * (threadIdx.x / CP < 16 ? threadIdx.x / CP : 0);
     const bf16* p[NG][4];

@@ -42,6 +42,7 @@ struct FwdOut {
 struct BwdArgs {
   const void* dout;  // [T, B, Hv, Dv] by strides, or null
   long ot, ob, oh;
+  int vecv, vecg;  // v and dout can be read four at a time
   const float* dlast;  // [B, Hv, Dk, Dv] contiguous, or null
   const float *Sc, *U, *Pseg, *pairs;
   float* dSc;   // [BH, N, DKp, Dvp] gradient of each chunk's last state

@@ -244,6 +244,14 @@ struct GatedDeltaFn : public torch::autograd::Function<GatedDeltaFn> {
       dlast = dlast.contiguous();
       o.dlast = dlast.data_ptr<float>();
     }
+    auto fours = [&](const Tensor& t) {
+      const int64_t e = t.element_size(), m = 4 * e;
+      bool ok = a.Dv % 4 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % m == 0;
+      for (int i = 0; i < 3; ++i) ok = ok && t.stride(i) * e % m == 0;
+      return ok;
+    };
+    o.vecv = fours(v);
+    o.vecg = dout.defined() ? fours(dout) : o.vecv;
     const DeltaSaved at(a, C);
     TORCH_CHECK(s[7].numel() == at.n, "gated_delta: the plan changed between the passes");
     const float* sp = s[7].data_ptr<float>();

@@ -5,7 +5,7 @@
 //   dS0 = gam_C dS + scale Q^T diag(gam) dO - K^T diag(beta gam) dR:
 // again nothing mixes the value columns, so delta_bwd_walk_kernel walks the chunks backwards with one wave a strip of 16
 // of them, dS in registers, split into segments over a long axis as the forward walk is (the map of dS over a segment
-// is the transpose of Pseg).  What sums over the value columns is left to delta_bwd_pair_kernel, one workgroup a chunk
+// is the transpose of Pseg).  What sums over the value columns is left to delta_grads_kernel, one workgroup a chunk
 // and no order among them:
 //   W1 = M o tril(dO U^T),  W2 = -diag(beta) M o tril(dR U^T, -1),  GO = dO S0^T, GR = dR S0^T, GU = U dS^T,
 //   dQ = scale (diag(gam) GO + W1 K),
@@ -226,6 +226,24 @@ __global__ void __launch_bounds__(64 * NWT) delta_bwd_walk_kernel(Args a, BwdArg
 
 constexpr int DVB = 32;  // value columns staged at once
 
+// One wave, lane i the chunk's step i: the sum of dG over the steps from i to the end of its segment, as suffix sums less
+// that of the next segment's first step.
+template <int C>
+__device__ __forceinline__ float segment_suffix(const Gates<C>& s, double dG, int i) {
+  double suf = dG;
+#pragma unroll
+  for (int x = 1; x < C; x <<= 1) {
+    const double y = __shfl_down(suf, x, 64);
+    if (i + x < C) suf += y;
+  }
+  const unsigned long long starts = __ballot(i < C && i > 0 && s.seg[i < C ? i : 0] != s.seg[i > 0 && i < C ? i - 1 : 0]);
+  const unsigned long long later = i < 63 ? starts >> (i + 1) : 0ull;
+  const int nx = later ? i + __ffsll((long long)later) : i;
+  const double beyond = __shfl(suf, nx, 64);
+  return (float)(suf - (later ? beyond : 0.0));
+}
+
+// Chunks of 16 (whole sequences): what sums over the value columns, one wave per 16 key columns.
 template <int DKT, int C>
 struct PairLds {
   static constexpr int LD = 16 * DKT + 4, LC = C + 4, LV = DVB + 4, NT = C / 16, NTL = NT * (NT + 1) / 2;
@@ -513,20 +531,388 @@ __global__ void __launch_bounds__(64 * DKT) delta_bwd_pair_kernel(Args a, BwdArg
       for (int w = 0; w < NW; ++w) sd += l.sd[w];
       dG += (double)(sumF + s.gam[C - 1] * sd);
     }
-    // sums over the steps from i to the end of the segment: suffix sums, less that of the next segment's first step
-    double suf = dG;
-#pragma unroll
-    for (int x = 1; x < C; x <<= 1) {
-      const double y = __shfl_down(suf, x, 64);
-      if (i + x < C) suf += y;
-    }
-    const unsigned long long starts = __ballot(i < C && i > 0 && s.seg[i < C ? i : 0] != s.seg[i > 0 && i < C ? i - 1 : 0]);
-    const unsigned long long later = i < 63 ? starts >> (i + 1) : 0ull;
-    const int nx = later ? i + __ffsll((long long)later) : i;
-    const double beyond = __shfl(suf, nx, 64);
-    const double g = suf - (later ? beyond : 0.0);
+    const float g = segment_suffix<C>(s, dG, i);
     if (i < C && t0 + i < a.T) {
-      o.dg[(long)(t0 + i) * BH + bh] = s.rst[i] ? 0.f : (float)g;
+      o.dg[(long)(t0 + i) * BH + bh] = s.rst[i] ? 0.f : g;
+      o.db[(long)(t0 + i) * BH + bh] = t0 + i < len ? db : 0.f;
+    }
+  }
+}
+
+// Value columns of U, dR and dO on their way to LDS, DVB at a time: [64][DVB], for operands over all of them at once.
+template <typename T, int TH>
+struct Values;
+
+template <int TH>
+struct Values<float, TH> {
+  static constexpr int LV = DVB + 4, BYTES = 3 * 64 * LV * 4;
+  float *O, *R, *U;
+  __device__ __forceinline__ explicit Values(void* lds) : O((float*)lds), R(O + 64 * LV), U(R + 64 * LV) {}
+  __device__ __forceinline__ void put(int i, int c, f4 g, f4 r, f4 u) {
+    *reinterpret_cast<f4*>(O + i * LV + c) = g;
+    *reinterpret_cast<f4*>(R + i * LV + c) = r;
+    *reinterpret_cast<f4*>(U + i * LV + c) = u;
+  }
+  struct Cut {
+    Op16<false> a, b;
+  };
+  static __device__ __forceinline__ Cut at(const float* M, int t, int l16, int kq) {
+    const float* p = M + (16 * t + l16) * LV + 4 * kq;
+    return {{row4(p)}, {row4(p + 16)}};
+  }
+  __device__ __forceinline__ Cut r(int t, int l16, int kq) const { return at(R, t, l16, kq); }
+  __device__ __forceinline__ Cut u(int t, int l16, int kq) const { return at(U, t, l16, kq); }
+  __device__ __forceinline__ Exact32<false> o(int t, int l16, int kq) const {
+    const float* p = O + (16 * t + l16) * LV + 4 * kq;
+    return {row4(p), row4(p + 16)};
+  }
+};
+
+template <int TH>
+struct Values<bf16, TH> {
+  static constexpr int LV = DVB + 8, PL = 64 * LV, BYTES = 7 * PL * 2;
+  uint16_t *O, *R, *U;  // R and U in three parts
+  __device__ __forceinline__ explicit Values(void* lds) : O((uint16_t*)lds), R(O + PL), U(R + 3 * PL) {}
+  __device__ __forceinline__ void put(int i, int c, f4 g, f4 r, f4 u) {
+    const int w = i * LV + place(c);
+    *reinterpret_cast<u2*>(O + w) = part(g);
+    const Op16<true> x = cut3(r), y = cut3(u);
+    *reinterpret_cast<u2*>(R + w) = x.p0;
+    *reinterpret_cast<u2*>(R + PL + w) = x.p1;
+    *reinterpret_cast<u2*>(R + 2 * PL + w) = x.p2;
+    *reinterpret_cast<u2*>(U + w) = y.p0;
+    *reinterpret_cast<u2*>(U + PL + w) = y.p1;
+    *reinterpret_cast<u2*>(U + 2 * PL + w) = y.p2;
+  }
+  struct Cut {
+    Op16<true> a, b;
+  };
+  static __device__ __forceinline__ Cut at(const uint16_t* M, int t, int l16, int kq) {
+    const uint16_t* p = M + (16 * t + l16) * LV + 8 * kq;
+    const u4 x = *reinterpret_cast<const u4*>(p), y = *reinterpret_cast<const u4*>(p + PL), z = *reinterpret_cast<const u4*>(p + 2 * PL);
+    return {{x.xy, y.xy, z.xy}, {x.zw, y.zw, z.zw}};
+  }
+  __device__ __forceinline__ Cut r(int t, int l16, int kq) const { return at(R, t, l16, kq); }
+  __device__ __forceinline__ Cut u(int t, int l16, int kq) const { return at(U, t, l16, kq); }
+  __device__ __forceinline__ Exact32<true> o(int t, int l16, int kq) const {
+    return {*reinterpret_cast<const u4*>(O + (16 * t + l16) * LV + 8 * kq)};
+  }
+};
+
+// four neighbours of a row of D that is read in whole fours (vec) or by its elements
+__device__ __forceinline__ f4 four(const float* p, int c, int D, bool vec) {
+  if (vec) return row4(p + min(c, D - 4));
+  return f4{p[min(c, D - 1)], p[min(c + 1, D - 1)], p[min(c + 2, D - 1)], p[min(c + 3, D - 1)]};
+}
+__device__ __forceinline__ f4 four(const bf16* p, int c, int D, bool vec) {
+  if (vec) {
+    const u2 w = *reinterpret_cast<const u2*>(p + min(c, D - 4));
+    return f4{__builtin_bit_cast(float, w.x << 16), __builtin_bit_cast(float, w.x & 0xffff0000u), __builtin_bit_cast(float, w.y << 16),
+              __builtin_bit_cast(float, w.y & 0xffff0000u)};
+  }
+  return f4{ld1(p + min(c, D - 1)), ld1(p + min(c + 1, D - 1)), ld1(p + min(c + 2, D - 1)), ld1(p + min(c + 3, D - 1))};
+}
+
+template <typename T, int DKT>
+struct GradsLds {
+  static constexpr int NTL = 10, W = 2 * NTL * TS * 4, V = Values<T, 64 * DKT>::BYTES, BIG = W > V ? W : V;
+  Gates<64> s;
+  float rows[NTL][16], cols[NTL][16], rowb[NTL][16], dots[5][DKT][64], dRv[64], sd[DKT];
+  __align__(16) unsigned char big[BIG], stage[Stage<T, DKT, DKT, 3>::BYTES];
+};
+
+// Chunks of 64: what sums over the value columns (the head of this file), one wave per 16 key columns.
+template <typename T, int DKT>
+__global__ void __launch_bounds__(64 * DKT) delta_grads_kernel(Args a, BwdArgs o, int per_value_head) {
+  using L = GradsLds<T, DKT>;
+  using St = Stage<T, DKT, DKT, 3>;
+  constexpr bool SP = St::SP;
+  constexpr int C = 64, NT = 4, NTL = 10, DKp = 16 * DKT, NW = DKT, TH = 64 * NW;
+  constexpr int TPW = (NTL + NW - 1) / NW, RPT = C * (DVB / 4) / TH;
+  extern __shared__ __align__(16) unsigned char lds[];
+  L& l = *reinterpret_cast<L*>(lds);
+  Gates<C>& s = l.s;
+  St st(l.stage);
+  Values<T, TH> val(l.big);
+  float *W1 = reinterpret_cast<float*>(l.big), *W2 = W1 + NTL * TS;
+
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, kq = lane >> 4, wave = tid >> 6;
+  const int BH = a.B * a.Hv, bh = blockIdx.x % BH, n = blockIdx.x / BH, t0 = n * C;
+  const int b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
+  const int Dvp = pitch(a.Dv), Dve = 16 * ((a.Dv + 15) >> 4);
+  const int len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
+  const int Ho = per_value_head ? a.Hv : a.Hk, ho = per_value_head ? h : hk;
+  const bool same = per_value_head == 0;  // the outputs have the inputs' type
+
+  auto put = [&](void* base, int i, int d, f4 v) {
+    const long at = (((long)(t0 + i) * a.B + b) * Ho + ho) * a.Dk + d;
+    if (a.Dk % 4 == 0) {
+      if (!same || sizeof(T) == 4) *reinterpret_cast<f4*>(reinterpret_cast<float*>(base) + at) = v;
+      else *reinterpret_cast<u2*>(reinterpret_cast<T*>(base) + at) = part(v);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (d + r >= a.Dk) break;
+        if (same) st1(reinterpret_cast<T*>(base) + at + r, v[r]);
+        else reinterpret_cast<float*>(base)[at + r] = v[r];
+      }
+    }
+  };
+  const f4 zero = {0.f, 0.f, 0.f, 0.f};
+
+  if (t0 >= len) {
+    const int m = min(C, a.T - t0), q4 = (a.Dk + 3) / 4;
+    for (int x = tid; x < m * q4; x += TH) {
+      put(o.dq, x / q4, 4 * (x % q4), zero);
+      put(o.dk, x / q4, 4 * (x % q4), zero);
+    }
+    if (tid < m) {
+      o.dg[(long)(t0 + tid) * BH + bh] = 0.f;
+      o.db[(long)(t0 + tid) * BH + bh] = 0.f;
+    }
+    return;
+  }
+
+  const float* pair = o.pairs + ((long)bh * a.N + n) * PAIR_FLOATS;
+  const T* vp = reinterpret_cast<const T*>(a.v) + (long)b * a.vb + (long)h * a.vh;
+  const T* gp = o.dout ? reinterpret_cast<const T*>(o.dout) + (long)b * o.ob + (long)h * o.oh : vp;  // without dO: read and left out
+  const long gt = o.dout ? o.ot : a.vt;
+  const float* up = o.U + ((long)bh * a.N + n) * C * Dvp;
+  const float* rp = o.dR + ((long)bh * a.N + n) * C * Dvp;
+  const float* s0 = o.Sc + (((long)bh * a.N + n) * DKp + 16 * wave + l16) * Dvp + 4 * kq;
+  const float* ds = o.dSc + (((long)bh * a.N + n) * DKp + 16 * wave + l16) * Dvp + 4 * kq;
+
+  // the next DVB value columns on their way
+  f4 g_[RPT], r_[RPT], u_[RPT], v_[RPT], x_[2], y_[2];
+  auto fetch = [&](int c0) {
+#pragma unroll
+    for (int x = 0; x < RPT; ++x) {
+      const int at = tid + x * TH, i = at / (DVB / 4), c = c0 + 4 * (at % (DVB / 4)), ce = min(c, Dve - 4);
+      const int t = min(t0 + i, len - 1);
+      r_[x] = row4(rp + i * Dvp + ce);
+      u_[x] = row4(up + i * Dvp + ce);
+      g_[x] = four(gp + t * gt, c, a.Dv, o.vecg);
+      v_[x] = four(vp + t * a.vt, c, a.Dv, o.vecv);
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const int c = min(c0 + 16 * m, Dve - 16);
+      x_[m] = row4(s0 + c);
+      y_[m] = row4(ds + c);
+    }
+  };
+
+  st.fetch(a, reinterpret_cast<const T*>(a.q) + (long)b * a.qb + (long)hk * a.qh, reinterpret_cast<const T*>(a.k) + (long)b * a.kb + (long)hk * a.kh,
+           pair, t0, len);
+  fetch(0);
+  if (wave == NW - 1) chunk_gates<C>(a, s, b, h, t0, len, lane);
+
+  f4 GO[NT], GR[NT], GU[NT], D1[TPW], D2[TPW];
+  float dRv[RPT], sdot = 0.f;
+#pragma unroll
+  for (int ti = 0; ti < NT; ++ti) GO[ti] = GR[ti] = GU[ti] = zero;
+#pragma unroll
+  for (int x = 0; x < TPW; ++x) D1[x] = D2[x] = zero;
+#pragma unroll
+  for (int x = 0; x < RPT; ++x) dRv[x] = 0.f;
+  st.commit(t0, len, a.Dk);
+
+  for (int c0 = 0; c0 < Dve; c0 += DVB) {
+    if (c0) lds_barrier();  // the columns before are done with LDS
+#pragma unroll
+    for (int x = 0; x < RPT; ++x) {
+      const int at = tid + x * TH, i = at / (DVB / 4), c = c0 + 4 * (at % (DVB / 4));
+      const bool live = t0 + i < len;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool in = c + j < a.Dv;
+        r_[x][j] = in ? r_[x][j] : 0.f;
+        u_[x][j] = in ? u_[x][j] : 0.f;
+        g_[x][j] = in && live && o.dout ? g_[x][j] : 0.f;
+        dRv[x] = fmaf(r_[x][j], in && live ? v_[x][j] : 0.f, dRv[x]);
+      }
+      val.put(i, c - c0, g_[x], r_[x], u_[x]);
+    }
+    const f4 x0 = x_[0], x1 = c0 + 16 < Dve ? x_[1] : zero, y0 = y_[0], y1 = c0 + 16 < Dve ? y_[1] : zero;
+    lds_barrier();
+    if (c0 + DVB < Dve) fetch(c0 + DVB);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sdot = fmaf(x0[j], y0[j], fmaf(x1[j], y1[j], sdot));
+    const Op16<SP> a0 = cut<SP>(x0), a1 = cut<SP>(x1), b0 = cut<SP>(y0), b1 = cut<SP>(y1);
+#pragma unroll
+    for (int ti = 0; ti < NT; ++ti) {
+      GO[ti] = mm32r(a0, a1, val.o(ti, l16, kq), GO[ti]);
+      const auto r = val.r(ti, l16, kq);
+      GR[ti] = mm32(a0, a1, r.a, r.b, GR[ti]);
+      const auto u = val.u(ti, l16, kq);
+      GU[ti] = mm32(b0, b1, u.a, u.b, GU[ti]);
+    }
+#pragma unroll
+    for (int x = 0; x < TPW; ++x) {
+      const int t = wave + x * NW;
+      if (t < NTL) {
+        int ti, tj;
+        lower_tile(t, ti, tj);
+        const auto u = val.u(tj, l16, kq);
+        D1[x] = mm32r(u.a, u.b, val.o(ti, l16, kq), D1[x]);
+        const auto r = val.r(ti, l16, kq);
+        D2[x] = mm32(u.a, u.b, r.a, r.b, D2[x]);
+      }
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < RPT; ++x) {
+    const float v = seg_sum(dRv[x], DVB / 4);
+    if ((tid & (DVB / 4 - 1)) == 0) l.dRv[(tid + x * TH) / (DVB / 4)] = v;
+  }
+  sdot = wave_sum(sdot);
+  if (lane == 0) l.sd[wave] = sdot;
+  lds_barrier();  // the values are done with
+
+  // W1, W2 in their place, and the row and column sums of what the decays see of them
+#pragma unroll
+  for (int x = 0; x < TPW; ++x) {
+    const int t = wave + x * NW;
+    if (t < NTL) {
+      int ti, tj;
+      lower_tile(t, ti, tj);
+      const int i = 16 * ti + l16, j0 = 16 * tj + 4 * kq;
+      const f4 p = row4(pair + (PAIR_P + t) * 256 + l16 * 16 + 4 * kq);
+      f4 kk = zero;
+#pragma unroll
+      for (int m2 = 0; m2 < DKT / 2; ++m2) kk = mm32x(st.k(tj, m2), st.k(ti, m2), kk);
+      if (SP) kk *= st.rk4(tj) * st.gates[256 + i];
+      const double Gi = s.G[i];
+      const int segi = s.seg[i];
+      const float be = s.beta[i];
+      f4 w1, w2;
+      float rs = 0.f, rb = 0.f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float m = pair_decay<C>(s, i, j0 + r, Gi, segi);
+        w1[r] = m * D1[x][r];
+        const float z = j0 + r < i ? -m * D2[x][r] : 0.f;
+        w2[r] = be * z;
+        rb = fmaf(z, kk[r], rb);
+        const float e = fmaf(D1[x][r], p[r], w2[r] * kk[r]);
+        rs += e;
+        const float cs = row16_sum(e);
+        if (l16 == 0) l.cols[t][4 * kq + r] = cs;
+      }
+      *reinterpret_cast<f4*>(W1 + t * TS + l16 * TL + 4 * kq) = w1;
+      *reinterpret_cast<f4*>(W2 + t * TS + l16 * TL + 4 * kq) = w2;
+      rs += __shfl_xor(rs, 16, 64);
+      rs += __shfl_xor(rs, 32, 64);
+      rb += __shfl_xor(rb, 16, 64);
+      rb += __shfl_xor(rb, 32, 64);
+      if (kq == 0) {
+        l.rows[t][l16] = rs;
+        l.rowb[t][l16] = rb;
+      }
+    }
+  }
+  lds_barrier();
+
+  // this wave's 16 key columns of dQ^T and dK^T
+  f4 dQ[NT], dK[NT];
+  const int kc = 16 * wave;
+  auto row_of = [&](const float* W, int ti, int tj) { return row4(W + (ti * (ti + 1) / 2 + tj) * TS + l16 * TL + 4 * kq); };
+  auto col_of = [&](const float* W, int ti, int tj) { return col4(W + (ti * (ti + 1) / 2 + tj) * TS + 4 * kq * TL + l16, TL); };
+#pragma unroll
+  for (int ti = 0; ti < NT; ++ti) {
+    const int i = 16 * ti + l16;
+    const float ga = s.gam[i], be = s.beta[i], e = s.e[i];
+    const f4 q = st.q_of(i, kc + 4 * kq), k = st.k_of(i, kc + 4 * kq);
+    float d0 = 0.f, d1 = 0.f, d2 = 0.f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      d0 = fmaf(q[r], GO[ti][r], d0);
+      d1 = fmaf(k[r], GR[ti][r], d1);
+      d2 = fmaf(k[r], GU[ti][r], d2);
+    }
+    f4 x = ga * GO[ti], w = zero, z = zero;
+#pragma unroll
+    for (int t2 = 0; t2 < 2; ++t2) {
+      const int ta = 2 * t2, tb = 2 * t2 + 1;
+      const Exact32<SP> kt = st.kt(wave, t2);
+      if (ta <= ti) x = mm32(kt, cut<SP>(row_of(W1, ti, ta) * st.rk4(ta)), cut<SP>(tb <= ti ? row_of(W1, ti, tb) * st.rk4(tb) : zero), x);
+      if (tb >= ti)
+        z = mm32(st.qt(wave, t2), cut<SP>(ta >= ti ? col_of(W1, ta, ti) * st.rq4(ta) : zero), cut<SP>(col_of(W1, tb, ti) * st.rq4(tb)), z);
+      f4 wa = zero, wb = zero;
+      if (ta <= ti) wa += row_of(W2, ti, ta);
+      if (ta >= ti) wa += col_of(W2, ta, ti);
+      if (tb <= ti) wb += row_of(W2, ti, tb);
+      if (tb >= ti) wb += col_of(W2, tb, ti);
+      w = mm32(kt, cut<SP>(wa * st.rk4(ta)), cut<SP>(wb * st.rk4(tb)), w);
+    }
+    dQ[ti] = a.scale * x;
+    dK[ti] = w + a.scale * z - (be * ga) * GR[ti] + e * GU[ti];
+    float d3 = 0.f, d4 = 0.f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      d3 = fmaf(q[r], dQ[ti][r], d3);
+      d4 = fmaf(k[r], dK[ti][r], d4);
+    }
+    float dd[5] = {d0, d1, d2, d3, d4};
+#pragma unroll
+    for (int y = 0; y < 5; ++y) {
+      dd[y] += __shfl_xor(dd[y], 16, 64);
+      dd[y] += __shfl_xor(dd[y], 32, 64);
+      if (kq == 0) l.dots[y][wave][i] = dd[y];
+    }
+  }
+  lds_barrier();
+#pragma unroll
+  for (int ti = 0; ti < NT; ++ti) {
+    const int i = 16 * ti + l16;
+    if (a.normalize) {
+      float dq = 0.f, dk = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        dq += l.dots[3][w][i];
+        dk += l.dots[4][w][i];
+      }
+      dQ[ti] = st.gates[192 + i] * (dQ[ti] - dq * st.q_of(i, kc + 4 * kq));
+      dK[ti] = st.gates[256 + i] * (dK[ti] - dk * st.k_of(i, kc + 4 * kq));
+    }
+    if (t0 + i < a.T && kc + 4 * kq < a.Dk) {
+      const bool live = t0 + i < len;
+      put(o.dq, i, kc + 4 * kq, live ? dQ[ti] : zero);
+      put(o.dk, i, kc + 4 * kq, live ? dK[ti] : zero);
+    }
+  }
+  if (wave == 0) {
+    const int i = lane;
+    float go = 0.f, gr = 0.f, gu = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      go += l.dots[0][w][i];
+      gr += l.dots[1][w][i];
+      gu += l.dots[2][w][i];
+    }
+    const float ga = s.gam[i], be = s.beta[i], F = s.e[i] * gu;
+    float db = l.dRv[i] - ga * gr;
+    double dG = (double)(a.scale * ga * go) - (double)(be * ga * gr) - (double)F;
+#pragma unroll
+    for (int t = 0; t < NTL; ++t) {
+      int ti, tj;
+      lower_tile(t, ti, tj);
+      if (ti == i >> 4) {
+        dG += (double)l.rows[t][i & 15];
+        db += l.rowb[t][i & 15];
+      }
+      if (tj == i >> 4) dG -= (double)l.cols[t][i & 15];
+    }
+    const float sumF = wave_sum(F);
+    if (i == C - 1) {
+      float sd = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) sd += l.sd[w];
+      dG += (double)(sumF + ga * sd);
+    }
+    const float g = segment_suffix<C>(s, dG, i);
+    if (t0 + i < a.T) {
+      o.dg[(long)(t0 + i) * BH + bh] = s.rst[i] ? 0.f : g;
       o.db[(long)(t0 + i) * BH + bh] = t0 + i < len ? db : 0.f;
     }
   }
@@ -555,6 +941,9 @@ static void launch_c(const Args& a, const BwdArgs& o, bool per_value_head, hipSt
   const int nvs = (a.Dv + 15) / 16, BH = a.B * a.Hv;
   if constexpr (C == 16) {
     delta_bwd_short_kernel<T, DKT><<<BH, 64 * nvs, strip_lds<DKT, 16>(true), st>>>(a, o);
+    const int lds = (int)sizeof(PairLds<DKT, C>);
+    allow_lds<delta_bwd_pair_kernel<T, DKT, C>>(lds);
+    delta_bwd_pair_kernel<T, DKT, C><<<BH, 64 * DKT, lds, st>>>(a, o, per_value_head ? 1 : 0);
   } else {
     if (a.nseg > 1) {
       if (nvs <= 4) launch_walk<T, DKT, 4, true>(a, o, st);
@@ -563,10 +952,10 @@ static void launch_c(const Args& a, const BwdArgs& o, bool per_value_head, hipSt
     }
     if (nvs <= 4) launch_walk<T, DKT, 4, false>(a, o, st);
     else launch_walk<T, DKT, 8, false>(a, o, st);
+    const int lds = (int)sizeof(GradsLds<T, DKT>);
+    allow_lds<delta_grads_kernel<T, DKT>>(lds);
+    delta_grads_kernel<T, DKT><<<BH * a.N, 64 * DKT, lds, st>>>(a, o, per_value_head ? 1 : 0);
   }
-  const int lds = (int)sizeof(PairLds<DKT, C>);
-  allow_lds<delta_bwd_pair_kernel<T, DKT, C>>(lds);
-  delta_bwd_pair_kernel<T, DKT, C><<<BH * a.N, 64 * DKT, lds, st>>>(a, o, per_value_head ? 1 : 0);
 }
 
 template <typename T>
