@@ -401,11 +401,17 @@ struct Stage<float, DKT, NWT, MODE> {
   float rk_[RR][NE], rq_[HQ ? RR : 1][NE];
   float nk[RR], nq[RR];
   f4 tl[NT4 > 0 ? NT4 : 1], ga;
-  int l16, kq;
+  int tid, l16, kq;
 
   __device__ __forceinline__ explicit Stage(void* lds)
-      : K((float*)lds), Q(K + 64 * LD), tile(K + (HQ ? 2 : 1) * 64 * LD), gates(tile + TI::N * TS), l16(threadIdx.x & 15),
+      : K((float*)lds), Q(K + 64 * LD), tile(K + (HQ ? 2 : 1) * 64 * LD), gates(tile + TI::N * TS), tid(threadIdx.x), l16(threadIdx.x & 15),
         kq((threadIdx.x >> 4) & 3) {}
+  // The lane's place, worked out afresh in each turn of a walk: see afresh().
+  __device__ __forceinline__ void turn() {
+    int t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    tid = t, l16 = t & 15, kq = (t >> 4) & 3;
+  }
   __device__ __forceinline__ Exact32<false> rows(const float* M, int ti, int m2) const {
     const float* p = M + (16 * ti + l16) * LD + 32 * m2 + 4 * kq;
     return {row4(p), row4(p + 16)};
@@ -436,10 +442,10 @@ struct Stage<float, DKT, NWT, MODE> {
   __device__ __forceinline__ f4 k_of(int i, int c) const { return row4(K + i * LD + c); }
   __device__ __forceinline__ f4 q_of(int i, int c) const { return row4(Q + i * LD + c); }
   __device__ __forceinline__ void rows_(float (*w)[NE], const float* src, long st, int D, int t0, int len, bool vec) {
-    const int c0 = (threadIdx.x & 15) * NE;
+    const int c0 = (tid & 15) * NE;
     const float* p[RR];
 #pragma unroll
-    for (int r = 0; r < RR; ++r) p[r] = src + (long)min(t0 + (int)(threadIdx.x >> 4) + r * 4 * NWT, len - 1) * st;
+    for (int r = 0; r < RR; ++r) p[r] = src + (long)min(t0 + (tid >> 4) + r * 4 * NWT, len - 1) * st;
     if (vec) {
 #pragma unroll
       for (int r = 0; r < RR; ++r) ldv<NE>(p[r] + min(c0, D - NE), w[r]);
@@ -455,22 +461,22 @@ struct Stage<float, DKT, NWT, MODE> {
     if constexpr (HQ) rows_(rq_, qp, a.qt, a.Dk, t0, len, a.vecq);
 #pragma unroll
     for (int r = 0; r < RR; ++r) {
-      const float* n = pair + PAIR_TILES * 256 + (threadIdx.x >> 4) + r * 4 * NWT;
+      const float* n = pair + PAIR_TILES * 256 + (tid >> 4) + r * 4 * NWT;
       nk[r] = n[256];
       if constexpr (HQ) nq[r] = n[192];
     }
 #pragma unroll
     for (int x = 0; x < NT4; ++x) {
-      const int at = min((int)threadIdx.x + x * TH, TI::N * 64 - 1);  // 16 bytes each
+      const int at = min(tid + x * TH, TI::N * 64 - 1);  // 16 bytes each
       tl[x] = row4(pair + 256 * TI::source(at >> 6) + 4 * (at & 63));
     }
-    ga = row4(pair + PAIR_TILES * 256 + 4 * min((int)threadIdx.x, 79));
+    ga = row4(pair + PAIR_TILES * 256 + 4 * min(tid, 79));
   }
   __device__ __forceinline__ void commit(int t0, int len, int D) {
-    const int c0 = (threadIdx.x & 15) * NE;
+    const int c0 = (tid & 15) * NE;
 #pragma unroll
     for (int r = 0; r < RR; ++r) {
-      const int i = (threadIdx.x >> 4) + r * 4 * NWT;
+      const int i = (tid >> 4) + r * 4 * NWT;
 #pragma unroll
       for (int j = 0; j < NE; ++j) {
         const bool in = t0 + i < len && c0 + j < D;
@@ -480,10 +486,10 @@ struct Stage<float, DKT, NWT, MODE> {
     }
 #pragma unroll
     for (int x = 0; x < NT4; ++x) {
-      const int at = threadIdx.x + x * TH;
+      const int at = tid + x * TH;
       if (at < TI::N * 64) *reinterpret_cast<f4*>(tile + (at >> 6) * TS + ((at >> 2) & 15) * TL + 4 * (at & 3)) = (at >> 6) < 10 ? -tl[x] : tl[x];
     }
-    if (threadIdx.x < 80) *reinterpret_cast<f4*>(gates + 4 * threadIdx.x) = ga;
+    if (tid < 80) *reinterpret_cast<f4*>(gates + 4 * tid) = ga;
   }
 };
 
@@ -503,11 +509,17 @@ struct Stage<bf16, DKT, NWT, MODE> {
   float* gates;  // beta, gam, e, rq, rk
   uint32_t rk_[NG][4], rq_[HQ ? NG : 1][4];
   f4 tl[NT4 > 0 ? NT4 : 1], ga;
-  int l16, kq;
+  int tid, l16, kq;
 
   __device__ __forceinline__ explicit Stage(void* lds)
       : Kr((uint16_t*)lds), Kc(Kr + ROWS), Qx(Kc + COLS), tile((u2*)(Qx + (HQ ? (QT ? COLS : ROWS) : 0))),
-        gates((float*)(tile + TI::N * 192)), l16(threadIdx.x & 15), kq((threadIdx.x >> 4) & 3) {}
+        gates((float*)(tile + TI::N * 192)), tid(threadIdx.x), l16(threadIdx.x & 15), kq((threadIdx.x >> 4) & 3) {}
+  // The lane's place, worked out afresh in each turn of a walk: see afresh().
+  __device__ __forceinline__ void turn() {
+    int t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    tid = t, l16 = t & 15, kq = (t >> 4) & 3;
+  }
   __device__ __forceinline__ Exact32<true> rows(const uint16_t* M, int ti, int m2) const {
     return {*reinterpret_cast<const u4*>(M + (16 * ti + l16) * LR + 32 * m2 + 8 * kq)};
   }
@@ -519,7 +531,7 @@ struct Stage<bf16, DKT, NWT, MODE> {
   __device__ __forceinline__ Exact32<true> kt(int m, int t2) const { return cols(Kc, m, t2); }
   __device__ __forceinline__ Exact32<true> qt(int m, int t2) const { return cols(Qx, m, t2); }
   __device__ __forceinline__ Op16<true> tl_(int x) const {
-    const u2* p = tile + x * 192 + (threadIdx.x & 63);
+    const u2* p = tile + x * 192 + 16 * kq + l16;
     return {p[0], p[64], p[128]};
   }
   __device__ __forceinline__ Op16<true> A(int ti, int tj) const { return tl_(TI::A(ti, tj)); }
@@ -544,7 +556,7 @@ struct Stage<bf16, DKT, NWT, MODE> {
     return f4{n * bf2f(p[0]), n * bf2f(p[LC]), n * bf2f(p[2 * LC]), n * bf2f(p[3 * LC])};
   }
   __device__ __forceinline__ void rows4(uint32_t (*w)[4], const bf16* src, long st, int D, int t0, int len, bool vec) {
-    const int c = 2 * (threadIdx.x % CP), i0 = 4 * (threadIdx.x / CP < 16 ? threadIdx.x / CP : 0);
+    const int c = 2 * (tid % CP), i0 = 4 * (tid / CP < 16 ? tid / CP : 0);
     const bf16* p[NG][4];
 #pragma unroll
     for (int g = 0; g < NG; ++g)
@@ -569,24 +581,24 @@ struct Stage<bf16, DKT, NWT, MODE> {
     if constexpr (HQ) rows4(rq_, qp, a.qt, a.Dk, t0, len, a.vecq);
 #pragma unroll
     for (int x = 0; x < NT4; ++x) {
-      const int at = min((int)threadIdx.x + x * TH, TI::N * 64 - 64 + (int)(threadIdx.x & 63));  // 64 divides TH: at & 63 is the lane
+      const int at = min(tid + x * TH, TI::N * 64 - 64 + (tid & 63));  // 64 divides TH: at & 63 is the lane
       const float* p = pair + 256 * TI::source(at >> 6);
       tl[x] = MODE == 2 ? col4(p + 4 * kq * 16 + l16, 16) : row4(p + 16 * l16 + 4 * kq);
     }
-    ga = row4(pair + PAIR_TILES * 256 + 4 * min((int)threadIdx.x, 79));
+    ga = row4(pair + PAIR_TILES * 256 + 4 * min(tid, 79));
   }
   __device__ __forceinline__ void put_rows(uint16_t* M, const uint32_t* w, int i) {
-    const int c = place(2 * (threadIdx.x % CP));
+    const int c = place(2 * (tid % CP));
 #pragma unroll
     for (int r = 0; r < 4; ++r) *reinterpret_cast<uint32_t*>(M + (i + r) * LR + c) = w[r];
   }
   __device__ __forceinline__ void put_cols(uint16_t* M, const uint32_t* w, int i) {
-    uint16_t* p = M + 2 * (threadIdx.x % CP) * LC + place(i);
+    uint16_t* p = M + 2 * (tid % CP) * LC + place(i);
     *reinterpret_cast<u2*>(p) = u2{(w[0] & 0xffffu) | (w[1] << 16), (w[2] & 0xffffu) | (w[3] << 16)};
     *reinterpret_cast<u2*>(p + LC) = u2{(w[0] >> 16) | (w[1] & 0xffff0000u), (w[2] >> 16) | (w[3] & 0xffff0000u)};
   }
   __device__ __forceinline__ void commit(int t0, int len, int D) {
-    const int g0 = threadIdx.x / CP, c = 2 * (threadIdx.x % CP);
+    const int g0 = tid / CP, c = 2 * (tid % CP);
     const uint32_t cm = c + 1 < D ? ~0u : c < D ? 0xffffu : 0u;
     if (g0 < 16) {
 #pragma unroll
@@ -608,16 +620,20 @@ struct Stage<bf16, DKT, NWT, MODE> {
     }
 #pragma unroll
     for (int x = 0; x < NT4; ++x) {
-      const int at = threadIdx.x + x * TH;
+      const int at = tid + x * TH;
       if (at < TI::N * 64) {
         const Op16<true> o = cut3((at >> 6) < 10 ? -tl[x] : tl[x]);
         u2* p = tile + (at >> 6) * 192 + (at & 63);
         p[0] = o.p0, p[64] = o.p1, p[128] = o.p2;
       }
     }
-    if (threadIdx.x < 80) *reinterpret_cast<f4*>(gates + 4 * threadIdx.x) = ga;
+    if (tid < 80) *reinterpret_cast<f4*>(gates + 4 * tid) = ga;
   }
 };
+
+// Between two parts of a walk: operands of the second are not read from LDS before the first is done, which would cost spills, and
+// a reload from memory waits for everything that is on its way.
+__device__ __forceinline__ void part_ends() { __builtin_amdgcn_sched_barrier(0); }
 
 // f(0), ..., f(N - 1) with compile-time indexes: arrays of operands stay in registers
 template <int I, int N, typename F>

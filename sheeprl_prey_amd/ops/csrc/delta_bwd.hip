@@ -141,6 +141,7 @@ __global__ void __launch_bounds__(64 * NWT) delta_bwd_walk_kernel(Args a, BwdArg
         for (int r = 0; r < 4; ++r) p[(16 * m + r) * Dvp] = S[m][r];
     }
     lds_barrier();
+    st.turn();
     st.commit(t0, len, a.Dk);
     lds_barrier();
     f4 dy[NT], u[NT];
@@ -151,12 +152,14 @@ __global__ void __launch_bounds__(64 * NWT) delta_bwd_walk_kernel(Args a, BwdArg
       if (gp) dn.fetch(gcol, o.ot, t0 - C, len, kq);
     }
     if (!works) continue;
+    part_ends();
 #pragma unroll
     for (int m2 = 0; m2 < DKT / 2; ++m2) {
       const Op16<SP> s0 = cut<SP>(S[2 * m2]), s1 = cut<SP>(S[2 * m2 + 1]);
 #pragma unroll
       for (int ti = 0; ti < NT; ++ti) u[ti] = mm32(st.k(ti, m2), s0, s1, u[ti]);
     }
+    part_ends();
     // dR: backward substitution by blocks of 16 steps
     Op16<SP> ub[NT], db[NT];
     each<0, NT>([&](auto I) {
@@ -183,6 +186,7 @@ __global__ void __launch_bounds__(64 * NWT) delta_bwd_walk_kernel(Args a, BwdArg
         }
       }
     }
+    part_ends();
     const float gc = st.gam_last();
 #pragma unroll
     for (int m = 0; m < DKT; ++m) S[m] *= gc;

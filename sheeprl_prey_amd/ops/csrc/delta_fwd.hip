@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(64 * NWT) delta_walk_kernel(Args a, FwdOut o) 
   const int n0 = seg * a.cps, n1 = min(a.N, n0 + a.cps), live = min(n1, (len + C - 1) / C);
   if (n0 < live) {
     st.fetch(a, qp, kp, pairs + (long)n0 * PAIR_FLOATS, n0 * C, len);
-    v.fetch(vcol, a.vt, n0 * C, len, kq);
+    if (vstrip) v.fetch(vcol, a.vt, n0 * C, len, kq);
   }
   for (int n = n0; n < live; ++n) {
     const int t0 = n * C;
@@ -220,6 +220,7 @@ __global__ void __launch_bounds__(64 * NWT) delta_walk_kernel(Args a, FwdOut o) 
         for (int r = 0; r < 4; ++r) p[(16 * m + r) * Dvp] = S[m][r];
     }
     lds_barrier();  // the chunk before is done with LDS
+    st.turn();
     st.commit(t0, len, a.Dk);
     lds_barrier();
     f4 u[NT];
@@ -227,9 +228,10 @@ __global__ void __launch_bounds__(64 * NWT) delta_walk_kernel(Args a, FwdOut o) 
     for (int ti = 0; ti < NT; ++ti) u[ti] = st.beta(ti) * v.get(ti, t0, len, kq, vstrip && dv < a.Dv);
     if (n + 1 < live) {
       st.fetch(a, qp, kp, pairs + (long)(n + 1) * PAIR_FLOATS, t0 + C, len);
-      v.fetch(vcol, a.vt, t0 + C, len, kq);
+      if (vstrip) v.fetch(vcol, a.vt, t0 + C, len, kq);
     }
     if (!works) continue;
+    part_ends();
     // K S0 and Q S0
     f4 ks[NT], y[NT];
 #pragma unroll
@@ -243,6 +245,7 @@ __global__ void __launch_bounds__(64 * NWT) delta_walk_kernel(Args a, FwdOut o) 
         if constexpr (!MAP) y[ti] = mm32(st.q(ti, m2), s0, s1, y[ti]);
       }
     }
+    part_ends();
     // U: forward substitution by blocks of 16 steps
     Op16<SP> ub[NT];
     each<0, NT>([&](auto I) {
@@ -252,6 +255,7 @@ __global__ void __launch_bounds__(64 * NWT) delta_walk_kernel(Args a, FwdOut o) 
       u[ti] = mm16o(st.Ti(ti), cut<SP>(r), zero);
       ub[ti] = cut<SP>(u[ti]);
     });
+    part_ends();
     if constexpr (!MAP) {
       if (o.U) {
         float* p = o.U + ((long)bh * a.N + n) * C * Dvp + 4 * kq * Dvp + dv;
@@ -273,6 +277,7 @@ __global__ void __launch_bounds__(64 * NWT) delta_walk_kernel(Args a, FwdOut o) 
         }
       });
     }
+    part_ends();
     // S' = gam_C S + K^T diag(e) U
     const float gc = st.gam_last();
 #pragma unroll
@@ -322,7 +327,7 @@ __global__ void __launch_bounds__(64 * DKT) delta_scan_kernel(const float* first
   __shared__ __align__(16) float S[2][16 * LD];
   const int lane = threadIdx.x & 63, m = threadIdx.x >> 6, l16 = lane & 15, kq = lane >> 4;
   const int nvs = (Dv + 15) >> 4, bh = blockIdx.x / nvs, strip = blockIdx.x % nvs, dv = 16 * strip + l16;
-  f4 s, x[DKT], r;
+  f4 s, x[2][DKT], r[2];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int d = 16 * m + 4 * kq + j;
@@ -330,29 +335,35 @@ __global__ void __launch_bounds__(64 * DKT) delta_scan_kernel(const float* first
   }
   auto at = [&](int i) { return (long)bh * nseg + (REV ? nseg - 1 - i : i); };
   auto native = [&](long g) { return ((g * nvs + strip) * DKT + m) * 256 + lane * 4; };
-  auto fetch = [&](int i) {
+  auto fetch = [&](int i, f4* xs, f4& rs) {
     const float* p = P + at(i) * DKp * DKp;
 #pragma unroll
     for (int k = 0; k < DKT; ++k)
-      x[k] = REV ? col4(p + (16 * k + 4 * kq) * DKp + 16 * m + l16, DKp) : row4(p + (16 * m + l16) * DKp + 16 * k + 4 * kq);
-    r = row4(R + native(at(i)));
+      xs[k] = REV ? col4(p + (16 * k + 4 * kq) * DKp + 16 * m + l16, DKp) : row4(p + (16 * m + l16) * DKp + 16 * k + 4 * kq);
+    rs = row4(R + native(at(i)));
   };
-  if (nseg > 1) fetch(0);
-  for (int i = 0; i < nseg; ++i) {
+  auto step = [&](int i, const f4* xs, const f4& rs, float* l) {
     *reinterpret_cast<f4*>(out + native(at(i))) = s;
-    if (i == nseg - 1) break;
-    float* l = S[i & 1];
     *reinterpret_cast<f4*>(l + l16 * LD + 16 * m + 4 * kq) = s;
     lds_barrier();  // two buffers: the one before is free once every wave is here
-    f4 n0 = r, n1 = {0.f, 0.f, 0.f, 0.f};
+    f4 n0 = rs, n1 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < DKT; k += 2) {
-      n0 = mm16(x[k], row4(l + l16 * LD + 16 * k + 4 * kq), n0);
-      n1 = mm16(x[k + 1], row4(l + l16 * LD + 16 * k + 16 + 4 * kq), n1);
+      n0 = mm16(xs[k], row4(l + l16 * LD + 16 * k + 4 * kq), n0);
+      n1 = mm16(xs[k + 1], row4(l + l16 * LD + 16 * k + 16 + 4 * kq), n1);
     }
-    if (i + 2 < nseg) fetch(i + 1);
     s = n0 + n1;
+  };
+  const int last = nseg - 1;  // the last segment's first state is the end of it
+  fetch(0, x[0], r[0]);
+  for (int i = 0; i < last; i += 2) {
+    fetch(min(i + 1, last), x[1], r[1]);
+    step(i, x[0], r[0], S[0]);
+    if (i + 1 >= last) break;
+    fetch(min(i + 2, last), x[0], r[0]);
+    step(i + 1, x[1], r[1], S[1]);
   }
+  *reinterpret_cast<f4*>(out + native(at(last))) = s;
 }
 
 template <typename T, int DKT, int NWT, bool MAP>
