@@ -49,7 +49,7 @@ struct BwdArgs {
   float* dR;    // [BH, N, C, Dvp]
   float* Xseg;   // as Rseg: the gradient of a segment's first state where that of its last is zero
   float* dSseg;  // as Sseg: the gradient of each segment's last state
-  void *dq, *dk;  // [T, B, H?, Dk] contiguous: per key head in the input's type (Hv == Hk), else per value head in fp32
+  void *dq, *dk;  // contiguous: [T, B, Hk, Dk] in the inputs' type, or [T, B, Hv, Dk] in fp32, to be summed
   void* dv;
   float *dg, *db, *dstate;
 };
@@ -58,7 +58,7 @@ void launch_delta_fwd(const Args& a, const FwdOut& o, int C, bool is_bf16, hipSt
 void launch_delta_bwd(const Args& a, const BwdArgs& o, int C, bool is_bf16, bool per_value_head, hipStream_t st);
 void launch_delta_scan_rev(const float* dlast, const float* P, const float* X, float* dS, int BH, int nseg, int Dk, int Dv,
                            hipStream_t st);
-void launch_delta_head_sum(const float* x, void* y, long rows, int rep, int Dk, bool is_bf16, hipStream_t st);
+void launch_delta_head_sum(const float* xq, const float* xk, void* yq, void* yk, long rows, int rep, int Dk, bool is_bf16, hipStream_t st);
 // delta_step.hip: the recurrent form; S2 (the state after it) may be a.state itself
 void launch_delta_steps(const Args& a, void* out, float* S2, long sb, long sh, bool is_bf16, hipStream_t st);
 

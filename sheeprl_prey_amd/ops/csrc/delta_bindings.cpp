@@ -256,7 +256,9 @@ struct GatedDeltaFn : public torch::autograd::Function<GatedDeltaFn> {
     TORCH_CHECK(s[7].numel() == at.n, "gated_delta: the plan changed between the passes");
     const float* sp = s[7].data_ptr<float>();
     o.Sc = sp + at.Sc, o.U = sp + at.U, o.Pseg = sp + at.P, o.pairs = sp + at.pairs;
-    const bool shared = a.Hk != a.Hv, bf = q.scalar_type() == torch::kBFloat16;
+    // dq and dk of shared key heads: one workgroup a key head where those fill the 256 CUs twice (4096 steps x 2 x 8: the
+    // separate sums cost 54 us more), else one a value head and a sum
+    const bool shared = a.Hk != a.Hv && (C == 16 || (int64_t)a.B * a.Hk * a.N < 512), bf = q.scalar_type() == torch::kBFloat16;
     Workspace w;
     const int64_t segs = a.nseg > 1 ? BH * a.nseg * DKp * Dvp : 0, heads = shared ? (int64_t)a.T * BH * a.Dk : 0;
     const int64_t ds = w.add(BH * a.N * DKp * Dvp), dr = w.add(BH * a.N * C * Dvp), x = w.add(segs), dss = w.add(segs), hq = w.add(heads),
@@ -277,8 +279,7 @@ struct GatedDeltaFn : public torch::autograd::Function<GatedDeltaFn> {
     srl::delta::launch_delta_bwd(a, o, C, bf, shared, cur());
     if (shared) {
       const long rows = (long)a.T * a.B * a.Hk;
-      srl::delta::launch_delta_head_sum(p + hq, dq.data_ptr(), rows, a.Hv / a.Hk, a.Dk, bf, cur());
-      srl::delta::launch_delta_head_sum(p + hk, dk.data_ptr(), rows, a.Hv / a.Hk, a.Dk, bf, cur());
+      srl::delta::launch_delta_head_sum(p + hq, p + hk, dq.data_ptr(), dk.data_ptr(), rows, a.Hv / a.Hk, a.Dk, bf, cur());
     }
     launched("gated_delta backward");
     g[0] = dq, g[1] = dk, g[2] = dv, g[3] = dg, g[4] = db;

@@ -625,9 +625,13 @@ struct GradsLds {
   __align__(16) unsigned char big[BIG], stage[Stage<T, DKT, DKT, 3>::BYTES];
 };
 
-// Chunks of 64: what sums over the value columns (the head of this file), one wave per 16 key columns.
-template <typename T, int DKT>
-__global__ void __launch_bounds__(64 * DKT) delta_grads_kernel(Args a, BwdArgs o, int per_value_head) {
+// Chunks of 64: what sums over the value columns (the head of this file), one wave per 16 key columns.  A workgroup takes the
+// G value heads that share a key head one after the other and leaves the sum of their dq and dk; with few chunks (G = 1) the
+// heads go to workgroups of their own, and delta_head_sum_kernel adds them.
+// ONE: a single head (G = 1), whose sums live in fewer registers: two workgroups of narrow heads fit a CU.
+template <typename T, int DKT, bool ONE>
+__global__ void __launch_bounds__(64 * DKT, ONE ? 2 : 1) delta_grads_kernel(Args a, BwdArgs o, int G_) {
+  const int G = ONE ? 1 : G_;
   using L = GradsLds<T, DKT>;
   using St = Stage<T, DKT, DKT, 3>;
   constexpr bool SP = St::SP;
@@ -640,13 +644,19 @@ __global__ void __launch_bounds__(64 * DKT) delta_grads_kernel(Args a, BwdArgs o
   Values<T, TH> val(l.big);
   float *W1 = reinterpret_cast<float*>(l.big), *W2 = W1 + NTL * TS;
 
-  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, kq = lane >> 4, wave = tid >> 6;
-  const int BH = a.B * a.Hv, bh = blockIdx.x % BH, n = blockIdx.x / BH, t0 = n * C;
-  const int b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
+  int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, kq = lane >> 4;
+  const int wave = tid >> 6;
+  // the lane's place afresh in each turn over the heads: see afresh()
+  auto turn = [&]() {
+    st.turn();
+    tid = st.tid, lane = tid & 63, l16 = st.l16, kq = st.kq;
+  };
+  const int BH = a.B * a.Hv, rep = a.Hv / a.Hk, BG = BH / G, bg = blockIdx.x % BG, n = blockIdx.x / BG, t0 = n * C;
+  const int b = bg / (a.Hv / G), h0 = (bg % (a.Hv / G)) * G, hk = h0 / rep;
   const int Dvp = pitch(a.Dv), Dve = 16 * ((a.Dv + 15) >> 4);
   const int len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
-  const int Ho = per_value_head ? a.Hv : a.Hk, ho = per_value_head ? h : hk;
-  const bool same = per_value_head == 0;  // the outputs have the inputs' type
+  const bool same = G == rep;  // dq and dk are whole: in the inputs' type, else fp32 for each value head
+  const int Ho = same ? a.Hk : a.Hv, ho = same ? hk : h0;
 
   auto put = [&](void* base, int i, int d, f4 v) {
     const long at = (((long)(t0 + i) * a.B + b) * Ho + ho) * a.Dk + d;
@@ -670,33 +680,34 @@ __global__ void __launch_bounds__(64 * DKT) delta_grads_kernel(Args a, BwdArgs o
       put(o.dq, x / q4, 4 * (x % q4), zero);
       put(o.dk, x / q4, 4 * (x % q4), zero);
     }
-    if (tid < m) {
-      o.dg[(long)(t0 + tid) * BH + bh] = 0.f;
-      o.db[(long)(t0 + tid) * BH + bh] = 0.f;
+    for (int x = tid; x < m * G; x += TH) {
+      const long at = (long)(t0 + x / G) * BH + b * a.Hv + h0 + x % G;
+      o.dg[at] = 0.f;
+      o.db[at] = 0.f;
     }
     return;
   }
 
-  const float* pair = o.pairs + ((long)bh * a.N + n) * PAIR_FLOATS;
-  const T* vp = reinterpret_cast<const T*>(a.v) + (long)b * a.vb + (long)h * a.vh;
-  const T* gp = o.dout ? reinterpret_cast<const T*>(o.dout) + (long)b * o.ob + (long)h * o.oh : vp;  // without dO: read and left out
-  const long gt = o.dout ? o.ot : a.vt;
-  const float* up = o.U + ((long)bh * a.N + n) * C * Dvp;
-  const float* rp = o.dR + ((long)bh * a.N + n) * C * Dvp;
-  const float* s0 = o.Sc + (((long)bh * a.N + n) * DKp + 16 * wave + l16) * Dvp + 4 * kq;
-  const float* ds = o.dSc + (((long)bh * a.N + n) * DKp + 16 * wave + l16) * Dvp + 4 * kq;
+  const T* vp = reinterpret_cast<const T*>(a.v) + (long)b * a.vb;
+  const T* gp = o.dout ? reinterpret_cast<const T*>(o.dout) + (long)b * o.ob : vp;  // without dO: read and left out
+  const long gt = o.dout ? o.ot : a.vt, gh = o.dout ? o.oh : a.vh;
+  const long c_at = (long)b * a.Hv * a.N + n;  // the chunk of head h: c_at + h N
 
   // the next DVB value columns on their way
   f4 g_[RPT], r_[RPT], u_[RPT], v_[RPT], x_[2], y_[2];
-  auto fetch = [&](int c0) {
+  auto fetch = [&](int h, int c0) {
+    const long ch = c_at + (long)h * a.N;
+    const float *up = o.U + ch * C * Dvp, *rp = o.dR + ch * C * Dvp;
+    const float* s0 = o.Sc + (ch * DKp + 16 * wave + l16) * Dvp + 4 * kq;
+    const float* ds = o.dSc + (ch * DKp + 16 * wave + l16) * Dvp + 4 * kq;
 #pragma unroll
     for (int x = 0; x < RPT; ++x) {
       const int at = tid + x * TH, i = at / (DVB / 4), c = c0 + 4 * (at % (DVB / 4)), ce = min(c, Dve - 4);
       const int t = min(t0 + i, len - 1);
       r_[x] = row4(rp + i * Dvp + ce);
       u_[x] = row4(up + i * Dvp + ce);
-      g_[x] = four(gp + t * gt, c, a.Dv, o.vecg);
-      v_[x] = four(vp + t * a.vt, c, a.Dv, o.vecv);
+      g_[x] = four(gp + t * gt + h * gh, c, a.Dv, o.vecg);
+      v_[x] = four(vp + t * a.vt + h * a.vh, c, a.Dv, o.vecv);
     }
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
@@ -707,10 +718,21 @@ __global__ void __launch_bounds__(64 * DKT) delta_grads_kernel(Args a, BwdArgs o
   };
 
   st.fetch(a, reinterpret_cast<const T*>(a.q) + (long)b * a.qb + (long)hk * a.qh, reinterpret_cast<const T*>(a.k) + (long)b * a.kb + (long)hk * a.kh,
-           pair, t0, len);
-  fetch(0);
-  if (wave == NW - 1) chunk_gates<C>(a, s, b, h, t0, len, lane);
+           o.pairs + (c_at + (long)h0 * a.N) * PAIR_FLOATS, t0, len);
+  fetch(h0, 0);
+  f4 dQ[NT], dK[NT];
+#pragma unroll
+  for (int ti = 0; ti < NT; ++ti) dQ[ti] = dK[ti] = zero;
+  st.commit(t0, len, a.Dk);
 
+  const int kc = 16 * wave;  // this wave's key columns
+  int h = h0;
+  do {
+  const long bh = (long)b * a.Hv + h;
+  const float* pair = o.pairs + (c_at + (long)h * a.N) * PAIR_FLOATS;
+  if (h > h0) lds_barrier();  // the head before is done with LDS
+  turn();
+  if (wave == NW - 1) chunk_gates<C>(a, s, b, h, t0, len, lane);
   f4 GO[NT], GR[NT], GU[NT], D1[TPW], D2[TPW];
   float dRv[RPT], sdot = 0.f;
 #pragma unroll
@@ -719,7 +741,6 @@ __global__ void __launch_bounds__(64 * DKT) delta_grads_kernel(Args a, BwdArgs o
   for (int x = 0; x < TPW; ++x) D1[x] = D2[x] = zero;
 #pragma unroll
   for (int x = 0; x < RPT; ++x) dRv[x] = 0.f;
-  st.commit(t0, len, a.Dk);
 
   for (int c0 = 0; c0 < Dve; c0 += DVB) {
     if (c0) lds_barrier();  // the columns before are done with LDS
@@ -739,9 +760,11 @@ __global__ void __launch_bounds__(64 * DKT) delta_grads_kernel(Args a, BwdArgs o
     }
     const f4 x0 = x_[0], x1 = c0 + 16 < Dve ? x_[1] : zero, y0 = y_[0], y1 = c0 + 16 < Dve ? y_[1] : zero;
     lds_barrier();
-    if (c0 + DVB < Dve) fetch(c0 + DVB);
+    if (c0 + DVB < Dve) fetch(h, c0 + DVB);
+    else if (!ONE && h + 1 < h0 + G) fetch(h + 1, 0);
 #pragma unroll
     for (int j = 0; j < 4; ++j) sdot = fmaf(x0[j], y0[j], fmaf(x1[j], y1[j], sdot));
+    part_ends();
     const Op16<SP> a0 = cut<SP>(x0), a1 = cut<SP>(x1), b0 = cut<SP>(y0), b1 = cut<SP>(y1);
 #pragma unroll
     for (int ti = 0; ti < NT; ++ti) {
@@ -772,6 +795,8 @@ __global__ void __launch_bounds__(64 * DKT) delta_grads_kernel(Args a, BwdArgs o
   sdot = wave_sum(sdot);
   if (lane == 0) l.sd[wave] = sdot;
   lds_barrier();  // the values are done with
+  turn();
+  part_ends();
 
   // W1, W2 in their place, and the row and column sums of what the decays see of them
 #pragma unroll
@@ -817,9 +842,9 @@ __global__ void __launch_bounds__(64 * DKT) delta_grads_kernel(Args a, BwdArgs o
   }
   lds_barrier();
 
-  // this wave's 16 key columns of dQ^T and dK^T
-  f4 dQ[NT], dK[NT];
-  const int kc = 16 * wave;
+  turn();
+  part_ends();
+  // this wave's key columns of dQ^T and dK^T
   auto row_of = [&](const float* W, int ti, int tj) { return row4(W + (ti * (ti + 1) / 2 + tj) * TS + l16 * TL + 4 * kq); };
   auto col_of = [&](const float* W, int ti, int tj) { return col4(W + (ti * (ti + 1) / 2 + tj) * TS + 4 * kq * TL + l16, TL); };
 #pragma unroll
@@ -834,6 +859,7 @@ __global__ void __launch_bounds__(64 * DKT) delta_grads_kernel(Args a, BwdArgs o
       d1 = fmaf(k[r], GR[ti][r], d1);
       d2 = fmaf(k[r], GU[ti][r], d2);
     }
+    part_ends();
     f4 x = ga * GO[ti], w = zero, z = zero;
 #pragma unroll
     for (int t2 = 0; t2 < 2; ++t2) {
@@ -849,42 +875,17 @@ __global__ void __launch_bounds__(64 * DKT) delta_grads_kernel(Args a, BwdArgs o
       if (tb >= ti) wb += col_of(W2, tb, ti);
       w = mm32(kt, cut<SP>(wa * st.rk4(ta)), cut<SP>(wb * st.rk4(tb)), w);
     }
-    dQ[ti] = a.scale * x;
-    dK[ti] = w + a.scale * z - (be * ga) * GR[ti] + e * GU[ti];
-    float d3 = 0.f, d4 = 0.f;
+    dQ[ti] += a.scale * x;
+    dK[ti] += w + a.scale * z - (be * ga) * GR[ti] + e * GU[ti];
+    float dd[3] = {d0, d1, d2};
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      d3 = fmaf(q[r], dQ[ti][r], d3);
-      d4 = fmaf(k[r], dK[ti][r], d4);
-    }
-    float dd[5] = {d0, d1, d2, d3, d4};
-#pragma unroll
-    for (int y = 0; y < 5; ++y) {
+    for (int y = 0; y < 3; ++y) {
       dd[y] += __shfl_xor(dd[y], 16, 64);
       dd[y] += __shfl_xor(dd[y], 32, 64);
       if (kq == 0) l.dots[y][wave][i] = dd[y];
     }
   }
   lds_barrier();
-#pragma unroll
-  for (int ti = 0; ti < NT; ++ti) {
-    const int i = 16 * ti + l16;
-    if (a.normalize) {
-      float dq = 0.f, dk = 0.f;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        dq += l.dots[3][w][i];
-        dk += l.dots[4][w][i];
-      }
-      dQ[ti] = st.gates[192 + i] * (dQ[ti] - dq * st.q_of(i, kc + 4 * kq));
-      dK[ti] = st.gates[256 + i] * (dK[ti] - dk * st.k_of(i, kc + 4 * kq));
-    }
-    if (t0 + i < a.T && kc + 4 * kq < a.Dk) {
-      const bool live = t0 + i < len;
-      put(o.dq, i, kc + 4 * kq, live ? dQ[ti] : zero);
-      put(o.dk, i, kc + 4 * kq, live ? dK[ti] : zero);
-    }
-  }
   if (wave == 0) {
     const int i = lane;
     float go = 0.f, gr = 0.f, gu = 0.f;
@@ -920,13 +921,58 @@ __global__ void __launch_bounds__(64 * DKT) delta_grads_kernel(Args a, BwdArgs o
       o.db[(long)(t0 + i) * BH + bh] = t0 + i < len ? db : 0.f;
     }
   }
+  } while (!ONE && ++h < h0 + G);
+
+  turn();
+  // through the scaling to unit length
+  if (a.normalize) {
+#pragma unroll
+    for (int ti = 0; ti < NT; ++ti) {
+      const int i = 16 * ti + l16;
+      const f4 q = st.q_of(i, kc + 4 * kq), k = st.k_of(i, kc + 4 * kq);
+      float dd[2] = {0.f, 0.f};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        dd[0] = fmaf(q[r], dQ[ti][r], dd[0]);
+        dd[1] = fmaf(k[r], dK[ti][r], dd[1]);
+      }
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        dd[y] += __shfl_xor(dd[y], 16, 64);
+        dd[y] += __shfl_xor(dd[y], 32, 64);
+        if (kq == 0) l.dots[3 + y][wave][i] = dd[y];
+      }
+    }
+  }
+  lds_barrier();
+#pragma unroll
+  for (int ti = 0; ti < NT; ++ti) {
+    const int i = 16 * ti + l16;
+    if (a.normalize) {
+      float dq = 0.f, dk = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        dq += l.dots[3][w][i];
+        dk += l.dots[4][w][i];
+      }
+      dQ[ti] = st.gates[192 + i] * (dQ[ti] - dq * st.q_of(i, kc + 4 * kq));
+      dK[ti] = st.gates[256 + i] * (dK[ti] - dk * st.k_of(i, kc + 4 * kq));
+    }
+    if (t0 + i < a.T && kc + 4 * kq < a.Dk) {
+      const bool live = t0 + i < len;
+      put(o.dq, i, kc + 4 * kq, live ? dQ[ti] : zero);
+      put(o.dk, i, kc + 4 * kq, live ? dK[ti] : zero);
+    }
+  }
 }
 
-// Per-value-head dq, dk in fp32 -> the sum over the value heads that share a key head, rounded once.
+// Per-value-head dq and dk in fp32 -> the sums over the value heads that share a key head, rounded once.
 template <typename T>
-__global__ void delta_head_sum_kernel(const float* x, T* y, long n, int rep, int Dk) {
+__global__ void delta_head_sum_kernel(const float* xq, const float* xk, T* yq, T* yk, long n, int rep, int Dk) {
   const long i = (long)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= n) return;
+  const float* x = blockIdx.y ? xk : xq;
+  T* y = blockIdx.y ? yk : yq;
   const long row = i / Dk, d = i % Dk;
   float v = 0.f;
   for (int r = 0; r < rep; ++r) v += x[(row * rep + r) * Dk + d];
@@ -956,9 +1002,14 @@ static void launch_c(const Args& a, const BwdArgs& o, bool per_value_head, hipSt
     }
     if (nvs <= 4) launch_walk<T, DKT, 4, false>(a, o, st);
     else launch_walk<T, DKT, 8, false>(a, o, st);
-    const int lds = (int)sizeof(GradsLds<T, DKT>);
-    allow_lds<delta_grads_kernel<T, DKT>>(lds);
-    delta_grads_kernel<T, DKT><<<BH * a.N, 64 * DKT, lds, st>>>(a, o, per_value_head ? 1 : 0);
+    const int lds = (int)sizeof(GradsLds<T, DKT>), G = per_value_head ? 1 : a.Hv / a.Hk;
+    if (G == 1) {
+      allow_lds<delta_grads_kernel<T, DKT, true>>(lds);
+      delta_grads_kernel<T, DKT, true><<<BH * a.N, 64 * DKT, lds, st>>>(a, o, 1);
+    } else {
+      allow_lds<delta_grads_kernel<T, DKT, false>>(lds);
+      delta_grads_kernel<T, DKT, false><<<BH / G * a.N, 64 * DKT, lds, st>>>(a, o, G);
+    }
   }
 }
 
@@ -980,11 +1031,11 @@ void launch_delta_bwd(const Args& a, const BwdArgs& o, int C, bool is_bf16, bool
   else launch_t<float>(a, o, C, per_value_head, st);
 }
 
-void launch_delta_head_sum(const float* x, void* y, long rows, int rep, int Dk, bool is_bf16, hipStream_t st) {
+void launch_delta_head_sum(const float* xq, const float* xk, void* yq, void* yk, long rows, int rep, int Dk, bool is_bf16, hipStream_t st) {
   const long n = rows * Dk;
-  const dim3 g((unsigned)((n + 255) / 256));
-  if (is_bf16) delta_head_sum_kernel<bf16><<<g, 256, 0, st>>>(x, reinterpret_cast<bf16*>(y), n, rep, Dk);
-  else delta_head_sum_kernel<float><<<g, 256, 0, st>>>(x, reinterpret_cast<float*>(y), n, rep, Dk);
+  const dim3 g((unsigned)((n + 255) / 256), 2);
+  if (is_bf16) delta_head_sum_kernel<bf16><<<g, 256, 0, st>>>(xq, xk, reinterpret_cast<bf16*>(yq), reinterpret_cast<bf16*>(yk), n, rep, Dk);
+  else delta_head_sum_kernel<float><<<g, 256, 0, st>>>(xq, xk, reinterpret_cast<float*>(yq), reinterpret_cast<float*>(yk), n, rep, Dk);
 }
 
 }  // namespace delta

@@ -83,80 +83,162 @@ __global__ void __launch_bounds__(512) delta_short_kernel(Args a, FwdOut o) {
   }
 }
 
+// One workgroup a chunk and G value heads that share a key head: the products k_j . k_i and q_i . k_j serve them all.
 template <typename T, int DKT>
-__global__ void __launch_bounds__(256) delta_pairs_kernel(Args a, float* pairs) {
-  constexpr int C = 64, LD = 16 * DKT + 4, NT = 4;
+struct PairsLds {
+  static constexpr bool SP = sizeof(T) == 2;
+  static constexpr int LD = SP ? 16 * DKT + 8 : 16 * DKT + 4;  // bf16 rows raw, in the order of place(); fp32 rows of unit length
+  typename std::conditional<SP, uint16_t, float>::type K[64 * LD], Q[64 * LD];
+  Gates<64> s;
+  float A[4 * TS];  // the four diagonal tiles
+};
+
+template <typename T, int DKT>
+__global__ void __launch_bounds__(256) delta_pairs_kernel(Args a, float* pairs, int G) {
+  using L = PairsLds<T, DKT>;
+  constexpr bool SP = L::SP;
+  constexpr int C = 64, LD = L::LD, NE = DKT;
   extern __shared__ __align__(16) unsigned char lds[];
-  Gates<C>& s = *reinterpret_cast<Gates<C>*>(lds);
-  float* K = reinterpret_cast<float*>(lds + sizeof(Gates<C>));
-  float* Q = K + C * LD;
-  float* A = Q + C * LD;  // the four diagonal tiles
+  L& l = *reinterpret_cast<L*>(lds);
+  Gates<C>& s = l.s;
 
   const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4, wave = threadIdx.x >> 6;
-  const int BH = a.B * a.Hv, bh = blockIdx.x % BH, n = blockIdx.x / BH, t0 = n * C;
-  const int b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
+  const int Hg = a.Hv / G, bg = blockIdx.x % (a.B * Hg), n = blockIdx.x / (a.B * Hg), t0 = n * C;
+  const int b = bg / Hg, h0 = (bg % Hg) * G, hk = h0 / (a.Hv / a.Hk);
   const int len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
   if (t0 >= len) return;
-  float* out = pairs + ((long)bh * a.N + n) * PAIR_FLOATS;
-  if (wave == 3) chunk_gates<C>(a, s, b, h, t0, len, lane);
-  load_rows<T, DKT, C, 4>(K, s.rk, reinterpret_cast<const T*>(a.k) + (long)b * a.kb + (long)hk * a.kh, a.kt, a.Dk, t0, len, a.veck,
-                       a.normalize, a.eps);
-  load_rows<T, DKT, C, 4>(Q, s.rq, reinterpret_cast<const T*>(a.q) + (long)b * a.qb + (long)hk * a.qh, a.qt, a.Dk, t0, len, a.vecq,
-                       a.normalize, a.eps);
-  lds_barrier();
-  // the diagonal tiles first: their inverses follow while the others are still made
-  for (int x = wave; x < 10; x += 4) {
-    const int ti = x < 4 ? x : x < 7 ? x - 3 : x < 9 ? x - 5 : 3, tj = x < 4 ? x : x < 7 ? x - 4 : x < 9 ? x - 7 : 0;
-    const int xi = (16 * ti + l16) * LD + 4 * kq;
-    const float* kj = K + (16 * tj + l16) * LD + 4 * kq;
-    f4 dk = {0.f, 0.f, 0.f, 0.f}, dq = dk;
+  const T* kp = reinterpret_cast<const T*>(a.k) + (long)b * a.kb + (long)hk * a.kh;
+  const T* qp = reinterpret_cast<const T*>(a.q) + (long)b * a.qb + (long)hk * a.qh;
+  if constexpr (!SP) {
+    load_rows<T, DKT, C, 4>(l.K, s.rk, kp, a.kt, a.Dk, t0, len, a.veck, a.normalize, a.eps);
+    load_rows<T, DKT, C, 4>(l.Q, s.rq, qp, a.qt, a.Dk, t0, len, a.vecq, a.normalize, a.eps);
+  } else {
+    const int sub = threadIdx.x & 15, c0 = sub * NE, D = a.Dk;
+    auto rows = [&](uint16_t* M, float* rn, const T* src, long st, bool vec) {
+      T x[4][NE];
 #pragma unroll
-    for (int m = 0; m < DKT; ++m) {
-      const f4 k = row4(kj + 16 * m), ki = row4(K + xi + 16 * m), qi = row4(Q + xi + 16 * m);
+      for (int r = 0; r < 4; ++r) {
+        const T* p = src + (long)max(0, min(t0 + (int)(threadIdx.x >> 4) + 16 * r, len - 1)) * st;
+        if (vec) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        dk = mfma4(k[j], ki[j], dk);
-        dq = mfma4(k[j], qi[j], dq);
-      }
-    }
-    const int i = 16 * ti + l16, j0 = 16 * tj + 4 * kq, t = ti * (ti + 1) / 2 + tj;
-    const double Gi = s.G[i];
-    const int segi = s.seg[i];
-    const float be = s.beta[i];
+          for (int j = 0; j < NE; j += 2)
+            *reinterpret_cast<uint32_t*>(&x[r][j]) = *reinterpret_cast<const uint32_t*>(p + min(c0 + j, D - 2));
+        } else {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float m = pair_decay<C>(s, i, j0 + r, Gi, segi);
-      dk[r] = j0 + r < i ? be * m * dk[r] : 0.f;
-      dq[r] = a.scale * m * dq[r];
-    }
-    *reinterpret_cast<f4*>(out + (PAIR_A + t) * 256 + l16 * 16 + 4 * kq) = dk;
-    *reinterpret_cast<f4*>(out + (PAIR_P + t) * 256 + l16 * 16 + 4 * kq) = dq;
-    if (ti == tj) {  // this wave's own tile: no barrier between its writes and its reads
-      float* d = A + ti * TS;
-      *reinterpret_cast<f4*>(d + l16 * TL + 4 * kq) = dk;
-      __builtin_amdgcn_wave_barrier();
-      float c[16];
-#pragma unroll
-      for (int i2 = 0; i2 < 16; ++i2) {
-        float v = i2 == l16 ? 1.f : 0.f;
-#pragma unroll
-        for (int m4 = 0; m4 < i2; m4 += 4) {
-          const f4 r = row4(d + i2 * TL + m4);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (m4 + j < i2) v = fmaf(-r[j], c[m4 + j], v);
+          for (int j = 0; j < NE; ++j) x[r][j] = p[min(c0 + j, D - 1)];
         }
-        c[i2] = v;
       }
 #pragma unroll
-      for (int i2 = 0; i2 < 16; ++i2)
-        if ((i2 >> 2) == kq) out[(PAIR_T + ti) * 256 + i2 * 16 + l16] = c[i2];
-    }
+      for (int r = 0; r < 4; ++r) {
+        const int i = (threadIdx.x >> 4) + 16 * r;
+        float ss = 0.f;
+#pragma unroll
+        for (int j = 0; j < NE; ++j) {
+          if (t0 + i >= len || c0 + j >= D) x[r][j].x = 0;
+          const float f = ld1(&x[r][j]);
+          ss = fmaf(f, f, ss);
+          M[i * LD + place(c0 + j)] = x[r][j].x;
+        }
+        const float nn = a.normalize ? 1.f / sqrtf(row16_sum(ss) + a.eps) : 1.f;
+        if (sub == 0) rn[i] = nn;
+      }
+    };
+    rows(l.K, s.rk, kp, a.kt, a.veck);
+    rows(l.Q, s.rq, qp, a.qt, a.vecq);
   }
-  float* g = out + PAIR_TILES * 256;
-  const int i = threadIdx.x & 63;
-  g[threadIdx.x] = wave == 0 ? s.beta[i] : wave == 1 ? s.gam[i] : wave == 2 ? s.e[i] : s.rq[i];
-  if (wave == 0) g[256 + i] = s.rk[i];
+  if (wave == 3) chunk_gates<C>(a, s, b, h0, t0, len, lane);
+  lds_barrier();
+
+  // This wave's tiles x = wave, wave + 4, wave + 8, the diagonal ones first: their inverses follow while the others wait.
+  auto tile_of = [](int x, int& ti, int& tj) {
+    ti = x < 4 ? x : x < 7 ? x - 3 : x < 9 ? x - 5 : 3;
+    tj = x < 4 ? x : x < 7 ? x - 4 : x < 9 ? x - 7 : 0;
+  };
+  f4 kk[3], qk[3];
+#pragma unroll
+  for (int y = 0; y < 3; ++y) {
+    kk[y] = qk[y] = f4{0.f, 0.f, 0.f, 0.f};
+    const int x = wave + 4 * y;
+    if (x >= 10) continue;
+    int ti, tj;
+    tile_of(x, ti, tj);
+    if constexpr (SP) {
+      const int at = 8 * kq, kj = (16 * tj + l16) * LD + at, xi = (16 * ti + l16) * LD + at;
+#pragma unroll
+      for (int m2 = 0; m2 < DKT / 2; ++m2) {
+        const b8 k = *reinterpret_cast<const b8*>(l.K + kj + 32 * m2);
+        kk[y] = mfma32(k, *reinterpret_cast<const b8*>(l.K + xi + 32 * m2), kk[y]);
+        qk[y] = mfma32(k, *reinterpret_cast<const b8*>(l.Q + xi + 32 * m2), qk[y]);
+      }
+      const f4 rj = row4(s.rk + 16 * tj + 4 * kq);
+      kk[y] *= rj * s.rk[16 * ti + l16];
+      qk[y] *= rj * s.rq[16 * ti + l16];
+    } else {
+      const int kj = (16 * tj + l16) * LD + 4 * kq, xi = (16 * ti + l16) * LD + 4 * kq;
+#pragma unroll
+      for (int m = 0; m < DKT; ++m) {
+        const f4 k = row4(l.K + kj + 16 * m), ki = row4(l.K + xi + 16 * m), qi = row4(l.Q + xi + 16 * m);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          kk[y] = mfma4(k[j], ki[j], kk[y]);
+          qk[y] = mfma4(k[j], qi[j], qk[y]);
+        }
+      }
+    }
+    qk[y] *= a.scale;
+  }
+  for (int g = 0; g < G; ++g) {
+    if (g > 0) {
+      lds_barrier();
+      if (wave == 3) chunk_gates<C>(a, s, b, h0 + g, t0, len, lane);
+      lds_barrier();
+    }
+    float* out = pairs + (((long)b * a.Hv + h0 + g) * a.N + n) * PAIR_FLOATS;
+#pragma unroll
+    for (int y = 0; y < 3; ++y) {
+      const int x = wave + 4 * y;
+      if (x >= 10) continue;
+      int ti, tj;
+      tile_of(x, ti, tj);
+      const int i = 16 * ti + l16, j0 = 16 * tj + 4 * kq, t = ti * (ti + 1) / 2 + tj;
+      const double Gi = s.G[i];
+      const int segi = s.seg[i];
+      const float be = s.beta[i];
+      f4 dk, dq;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float m = pair_decay<C>(s, i, j0 + r, Gi, segi);
+        dk[r] = j0 + r < i ? be * m * kk[y][r] : 0.f;
+        dq[r] = m * qk[y][r];
+      }
+      *reinterpret_cast<f4*>(out + (PAIR_A + t) * 256 + l16 * 16 + 4 * kq) = dk;
+      *reinterpret_cast<f4*>(out + (PAIR_P + t) * 256 + l16 * 16 + 4 * kq) = dq;
+      if (y == 0) {  // diagonal: this wave's own tile, no barrier between its writes and its reads
+        float* d = l.A + ti * TS;
+        *reinterpret_cast<f4*>(d + l16 * TL + 4 * kq) = dk;
+        __builtin_amdgcn_wave_barrier();
+        float c[16];
+#pragma unroll
+        for (int i2 = 0; i2 < 16; ++i2) {
+          float v = i2 == l16 ? 1.f : 0.f;
+#pragma unroll
+          for (int m4 = 0; m4 < i2; m4 += 4) {
+            const f4 r = row4(d + i2 * TL + m4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (m4 + j < i2) v = fmaf(-r[j], c[m4 + j], v);
+          }
+          c[i2] = v;
+        }
+#pragma unroll
+        for (int i2 = 0; i2 < 16; ++i2)
+          if ((i2 >> 2) == kq) out[(PAIR_T + ti) * 256 + i2 * 16 + l16] = c[i2];
+      }
+    }
+    float* gt = out + PAIR_TILES * 256;
+    gt[threadIdx.x] = wave == 0 ? s.beta[lane] : wave == 1 ? s.gam[lane] : wave == 2 ? s.e[lane] : s.rq[lane];
+    if (wave == 0) gt[256 + lane] = s.rk[lane];
+  }
 }
 
 template <typename T, int DKT, int NWT, bool MAP>
@@ -319,15 +401,17 @@ __global__ void __launch_bounds__(64 * NWT) delta_walk_kernel(Args a, FwdOut o) 
 }
 
 // Joins the segments: S_{s+1} = Pseg_s S_s + Rseg_s (REV: dS_s = Pseg_s^T dS_{s+1} + Xseg_s).  One workgroup per 16
-// columns, one wave per 16 rows; the state goes through LDS, the next segment's map is on its way meanwhile.
+// columns, one wave per 16 rows; the state goes through LDS in three bf16 parts, the next two segments' maps are on their way
+// meanwhile.  A chain of steps that wait for each other: with fp32 products (1024 cycles a wave) a step of 128 x 128 took 2.0 us.
 template <int DKT, bool REV>
 __global__ void __launch_bounds__(64 * DKT) delta_scan_kernel(const float* first, const float* P, const float* R, float* out, int nseg,
                                                               int Dk, int Dv) {
-  constexpr int DKp = 16 * DKT, LD = DKp + 4;
-  __shared__ __align__(16) float S[2][16 * LD];
+  constexpr int DKp = 16 * DKT, LD = DKp + 8;
+  __shared__ __align__(16) uint16_t S[2][3][16 * LD];
   const int lane = threadIdx.x & 63, m = threadIdx.x >> 6, l16 = lane & 15, kq = lane >> 4;
-  const int nvs = (Dv + 15) >> 4, bh = blockIdx.x / nvs, strip = blockIdx.x % nvs, dv = 16 * strip + l16;
-  f4 s, x[2][DKT], r[2];
+  // the strips of a head BH workgroups apart: on one chiplet, whose L2 then has the head's maps, where 8 divides BH
+  const int nvs = (Dv + 15) >> 4, BH = gridDim.x / nvs, bh = blockIdx.x % BH, strip = blockIdx.x / BH, dv = 16 * strip + l16;
+  f4 s, x[3][DKT], r[3];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int d = 16 * m + 4 * kq + j;
@@ -342,26 +426,37 @@ __global__ void __launch_bounds__(64 * DKT) delta_scan_kernel(const float* first
       xs[k] = REV ? col4(p + (16 * k + 4 * kq) * DKp + 16 * m + l16, DKp) : row4(p + (16 * m + l16) * DKp + 16 * k + 4 * kq);
     rs = row4(R + native(at(i)));
   };
-  auto step = [&](int i, const f4* xs, const f4& rs, float* l) {
+  auto step = [&](int i, const f4* xs, const f4& rs, uint16_t (*l)[16 * LD]) {
     *reinterpret_cast<f4*>(out + native(at(i))) = s;
-    *reinterpret_cast<f4*>(l + l16 * LD + 16 * m + 4 * kq) = s;
+    const Op16<true> c = cut3(s);
+    const int w = l16 * LD + place(16 * m + 4 * kq);
+    *reinterpret_cast<u2*>(l[0] + w) = c.p0;
+    *reinterpret_cast<u2*>(l[1] + w) = c.p1;
+    *reinterpret_cast<u2*>(l[2] + w) = c.p2;
     lds_barrier();  // two buffers: the one before is free once every wave is here
     f4 n0 = rs, n1 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < DKT; k += 2) {
-      n0 = mm16(xs[k], row4(l + l16 * LD + 16 * k + 4 * kq), n0);
-      n1 = mm16(xs[k + 1], row4(l + l16 * LD + 16 * k + 16 + 4 * kq), n1);
+      const int a = l16 * LD + 16 * k + 8 * kq;
+      const u4 p0 = *reinterpret_cast<const u4*>(l[0] + a), p1 = *reinterpret_cast<const u4*>(l[1] + a), p2 = *reinterpret_cast<const u4*>(l[2] + a);
+      const Op16<true> b0 = {p0.xy, p1.xy, p2.xy}, b1 = {p0.zw, p1.zw, p2.zw};
+      if (k & 2) n1 = mm32(cut3(xs[k]), cut3(xs[k + 1]), b0, b1, n1);
+      else n0 = mm32(cut3(xs[k]), cut3(xs[k + 1]), b0, b1, n0);
     }
     s = n0 + n1;
   };
   const int last = nseg - 1;  // the last segment's first state is the end of it
   fetch(0, x[0], r[0]);
-  for (int i = 0; i < last; i += 2) {
-    fetch(min(i + 1, last), x[1], r[1]);
-    step(i, x[0], r[0], S[0]);
+  fetch(min(1, last), x[1], r[1]);
+  for (int i = 0; i < last; i += 3) {
+    fetch(min(i + 2, last), x[2], r[2]);
+    step(i, x[0], r[0], S[i & 1]);
     if (i + 1 >= last) break;
-    fetch(min(i + 2, last), x[0], r[0]);
-    step(i + 1, x[1], r[1], S[1]);
+    fetch(min(i + 3, last), x[0], r[0]);
+    step(i + 1, x[1], r[1], S[(i + 1) & 1]);
+    if (i + 2 >= last) break;
+    fetch(min(i + 4, last), x[1], r[1]);
+    step(i + 2, x[2], r[2], S[i & 1]);
   }
   *reinterpret_cast<f4*>(out + native(at(last))) = s;
 }
@@ -381,9 +476,10 @@ static void launch_dk(const Args& a, const FwdOut& o, int C, hipStream_t st) {
     delta_short_kernel<T, DKT><<<BH, 64 * nvs, lds, st>>>(a, o);
     return;
   }
-  const int lds = (int)sizeof(Gates<64>) + (2 * 64 * (16 * DKT + 4) + 4 * TS) * (int)sizeof(float);
+  const int lds = (int)sizeof(PairsLds<T, DKT>);
   allow_lds<delta_pairs_kernel<T, DKT>>(lds);
-  delta_pairs_kernel<T, DKT><<<BH * a.N, 256, lds, st>>>(a, o.pairs);
+  const int G = a.B * a.Hk * a.N >= 512 ? a.Hv / a.Hk : 1;  // fewer workgroups than that leave CUs idle
+  delta_pairs_kernel<T, DKT><<<BH / G * a.N, 256, lds, st>>>(a, o.pairs, G);
   if (a.nseg > 1) {
     if (nvs + DKT <= 8) launch_walk<T, DKT, 8, true>(a, o, st);
     else launch_walk<T, DKT, 16, true>(a, o, st);
