@@ -1,6 +1,7 @@
 """Recurrent PPO agent (reference: ``sheeprl/algos/ppo_recurrent/agent.py:16-318``).
 
-features(obs) || prev_action -> [pre-MLP] -> LSTM -> [post-MLP] -> actor heads / critic.
+features(obs) || prev_action -> [pre-MLP] -> recurrent cell -> [post-MLP] -> actor heads / critic, the cell an LSTM
+(``algo.rnn.cell=lstm``) or gated-delta-rule blocks (``algo.rnn.cell=gated_delta``, no counterpart in the reference).
 
 Padded training sequences are run straight through the LSTM instead of ``pack_padded_sequence``:
 the padding sits at the END of every sequence, so each valid step's output is computed before any
@@ -20,6 +21,7 @@ from torch.distributions import Independent, Normal
 
 from sheeprl_prey_amd import ops
 from sheeprl_prey_amd.algos.ppo.agent import CNNEncoder, MLPEncoder, _act
+from sheeprl_prey_amd.models.gated_delta import GatedDeltaBlocks
 from sheeprl_prey_amd.models.models import MLP, MultiEncoder
 from sheeprl_prey_amd.utils.distribution import OneHotCategoricalValidateArgs
 
@@ -34,8 +36,11 @@ def _opt_mlp(input_dim: int, cfg) -> Tuple[nn.Module, int]:
 
 
 class RecurrentModel(nn.Module):
+    state_keys = ("prev_hx", "prev_cx")  # names of the states in the rollout buffer
+
     def __init__(self, input_size: int, lstm_hidden_size: int, pre_rnn_mlp_cfg, post_rnn_mlp_cfg) -> None:
         super().__init__()
+        self._hidden_size = lstm_hidden_size
         self._pre_mlp, d = _opt_mlp(input_size, pre_rnn_mlp_cfg)
         self._lstm = nn.LSTM(input_size=d, hidden_size=lstm_hidden_size, batch_first=False)
         self._post_mlp, self._output_dim = _opt_mlp(lstm_hidden_size, post_rnn_mlp_cfg)
@@ -43,6 +48,14 @@ class RecurrentModel(nn.Module):
     @property
     def output_dim(self) -> int:
         return self._output_dim
+
+    def initial_states(self, n: int, device=None) -> Tuple[Tensor, ...]:
+        z = torch.zeros(1, n, self._hidden_size, device=device)
+        return (z, z.clone())
+
+    def step(self, input: Tensor, states: Tuple[Tensor, ...]):
+        """One step without a gradient; the states given may be updated in place."""
+        return self(input, states)
 
     def forward(self, input: Tensor, states: Tuple[Tensor, Tensor], mask: Optional[Tensor] = None):
         x = self._pre_mlp(input)
@@ -52,6 +65,47 @@ class RecurrentModel(nn.Module):
             out, states = self._lstm(x, states)
         shape = out.shape
         return self._post_mlp(out.reshape(-1, shape[-1])).view(*shape[:-1], -1), states
+
+
+class GatedDeltaModel(nn.Module):
+    """The recurrent model with gated-delta-rule blocks in the LSTM's place: one matrix state a head instead of (h, c)."""
+
+    state_keys = ("prev_state",)
+
+    def __init__(self, input_size: int, cfg, pre_rnn_mlp_cfg, post_rnn_mlp_cfg) -> None:
+        super().__init__()
+        self._pre_mlp, d = _opt_mlp(input_size, pre_rnn_mlp_cfg)
+        self._blocks = GatedDeltaBlocks(d, cfg.hidden_size, cfg.num_blocks, cfg.key_heads, cfg.value_heads, cfg.key_dim, cfg.value_dim)
+        self._post_mlp, self._output_dim = _opt_mlp(cfg.hidden_size, post_rnn_mlp_cfg)
+
+    @property
+    def output_dim(self) -> int:
+        return self._output_dim
+
+    def initial_states(self, n: int, device=None) -> Tuple[Tensor, ...]:
+        return (self._blocks.initial_state(n, device),)
+
+    def _end(self, out: Tensor) -> Tensor:
+        return self._post_mlp(out.reshape(-1, out.shape[-1])).view(*out.shape[:-1], -1)
+
+    def step(self, input: Tensor, states: Tuple[Tensor, ...]):
+        """One step without a gradient, the state updated in place."""
+        return self._end(self._blocks.step(self._pre_mlp(input), states[0])), states
+
+    def forward(self, input: Tensor, states: Tuple[Tensor, ...], mask: Optional[Tensor] = None):
+        lengths = None if mask is None else mask.reshape(mask.shape[0], -1).sum(0, dtype=torch.int32)
+        out, state = self._blocks(self._pre_mlp(input), states[0], lengths)
+        return self._end(out), (state,)
+
+
+def build_recurrent_model(input_size: int, rnn_cfg) -> Tuple[nn.Module, int]:
+    """The cell that ``algo.rnn.cell`` names, and the width of its output."""
+    cell = str(rnn_cfg.get("cell", "lstm")).lower()
+    if cell == "lstm":
+        return RecurrentModel(input_size, rnn_cfg.lstm.hidden_size, rnn_cfg.pre_rnn_mlp, rnn_cfg.post_rnn_mlp), rnn_cfg.lstm.hidden_size
+    if cell == "gated_delta":
+        return GatedDeltaModel(input_size, rnn_cfg.gated_delta, rnn_cfg.pre_rnn_mlp, rnn_cfg.post_rnn_mlp), rnn_cfg.gated_delta.hidden_size
+    raise ValueError(f"algo.rnn.cell must be 'lstm' or 'gated_delta', got {rnn_cfg.cell!r}")
 
 
 class _SeqCNNEncoder(CNNEncoder):
@@ -71,7 +125,6 @@ class RecurrentPPOAgent(nn.Module):
         self.num_envs = num_envs
         self.actions_dim = list(actions_dim)
         self.distribution_cfg = distribution_cfg
-        self.rnn_hidden_size = rnn_cfg.lstm.hidden_size
         self.device = torch.device(device) if isinstance(device, str) else device
         in_channels = sum(prod(obs_space[k].shape[:-2]) for k in cnn_keys)
         mlp_input_dim = sum(obs_space[k].shape[0] for k in mlp_keys)
@@ -82,8 +135,7 @@ class RecurrentPPOAgent(nn.Module):
         self.feature_extractor = MultiEncoder(cnn_encoder, mlp_encoder)
         self.is_continuous = is_continuous
         features_dim = self.feature_extractor.output_dim
-        self.rnn = RecurrentModel(int(features_dim + sum(actions_dim)), rnn_cfg.lstm.hidden_size,
-                                  rnn_cfg.pre_rnn_mlp, rnn_cfg.post_rnn_mlp)
+        self.rnn, self.rnn_hidden_size = build_recurrent_model(int(features_dim + sum(actions_dim)), rnn_cfg)
 
         def mlp(out, cfg):
             n = cfg.mlp_layers
@@ -101,16 +153,15 @@ class RecurrentPPOAgent(nn.Module):
         self._initial_states = self.reset_hidden_states()
 
     @property
-    def initial_states(self) -> Tuple[Tensor, Tensor]:
+    def initial_states(self) -> Tuple[Tensor, ...]:
         return self._initial_states
 
     @initial_states.setter
     def initial_states(self, value) -> None:
         self._initial_states = value
 
-    def reset_hidden_states(self) -> Tuple[Tensor, Tensor]:
-        z = torch.zeros(1, self.num_envs, self.rnn_hidden_size, device=self.device)
-        return (z, z.clone())
+    def reset_hidden_states(self) -> Tuple[Tensor, ...]:
+        return self.rnn.initial_states(self.num_envs, self.device)
 
     def get_pre_dist(self, x: Tensor):
         feat = self.actor_backbone(x)
@@ -133,7 +184,7 @@ class RecurrentPPOAgent(nn.Module):
 
         return categorical_heads(list(pre_dist), actions)
 
-    def forward(self, obs: Dict[str, Tensor], prev_actions: Tensor, prev_states: Tuple[Tensor, Tensor],
+    def forward(self, obs: Dict[str, Tensor], prev_actions: Tensor, prev_states: Tuple[Tensor, ...],
                 actions: Optional[List[Tensor]] = None, mask: Optional[Tensor] = None):
         emb = self.feature_extractor(obs)
         out, states = self.rnn(torch.cat((emb, prev_actions), -1), prev_states, mask)
@@ -143,7 +194,10 @@ class RecurrentPPOAgent(nn.Module):
 
     def get_greedy_actions(self, obs: Dict[str, Tensor], prev_states, prev_actions: Tensor, mask=None):
         emb = self.feature_extractor(obs)
-        out, states = self.rnn(torch.cat((emb, prev_actions), -1), prev_states, mask)
+        x = torch.cat((emb, prev_actions), -1)
+        # single steps without a gradient may update the states they are given in place
+        single = mask is None and x.shape[0] == 1 and not torch.is_grad_enabled()
+        out, states = self.rnn.step(x, prev_states) if single else self.rnn(x, prev_states, mask)
         pre = self.get_pre_dist(out)
         if self.is_continuous:
             return (pre[0],), states

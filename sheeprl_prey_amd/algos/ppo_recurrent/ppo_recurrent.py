@@ -90,8 +90,8 @@ def train(runner, agent: RecurrentPPOAgent, optimizer, data: TensorDict, aggrega
         m = batch["mask"].unsqueeze(-1).float()
         obs = {k: batch[k] / 255.0 - 0.5 if k in cfg.cnn_keys.encoder else batch[k] for k in obs_keys}
         _, logprobs, entropies, values, _ = agent(
-            obs, prev_actions=batch["prev_actions"], prev_states=(batch["prev_hx"][:1], batch["prev_cx"][:1]),
-            actions=torch.split(batch["actions"], agent.actions_dim, dim=-1))
+            obs, prev_actions=batch["prev_actions"], prev_states=tuple(batch[k][:1] for k in agent.rnn.state_keys),
+            actions=torch.split(batch["actions"], agent.actions_dim, dim=-1), mask=batch["mask"])
         pg, vl, el = masked_losses(logprobs, batch["logprobs"], batch["advantages"], values, batch["values"],
                                    batch["returns"], entropies, m, cfg)
         loss = pg + cfg.algo.vf_coef * vl + cfg.algo.ent_coef * el
@@ -236,8 +236,8 @@ def main(runner, cfg: Dict[str, Any]):
             step_data["actions"] = actions
             step_data["rewards"] = rewards
             step_data["logprobs"] = logprobs
-            step_data["prev_hx"] = prev_states[0]
-            step_data["prev_cx"] = prev_states[1]
+            for k, s in zip(agent.rnn.state_keys, prev_states):
+                step_data[k] = s
             step_data["prev_actions"] = prev_actions
             step_data["returns"] = torch.zeros_like(rewards)
             step_data["advantages"] = torch.zeros_like(rewards)

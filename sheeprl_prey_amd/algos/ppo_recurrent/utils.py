@@ -25,7 +25,7 @@ def test(agent, runner, cfg: Dict[str, Any], log_dir: str) -> float:
     done = False
     cumulative_rew = 0.0
     obs = to_obs(env.reset(seed=cfg.seed)[0])
-    state = (torch.zeros(1, 1, agent.rnn_hidden_size, device=dev), torch.zeros(1, 1, agent.rnn_hidden_size, device=dev))
+    state = agent.rnn.initial_states(1, dev)
     actions = torch.zeros(1, 1, sum(agent.actions_dim), device=dev)
     while not done:
         acts, state = agent.get_greedy_actions(obs, state, actions)

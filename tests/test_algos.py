@@ -223,6 +223,15 @@ def test_ppo_recurrent(devices):
     _check_ckpt("ppo_rec", f"r{devices}", PPO_KEYS, False)
 
 
+@pytest.mark.timeout(180)
+@pytest.mark.parametrize("devices", [1, 2])
+def test_ppo_recurrent_gated_delta(devices):
+    _run(STD + ["exp=ppo_recurrent", "algo.rnn.cell=gated_delta", "algo.rnn.gated_delta.hidden_size=16", "algo.rnn.gated_delta.num_blocks=2",
+                "algo.rnn.gated_delta.key_dim=8", "algo.rnn.gated_delta.value_dim=8", "algo.rollout_steps=2", "per_rank_batch_size=1",
+                "per_rank_sequence_length=2", "algo.update_epochs=2", "root_dir=ppo_rec_delta", f"run_name=r{devices}"], devices)
+    _check_ckpt("ppo_rec_delta", f"r{devices}", PPO_KEYS, False)
+
+
 def test_pad_sequence_and_masked_losses():
     from sheeprl_prey_amd.algos.ppo_recurrent.ppo_recurrent import masked_losses
     from sheeprl_prey_amd.data.tensordict import TensorDict, pad_sequence

@@ -173,3 +173,88 @@ def test_norm_defaults_and_broadcast_gate():
 def test_norm_refusals(kw, match):
     with pytest.raises(ValueError, match=match):
         ops.gated_residual_norm(**{**dict(x=torch.zeros(4, 6), h=torch.zeros(4, 6)), **kw})
+
+
+# ------------------------------------------------------------------ the recurrent policy's blocks
+def _blocks(num_blocks=2, **kw):
+    from sheeprl_prey_amd.models import GatedDeltaBlocks
+
+    torch.manual_seed(0)
+    m = GatedDeltaBlocks(7, 12, num_blocks, **{**dict(key_heads=1, value_heads=2, key_dim=5, value_dim=6), **kw})
+    with torch.no_grad():
+        for p in m.parameters():
+            p.add_(0.1 * torch.randn_like(p))
+    return m
+
+
+def test_blocks_step_by_step_are_the_sequence():
+    m = _blocks()
+    x, state = torch.randn(5, 3, 7), m.initial_state(3)
+    out, last = m(x, state)
+    assert out.shape == (5, 3, 12) and last.shape == (1, 3, m.state_size) and not state.any()
+    with torch.no_grad():
+        steps = torch.cat([m.step(x[t:t + 1], state) for t in range(5)])
+    torch.testing.assert_close(out, steps)
+    torch.testing.assert_close(last, state)
+
+
+def test_blocks_lengths_are_the_sequences_alone():
+    m = _blocks()
+    x, state = torch.randn(6, 2, 7), torch.randn(1, 2, m.state_size)
+    out, last = m(x, state, lengths=torch.tensor([4, 6]))
+    a, la = m(x[:4, :1], state[:, :1])
+    torch.testing.assert_close(out[:4, :1], a)
+    torch.testing.assert_close(last[:, :1], la)
+    first = torch.zeros(6, 2, 1)
+    first[3] = 1
+    out, last = m(x, state, is_first=first)
+    b, lb = m(x[3:], torch.zeros_like(state))
+    torch.testing.assert_close(out[3:], b)
+    torch.testing.assert_close(last, lb)
+
+
+def test_blocks_gradients_reach_every_parameter_and_agree_with_differences():
+    m = _blocks().double()
+    x = torch.randn(4, 2, 7, dtype=torch.float64)
+    w = torch.randn(4, 2, 12, dtype=torch.float64)
+
+    def loss():
+        # the stream is fp32 by design: this test follows the same operations in fp64
+        s, u = m.input(x), None
+        u = torch.nn.functional.layer_norm(s, (12,), m.norm_weight[0], m.norm_bias[0], m.eps)
+        states = m._states(torch.zeros(1, 2, m.state_size, dtype=torch.float64))
+        for i in range(m.num_blocks):
+            (q, k, v, _, _), gate = m._project(u, i)
+            a, b = m.proj[i](u).split(m._sizes, -1)[3:5]
+            decay = -torch.nn.functional.softplus(a) * m.rate[i].exp()
+            o, _ = ops.gated_delta(q, k, v, decay, torch.sigmoid(b), states[:, i])
+            s, u = m._close(s, o, gate, i)
+        return (u * w).sum()
+
+    loss().backward()
+    g = torch.Generator().manual_seed(3)
+    for n, p in m.named_parameters():
+        assert p.grad is not None and p.grad.abs().max() > 0, n
+        d = torch.randn(p.shape, generator=g, dtype=torch.float64)
+        with torch.no_grad():
+            p.add_(1e-5 * d)
+            up = loss()
+            p.sub_(2e-5 * d)
+            down = loss()
+            p.add_(1e-5 * d)
+        # central differences: h^2 = 1e-10 of the third derivative, and 2^-52 / h of the loss
+        assert abs((up - down) / 2e-5 - (p.grad * d).sum()) <= 1e-6 * (1 + p.grad.norm() * d.norm()), n
+
+
+@pytest.mark.parametrize("kw,match", [(dict(num_blocks=0), "num_blocks"), (dict(key_heads=2, value_heads=3), "multiple of")])
+def test_blocks_refusals(kw, match):
+    with pytest.raises(ValueError, match=match):
+        _blocks(**kw)
+
+
+def test_recurrent_ppo_refuses_another_cell():
+    from sheeprl_prey_amd.algos.ppo_recurrent.agent import build_recurrent_model
+    from sheeprl_prey_amd.utils.utils import dotdict
+
+    with pytest.raises(ValueError, match="algo.rnn.cell"):
+        build_recurrent_model(4, dotdict({"cell": "gru"}))
