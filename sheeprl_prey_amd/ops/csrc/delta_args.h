@@ -36,7 +36,9 @@ struct FwdOut {
   float* U;         // [BH, N, C, Dvp], or null
   float* Sseg;      // [BH, nseg, ceil(Dv / 16), DKp / 16, 64, 4] each segment's first state (nseg > 1), as the registers hold it
   float* Rseg;      // the same: a segment's last state from a zero first state
-  float* Pseg;      // [BH, nseg, DKp, DKp] the map from a segment's first to its last state
+  // the map from a segment's first to its last state, tile by tile as the products that join segments read it (a wave's
+  // read is 1 KB in a row): Pseg by rows, and transposed for the backward pass (or null)
+  float *Pseg, *Ptr;  // [BH, nseg, DKp / 16, DKp / 16, 64, 4]
 };
 
 struct BwdArgs {
@@ -44,7 +46,7 @@ struct BwdArgs {
   long ot, ob, oh;
   int vecv, vecg;  // v and dout can be read four at a time
   const float* dlast;  // [B, Hv, Dk, Dv] contiguous, or null
-  const float *Sc, *U, *Pseg, *pairs;
+  const float *Sc, *U, *pairs, *Ptr;
   float* dSc;   // [BH, N, DKp, Dvp] gradient of each chunk's last state
   float* dR;    // [BH, N, C, Dvp]
   float* Xseg;   // as Rseg: the gradient of a segment's first state where that of its last is zero
@@ -56,8 +58,8 @@ struct BwdArgs {
 
 void launch_delta_fwd(const Args& a, const FwdOut& o, int C, bool is_bf16, hipStream_t st);
 void launch_delta_bwd(const Args& a, const BwdArgs& o, int C, bool is_bf16, bool per_value_head, hipStream_t st);
-void launch_delta_scan_rev(const float* dlast, const float* P, const float* X, float* dS, int BH, int nseg, int Dk, int Dv,
-                           hipStream_t st);
+void launch_delta_scan(const float* first, const float* P, const float* X, float* S, int BH, int nseg, int Dk, int Dv, bool rev,
+                       hipStream_t st);
 void launch_delta_head_sum(const float* xq, const float* xk, void* yq, void* yk, long rows, int rep, int Dk, bool is_bf16, hipStream_t st);
 // delta_step.hip: the recurrent form; S2 (the state after it) may be a.state itself
 void launch_delta_steps(const Args& a, void* out, float* S2, long sb, long sh, bool is_bf16, hipStream_t st);

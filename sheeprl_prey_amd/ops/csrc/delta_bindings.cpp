@@ -101,30 +101,32 @@ struct DeltaOpts {
   bool normalize;
 };
 
-// operands as delta_check and the conversions above leave them, each with a unit last stride
+// operands as delta_check and the conversions above leave them, each with a unit last stride; single steps (lead = 1) come
+// without the time axis
 srl::delta::Args delta_args(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& decay, const Tensor& beta,
-                            const Tensor& first, const Tensor& lengths, const DeltaOpts& o) {
+                            const Tensor& first, const Tensor& lengths, const DeltaOpts& o, int lead = 2) {
   using namespace srl::delta;
   Args a{};
   a.q = q.data_ptr(), a.k = k.data_ptr(), a.v = v.data_ptr();
   a.g = decay.data_ptr<float>(), a.beta = beta.data_ptr<float>();
-  a.qt = q.stride(0), a.qb = q.stride(1), a.qh = q.stride(2);
-  a.kt = k.stride(0), a.kb = k.stride(1), a.kh = k.stride(2);
-  a.vt = v.stride(0), a.vb = v.stride(1), a.vh = v.stride(2);
-  a.gt = decay.stride(0), a.gb = decay.stride(1), a.gh = decay.stride(2);
-  a.bt = beta.stride(0), a.bb = beta.stride(1), a.bh_ = beta.stride(2);
+  const int i = lead - 1;  // the batch axis
+  a.qb = q.stride(i), a.qh = q.stride(i + 1), a.kb = k.stride(i), a.kh = k.stride(i + 1), a.vb = v.stride(i), a.vh = v.stride(i + 1);
+  a.gb = decay.stride(i), a.gh = decay.stride(i + 1), a.bb = beta.stride(i), a.bh_ = beta.stride(i + 1);
+  if (lead == 2) a.qt = q.stride(0), a.kt = k.stride(0), a.vt = v.stride(0), a.gt = decay.stride(0), a.bt = beta.stride(0);
   if (first.defined()) {
     a.first = reinterpret_cast<const uint8_t*>(first.data_ptr());
-    a.ft = first.stride(0), a.fb = first.stride(1);
+    a.fb = first.stride(i);
+    if (lead == 2) a.ft = first.stride(0);
   }
   if (lengths.defined()) a.lengths = lengths.data_ptr<int>();
-  a.T = (int)v.size(0), a.B = (int)v.size(1), a.Hk = (int)q.size(2), a.Hv = (int)v.size(2), a.Dk = (int)q.size(3), a.Dv = (int)v.size(3);
+  a.T = lead == 2 ? (int)v.size(0) : 1, a.B = (int)v.size(i), a.Hk = (int)q.size(i + 1), a.Hv = (int)v.size(i + 1), a.Dk = (int)q.size(i + 2),
+  a.Dv = (int)v.size(i + 2);
   a.normalize = o.normalize, a.scale = (float)o.scale, a.eps = (float)o.eps;
   // wide reads of a row: 16 lanes take a sixteenth of the padded width each
   const int Dk = a.Dk, ne = Dk <= 32 ? 2 : Dk <= 64 ? 4 : 8, bytes = std::min<int>(16, ne * (int)q.element_size());
   auto wide = [&](const Tensor& t) {
     bool ok = Dk % ne == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % bytes == 0;
-    for (int i = 0; i < 3; ++i) ok = ok && t.stride(i) * t.element_size() % bytes == 0;
+    for (int d = 0; d <= lead; ++d) ok = ok && t.stride(d) * t.element_size() % bytes == 0;
     return ok;
   };
   a.vecq = wide(q), a.veck = wide(k);
@@ -159,7 +161,10 @@ struct Workspace {
   Tensor make(const Tensor& like) const { return torch::empty({n}, like.options().dtype(torch::kFloat32)); }
 };
 
-// What a forward pass leaves for the backward pass, in one workspace: Sc, U, Pseg, pairs
+// the maps of all segments
+int64_t map_floats(const srl::delta::Args& a) { return (int64_t)a.B * a.Hv * a.nseg * dkp(a.Dk) * dkp(a.Dk); }
+
+// What a forward pass leaves for the backward pass, in one workspace: Sc, U, the transposed maps, pairs
 struct DeltaSaved {
   int64_t Sc, U, P, pairs, n;
   DeltaSaved(const srl::delta::Args& a, int C) {
@@ -167,7 +172,7 @@ struct DeltaSaved {
     Workspace w;
     Sc = w.add(BH * a.N * DKp * Dvp);
     U = w.add(BH * a.N * C * Dvp);
-    P = w.add(a.nseg > 1 ? BH * a.nseg * DKp * DKp : 0);
+    P = w.add(a.nseg > 1 ? map_floats(a) : 0);
     pairs = w.add(C == 64 ? BH * a.N * srl::delta::PAIR_FLOATS : 0);
     n = w.n;
   }
@@ -190,17 +195,18 @@ std::pair<Tensor, Tensor> delta_forward(const Tensor& q, const Tensor& k, const 
   if (saved) {
     *saved = torch::empty({at.n}, decay.options());
     float* p = saved->data_ptr<float>();
-    o.Sc = p + at.Sc, o.U = p + at.U, o.Pseg = p + at.P, o.pairs = p + at.pairs;
+    o.Sc = p + at.Sc, o.U = p + at.U, o.pairs = p + at.pairs;
+    if (a.nseg > 1) o.Ptr = p + at.P;
   }
   Tensor ws;
   if (a.nseg > 1 || !saved) {
     Workspace w;
     const int64_t segs = a.nseg > 1 ? BH * a.nseg * DKp : 0, s = w.add(segs * Dvp), r = w.add(segs * Dvp);
-    const int64_t m = w.add(saved ? 0 : segs * DKp), pr = w.add(!saved && C == 64 ? BH * a.N * srl::delta::PAIR_FLOATS : 0);
+    const int64_t m = w.add(segs ? map_floats(a) : 0), pr = w.add(!saved && C == 64 ? BH * a.N * srl::delta::PAIR_FLOATS : 0);
     ws = w.make(q);
     float* p = ws.data_ptr<float>();
-    o.Sseg = p + s, o.Rseg = p + r;
-    if (!saved) o.Pseg = p + m, o.pairs = p + pr;
+    o.Sseg = p + s, o.Rseg = p + r, o.Pseg = p + m;
+    if (!saved) o.pairs = p + pr;
   }
   srl::delta::launch_delta_fwd(a, o, C, q.scalar_type() == torch::kBFloat16, cur());
   launched("gated_delta");
@@ -255,7 +261,7 @@ struct GatedDeltaFn : public torch::autograd::Function<GatedDeltaFn> {
     const DeltaSaved at(a, C);
     TORCH_CHECK(s[7].numel() == at.n, "gated_delta: the plan changed between the passes");
     const float* sp = s[7].data_ptr<float>();
-    o.Sc = sp + at.Sc, o.U = sp + at.U, o.Pseg = sp + at.P, o.pairs = sp + at.pairs;
+    o.Sc = sp + at.Sc, o.U = sp + at.U, o.pairs = sp + at.pairs, o.Ptr = sp + at.P;
     // dq and dk of shared key heads: one workgroup a key head where those fill the 256 CUs twice (4096 steps x 2 x 8: the
     // separate sums cost 54 us more), else one a value head and a sum
     const bool shared = a.Hk != a.Hv && (C == 16 || (int64_t)a.B * a.Hk * a.N < 512), bf = q.scalar_type() == torch::kBFloat16;
@@ -288,13 +294,13 @@ struct GatedDeltaFn : public torch::autograd::Function<GatedDeltaFn> {
   }
 };
 
-// The recurrent form over all T steps; the state after them goes to `after` (which may be `state`)
+// The recurrent form over all steps; the state after them goes to `after` (which may be `state`)
 Tensor delta_steps(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& decay, const Tensor& beta, const Tensor& state,
-                   const Tensor& first, const Tensor& lengths, const DeltaOpts& opt, const Tensor& after) {
-  auto a = delta_args(q, k, v, decay, beta, first, lengths, opt);
+                   const Tensor& first, const Tensor& lengths, const DeltaOpts& opt, const Tensor& after, int lead) {
+  auto a = delta_args(q, k, v, decay, beta, first, lengths, opt, lead);
   a.state = fp(state);
   const c10::DeviceGuard guard(q.device());
-  auto out = torch::empty({a.T, a.B, a.Hv, a.Dv}, v.options());
+  auto out = torch::empty(v.sizes(), v.options());
   srl::delta::launch_delta_steps(a, out.data_ptr(), after.data_ptr<float>(), after.stride(0), after.stride(1),
                                  q.scalar_type() == torch::kBFloat16, cur());
   launched("gated_delta");
@@ -319,7 +325,7 @@ std::pair<Tensor, Tensor> gated_delta(Tensor q, Tensor k, Tensor v, Tensor decay
   }
   if (T <= RECURRENT_MAX_STEPS) {
     auto last = torch::empty({B, v.size(2), q.size(3), v.size(3)}, decay.options());
-    auto out = delta_steps(q, k, v, decay, beta, state, first, lengths, opt, last);
+    auto out = delta_steps(q, k, v, decay, beta, state, first, lengths, opt, last, 2);
     return {out, last};
   }
   return delta_forward(q, k, v, decay, beta, state, first, lengths, opt, nullptr);
@@ -347,9 +353,7 @@ Tensor gated_delta_step(Tensor q, Tensor k, Tensor v, Tensor decay, Tensor beta,
   }
   const DeltaOpts opt{scale.has_value() ? *scale : 1.0 / std::sqrt((double)Dk), eps, normalize};
   if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
-  return delta_steps(unit_last(q).unsqueeze(0), unit_last(k).unsqueeze(0), unit_last(v).unsqueeze(0), f32(decay).unsqueeze(0),
-                     f32(beta).unsqueeze(0), state, first.defined() ? first.unsqueeze(0) : first, Tensor(), opt, state)
-      .squeeze(0);
+  return delta_steps(unit_last(q), unit_last(k), unit_last(v), f32(decay), f32(beta), state, first, Tensor(), opt, state, 1);
 }
 
 // ------------------------------------------------------------------ gated residual norms

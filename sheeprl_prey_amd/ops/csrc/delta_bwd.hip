@@ -998,7 +998,7 @@ static void launch_c(const Args& a, const BwdArgs& o, bool per_value_head, hipSt
     if (a.nseg > 1) {
       if (nvs <= 4) launch_walk<T, DKT, 4, true>(a, o, st);
       else launch_walk<T, DKT, 8, true>(a, o, st);
-      launch_delta_scan_rev(o.dlast, o.Pseg, o.Xseg, o.dSseg, BH, a.nseg, a.Dk, a.Dv, st);
+      launch_delta_scan(o.dlast, o.Ptr, o.Xseg, o.dSseg, BH, a.nseg, a.Dk, a.Dv, true, st);
     }
     if (nvs <= 4) launch_walk<T, DKT, 4, false>(a, o, st);
     else launch_walk<T, DKT, 8, false>(a, o, st);

@@ -378,11 +378,17 @@ __global__ void __launch_bounds__(64 * NWT) delta_walk_kernel(Args a, FwdOut o) 
 #pragma unroll
       for (int m = 0; m < DKT; ++m) *reinterpret_cast<f4*>(p + m * 256) = S[m];
     } else {
-      float* p = o.Pseg + ((long)bh * a.nseg + seg) * DKp * DKp + dv;
+      const int col = wave - nvs;  // the tile column
+      float* p = o.Pseg + ((long)bh * a.nseg + seg) * DKp * DKp + col * 256 + ((l16 >> 2) * 16 + 4 * kq) * 4 + (l16 & 3);
 #pragma unroll
       for (int m = 0; m < DKT; ++m)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) p[(16 * m + 4 * kq + r) * DKp] = S[m][r];
+        for (int r = 0; r < 4; ++r) p[m * DKT * 256 + 4 * r] = S[m][r];
+      if (o.Ptr) {
+        float* t = o.Ptr + ((long)bh * a.nseg + seg) * DKp * DKp + col * DKT * 256 + lane * 4;
+#pragma unroll
+        for (int m = 0; m < DKT; ++m) *reinterpret_cast<f4*>(t + m * 256) = S[m];
+      }
     }
     return;
   }
@@ -400,9 +406,9 @@ __global__ void __launch_bounds__(64 * NWT) delta_walk_kernel(Args a, FwdOut o) 
   }
 }
 
-// Joins the segments: S_{s+1} = Pseg_s S_s + Rseg_s (REV: dS_s = Pseg_s^T dS_{s+1} + Xseg_s).  One workgroup per 16
-// columns, one wave per 16 rows; the state goes through LDS in three bf16 parts, the next two segments' maps are on their way
-// meanwhile.  A chain of steps that wait for each other: with fp32 products (1024 cycles a wave) a step of 128 x 128 took 2.0 us.
+// Joins the segments: S_{s+1} = Pseg_s S_s + Rseg_s, or backwards (REV) dS_s = Pseg_s^T dS_{s+1} + Xseg_s with the maps
+// transposed.  One workgroup per 16 columns, one wave per 16 rows; the state goes through LDS in three bf16 parts, and the
+// next two maps are on their way meanwhile.
 template <int DKT, bool REV>
 __global__ void __launch_bounds__(64 * DKT) delta_scan_kernel(const float* first, const float* P, const float* R, float* out, int nseg,
                                                               int Dk, int Dv) {
@@ -411,7 +417,7 @@ __global__ void __launch_bounds__(64 * DKT) delta_scan_kernel(const float* first
   const int lane = threadIdx.x & 63, m = threadIdx.x >> 6, l16 = lane & 15, kq = lane >> 4;
   // the strips of a head BH workgroups apart: on one chiplet, whose L2 then has the head's maps, where 8 divides BH
   const int nvs = (Dv + 15) >> 4, BH = gridDim.x / nvs, bh = blockIdx.x % BH, strip = blockIdx.x / BH, dv = 16 * strip + l16;
-  f4 s, x[3][DKT], r[3];
+  f4 s, r[3], x[3][DKT];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int d = 16 * m + 4 * kq + j;
@@ -420,10 +426,9 @@ __global__ void __launch_bounds__(64 * DKT) delta_scan_kernel(const float* first
   auto at = [&](int i) { return (long)bh * nseg + (REV ? nseg - 1 - i : i); };
   auto native = [&](long g) { return ((g * nvs + strip) * DKT + m) * 256 + lane * 4; };
   auto fetch = [&](int i, f4* xs, f4& rs) {
-    const float* p = P + at(i) * DKp * DKp;
+    const float* p = P + at(i) * DKp * DKp + m * DKT * 256 + lane * 4;
 #pragma unroll
-    for (int k = 0; k < DKT; ++k)
-      xs[k] = REV ? col4(p + (16 * k + 4 * kq) * DKp + 16 * m + l16, DKp) : row4(p + (16 * m + l16) * DKp + 16 * k + 4 * kq);
+    for (int k = 0; k < DKT; ++k) xs[k] = row4(p + k * 256);
     rs = row4(R + native(at(i)));
   };
   auto step = [&](int i, const f4* xs, const f4& rs, uint16_t (*l)[16 * LD]) {
@@ -434,16 +439,15 @@ __global__ void __launch_bounds__(64 * DKT) delta_scan_kernel(const float* first
     *reinterpret_cast<u2*>(l[1] + w) = c.p1;
     *reinterpret_cast<u2*>(l[2] + w) = c.p2;
     lds_barrier();  // two buffers: the one before is free once every wave is here
-    f4 n0 = rs, n1 = {0.f, 0.f, 0.f, 0.f};
+    f4 n[2] = {rs, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (int k = 0; k < DKT; k += 2) {
       const int a = l16 * LD + 16 * k + 8 * kq;
       const u4 p0 = *reinterpret_cast<const u4*>(l[0] + a), p1 = *reinterpret_cast<const u4*>(l[1] + a), p2 = *reinterpret_cast<const u4*>(l[2] + a);
       const Op16<true> b0 = {p0.xy, p1.xy, p2.xy}, b1 = {p0.zw, p1.zw, p2.zw};
-      if (k & 2) n1 = mm32(cut3(xs[k]), cut3(xs[k + 1]), b0, b1, n1);
-      else n0 = mm32(cut3(xs[k]), cut3(xs[k + 1]), b0, b1, n0);
+      n[(k >> 1) & 1] = mm32(cut3(xs[k]), cut3(xs[k + 1]), b0, b1, n[(k >> 1) & 1]);
     }
-    s = n0 + n1;
+    s = n[0] + n[1];
   };
   const int last = nseg - 1;  // the last segment's first state is the end of it
   fetch(0, x[0], r[0]);
@@ -483,7 +487,7 @@ static void launch_dk(const Args& a, const FwdOut& o, int C, hipStream_t st) {
   if (a.nseg > 1) {
     if (nvs + DKT <= 8) launch_walk<T, DKT, 8, true>(a, o, st);
     else launch_walk<T, DKT, 16, true>(a, o, st);
-    delta_scan_kernel<DKT, false><<<BH * nvs, 64 * DKT, 0, st>>>(a.state, o.Pseg, o.Rseg, o.Sseg, a.nseg, a.Dk, a.Dv);
+    launch_delta_scan(a.state, o.Pseg, o.Rseg, o.Sseg, BH, a.nseg, a.Dk, a.Dv, false, st);
   }
   if (nvs <= 4) launch_walk<T, DKT, 4, false>(a, o, st);
   else launch_walk<T, DKT, 8, false>(a, o, st);
@@ -501,12 +505,19 @@ void launch_delta_fwd(const Args& a, const FwdOut& o, int C, bool is_bf16, hipSt
   else launch_t<float>(a, o, C, st);
 }
 
-void launch_delta_scan_rev(const float* dlast, const float* P, const float* X, float* dS, int BH, int nseg, int Dk, int Dv,
-                           hipStream_t st) {
+template <int DKT>
+static void launch_scan(const float* first, const float* P, const float* X, float* S, int BH, int nseg, int Dk, int Dv, bool rev,
+                        hipStream_t st) {
   const int g = BH * ((Dv + 15) / 16);
-  if (Dk <= 32) delta_scan_kernel<2, true><<<g, 128, 0, st>>>(dlast, P, X, dS, nseg, Dk, Dv);
-  else if (Dk <= 64) delta_scan_kernel<4, true><<<g, 256, 0, st>>>(dlast, P, X, dS, nseg, Dk, Dv);
-  else delta_scan_kernel<8, true><<<g, 512, 0, st>>>(dlast, P, X, dS, nseg, Dk, Dv);
+  if (rev) delta_scan_kernel<DKT, true><<<g, 64 * DKT, 0, st>>>(first, P, X, S, nseg, Dk, Dv);
+  else delta_scan_kernel<DKT, false><<<g, 64 * DKT, 0, st>>>(first, P, X, S, nseg, Dk, Dv);
+}
+
+void launch_delta_scan(const float* first, const float* P, const float* X, float* S, int BH, int nseg, int Dk, int Dv, bool rev,
+                       hipStream_t st) {
+  if (Dk <= 32) launch_scan<2>(first, P, X, S, BH, nseg, Dk, Dv, rev, st);
+  else if (Dk <= 64) launch_scan<4>(first, P, X, S, BH, nseg, Dk, Dv, rev, st);
+  else launch_scan<8>(first, P, X, S, BH, nseg, Dk, Dv, rev, st);
 }
 
 }  // namespace delta

@@ -14,6 +14,7 @@ from typing import Optional, Tuple
 import torch
 from torch import Tensor
 
+import sheeprl_prey_amd.ops as ops
 from sheeprl_prey_amd.ops import reference as ref
 
 MAX_HEAD_DIM = 128
@@ -73,17 +74,9 @@ def _lengths(x: Optional[Tensor], B: int, device) -> Optional[Tensor]:
     return x.to(torch.int32).contiguous()
 
 
-def _ext():
-    from sheeprl_prey_amd import ops
-
-    return ops._ext()  # loud failure if missing
-
-
 def _fused(t: Tensor) -> bool:
     """The kernels take fp32 and bf16 as they come, so autocast regions use them too.  They check their operands as
     ``_check`` and its neighbours do here for the eager form."""
-    from sheeprl_prey_amd import ops
-
     return t.is_cuda and ops._FUSED
 
 
@@ -105,7 +98,7 @@ def gated_delta(
     Differentiable in ``q``, ``k``, ``v``, ``decay``, ``beta`` and ``state`` (once).  The sums, decays and states are fp32;
     outputs and gradients are rounded once to the operand's type, those of shared key heads after their sum."""
     if _fused(v) and v.numel() and q.numel():
-        return _ext().gated_delta(q, k, v, decay, beta, state, is_first, lengths, scale, normalize, eps)
+        return ops._ext().gated_delta(q, k, v, decay, beta, state, is_first, lengths, scale, normalize, eps)
     _check(q, k, v, decay, beta, state, ("T", "B"))
     T, B = v.shape[:2]
     first = _flags(is_first, (T, B), "is_first", v.device)
@@ -124,7 +117,7 @@ def gated_delta_step(
     :func:`gated_delta`; ``state`` fp32 ``[B, Hv, Dk, Dv]``, each ``[Dk, Dv]`` contiguous and none overlapping (a slice of a larger
     store of states is fine).  No gradient; a captured graph replays it on the same state."""
     if _fused(v) and v.numel() and q.numel():
-        return _ext().gated_delta_step(q, k, v, decay, beta, state, is_first, scale, normalize, eps)
+        return ops._ext().gated_delta_step(q, k, v, decay, beta, state, is_first, scale, normalize, eps)
     _check(q, k, v, decay, beta, state, ("B",))
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, decay, beta, state)):
         raise RuntimeError("gated_delta_step updates the state in place and has no gradient: use gated_delta, or torch.no_grad()")

@@ -6,6 +6,7 @@ from typing import Optional, Tuple, Union
 import torch
 from torch import Tensor
 
+import sheeprl_prey_amd.ops as ops
 from sheeprl_prey_amd.ops import reference as ref
 
 MAX_WIDTH = 8192
@@ -34,12 +35,9 @@ def gated_residual_norm(
     s1 = 1.0
     if scale is not None and not isinstance(scale, Tensor):
         s1, scale = float(scale), None
-    if x.is_cuda and x.numel():
-        from sheeprl_prey_amd import ops
-
-        if ops._FUSED:
-            return ops._ext().gated_residual_norm(x, h, gate, scale, post_weight, post_bias, pre_weight, pre_bias, norm == "layer",
-                                                  GATE_ACTS[act], eps, s1)
+    if x.is_cuda and ops._FUSED and x.numel():
+        return ops._ext().gated_residual_norm(x, h, gate, scale, post_weight, post_bias, pre_weight, pre_bias, norm == "layer",
+                                              GATE_ACTS[act], eps, s1)
     if x.dim() < 1 or h.shape != x.shape:
         raise ValueError(f"x and h must have one shape, got {tuple(x.shape)} and {tuple(h.shape)}")
     D = x.shape[-1]
