@@ -33,6 +33,8 @@ __device__ __forceinline__ uint32_t f2bf2(float lo, float hi) {
 }
 __device__ __forceinline__ uint16_t f2bf(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }
 struct bf16 { uint16_t x; };
+// the wave's number in its workgroup, in a scalar register: branches and addresses that go by it cost no vector registers
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 __device__ __forceinline__ float ld1(const float* p) { return *p; }
 __device__ __forceinline__ float ld1(const bf16* p) { return bf2f(p->x); }
 __device__ __forceinline__ void st1(float* p, float v) { *p = v; }
@@ -372,9 +374,19 @@ __device__ __forceinline__ f4 mm16o(const Op16<true>& a, const Op16<true>& b, f4
   return c + d;
 }
 
+// f(0), ..., f(N - 1) with compile-time indexes: arrays of operands stay in registers
+template <int I, int N, typename F>
+__device__ __forceinline__ void each(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    each<I + 1, N>(f);
+  }
+}
+
 // A chunk of 64 steps on its way from memory to LDS for the strip kernels: K (and Q) as they lie in memory, the pair tiles,
 // the gates.  fetch() starts the reads for the next chunk, commit() writes what has arrived to LDS: the reads have the whole
-// walk over the present chunk to arrive in.  MODE: 0 forward, 1 forward without Q and P (maps), 2 backward,
+// walk over the present chunk to arrive in, and are issued in three parts (K; Q; tiles and gates) between its products: all at
+// once they queue up, and the waves with them, for 2000 to 5000 of a chunk's 16000 to 23000 cycles.  MODE: 0 forward, 1 forward without Q and P (maps), 2 backward,
 // 3 without the tiles (gradients of q and k).
 // What the kernels read: k(ti, m2), q(ti, m2): rows of steps against 32 key columns; kt(m, t2), qt(m, t2): rows of key columns
 // against 32 steps; A (negated), P, Ti: tiles, transposed in the backward mode; rk4, rq4: factors that are not in k and q yet.
@@ -411,6 +423,11 @@ struct Stage<float, DKT, NWT, MODE> {
     int t = threadIdx.x;
     asm volatile("" : "+v"(t));
     tid = t, l16 = t & 15, kq = (t >> 4) & 3;
+  }
+  // all of a chunk at once
+  template <typename T>
+  __device__ __forceinline__ void fetch(const Args& a, const T* qp, const T* kp, const float* pair, int t0, int len) {
+    each<0, 3>([&](auto part) { fetch(part, a, qp, kp, pair, t0, len); });
   }
   __device__ __forceinline__ Exact32<false> rows(const float* M, int ti, int m2) const {
     const float* p = M + (16 * ti + l16) * LD + 32 * m2 + 4 * kq;
@@ -456,9 +473,12 @@ struct Stage<float, DKT, NWT, MODE> {
         for (int j = 0; j < NE; ++j) w[r][j] = p[r][min(c0 + j, D - 1)];
     }
   }
-  __device__ __forceinline__ void fetch(const Args& a, const float* qp, const float* kp, const float* pair, int t0, int len) {
-    rows_(rk_, kp, a.kt, a.Dk, t0, len, a.veck);
-    if constexpr (HQ) rows_(rq_, qp, a.qt, a.Dk, t0, len, a.vecq);
+  template <int P>
+  __device__ __forceinline__ void fetch(std::integral_constant<int, P>, const Args& a, const float* qp, const float* kp, const float* pair,
+                                        int t0, int len) {
+    if constexpr (P == 0) rows_(rk_, kp, a.kt, a.Dk, t0, len, a.veck);
+    if constexpr (P == 1 && HQ) rows_(rq_, qp, a.qt, a.Dk, t0, len, a.vecq);
+    if constexpr (P != 2) return;
 #pragma unroll
     for (int r = 0; r < RR; ++r) {
       const float* n = pair + PAIR_TILES * 256 + (tid >> 4) + r * 4 * NWT;
@@ -520,6 +540,11 @@ struct Stage<bf16, DKT, NWT, MODE> {
     asm volatile("" : "+v"(t));
     tid = t, l16 = t & 15, kq = (t >> 4) & 3;
   }
+  // all of a chunk at once
+  template <typename T>
+  __device__ __forceinline__ void fetch(const Args& a, const T* qp, const T* kp, const float* pair, int t0, int len) {
+    each<0, 3>([&](auto part) { fetch(part, a, qp, kp, pair, t0, len); });
+  }
   __device__ __forceinline__ Exact32<true> rows(const uint16_t* M, int ti, int m2) const {
     return {*reinterpret_cast<const u4*>(M + (16 * ti + l16) * LR + 32 * m2 + 8 * kq)};
   }
@@ -576,9 +601,12 @@ struct Stage<bf16, DKT, NWT, MODE> {
         for (int r = 0; r < 4; ++r) w[g][r] = (uint32_t)p[g][r][x].x | (uint32_t)p[g][r][y].x << 16;
     }
   }
-  __device__ __forceinline__ void fetch(const Args& a, const bf16* qp, const bf16* kp, const float* pair, int t0, int len) {
-    rows4(rk_, kp, a.kt, a.Dk, t0, len, a.veck);
-    if constexpr (HQ) rows4(rq_, qp, a.qt, a.Dk, t0, len, a.vecq);
+  template <int P>
+  __device__ __forceinline__ void fetch(std::integral_constant<int, P>, const Args& a, const bf16* qp, const bf16* kp, const float* pair,
+                                        int t0, int len) {
+    if constexpr (P == 0) rows4(rk_, kp, a.kt, a.Dk, t0, len, a.veck);
+    if constexpr (P == 1 && HQ) rows4(rq_, qp, a.qt, a.Dk, t0, len, a.vecq);
+    if constexpr (P != 2) return;
 #pragma unroll
     for (int x = 0; x < NT4; ++x) {
       const int at = min(tid + x * TH, TI::N * 64 - 64 + (tid & 63));  // 64 divides TH: at & 63 is the lane
@@ -635,14 +663,6 @@ struct Stage<bf16, DKT, NWT, MODE> {
 // a reload from memory waits for everything that is on its way.
 __device__ __forceinline__ void part_ends() { __builtin_amdgcn_sched_barrier(0); }
 
-// f(0), ..., f(N - 1) with compile-time indexes: arrays of operands stay in registers
-template <int I, int N, typename F>
-__device__ __forceinline__ void each(F&& f) {
-  if constexpr (I < N) {
-    f(std::integral_constant<int, I>{});
-    each<I + 1, N>(f);
-  }
-}
 // c + sum over x = X..N-1 of tile(x) operand(x): pairs of tiles where there are two
 template <int X, int N, typename FA, typename FB>
 __device__ __forceinline__ f4 mm_tiles(FA&& tile, FB&& operand, f4 c) {

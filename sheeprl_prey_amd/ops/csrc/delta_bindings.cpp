@@ -262,9 +262,9 @@ struct GatedDeltaFn : public torch::autograd::Function<GatedDeltaFn> {
     TORCH_CHECK(s[7].numel() == at.n, "gated_delta: the plan changed between the passes");
     const float* sp = s[7].data_ptr<float>();
     o.Sc = sp + at.Sc, o.U = sp + at.U, o.pairs = sp + at.pairs, o.Ptr = sp + at.P;
-    // dq and dk of shared key heads: one workgroup a key head where those fill the 256 CUs twice (4096 steps x 2 x 8: the
-    // separate sums cost 54 us more), else one a value head and a sum
-    const bool shared = a.Hk != a.Hv && (C == 16 || (int64_t)a.B * a.Hk * a.N < 512), bf = q.scalar_type() == torch::kBFloat16;
+    // dq and dk of shared key heads: one workgroup a key head where heads are wide (delta_grads_kernel) and fill the 256 CUs
+    // twice so (4096 steps x 2 x 8: the separate sums cost 54 us more), else one a value head and a sum
+    const bool shared = a.Hk != a.Hv && (C == 16 || a.Dk <= 64 || (int64_t)a.B * a.Hk * a.N < 512), bf = q.scalar_type() == torch::kBFloat16;
     Workspace w;
     const int64_t segs = a.nseg > 1 ? BH * a.nseg * DKp * Dvp : 0, heads = shared ? (int64_t)a.T * BH * a.Dk : 0;
     const int64_t ds = w.add(BH * a.N * DKp * Dvp), dr = w.add(BH * a.N * C * Dvp), x = w.add(segs), dss = w.add(segs), hq = w.add(heads),

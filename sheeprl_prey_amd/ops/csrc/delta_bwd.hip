@@ -30,7 +30,7 @@ __global__ void __launch_bounds__(512) delta_bwd_short_kernel(Args a, BwdArgs o)
   float* P = A + C * LC;
   float* Td = P + C * LC;
 
-  const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4, wave = wave_id(), nw = blockDim.x >> 6;
   const int BH = a.B * a.Hv, bh = blockIdx.x, b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
   const int Dvp = pitch(a.Dv), dv = 16 * wave + l16;
   const int len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(64 * NWT) delta_bwd_walk_kernel(Args a, BwdArg
   extern __shared__ __align__(16) unsigned char lds[];
   St st(lds);
 
-  const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4, wave = wave_id();
   const int BH = a.B * a.Hv, bh = blockIdx.x % BH, seg = blockIdx.x / BH;
   const int b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
   const int nvs = (a.Dv + 15) >> 4, dv = 16 * wave + l16;
@@ -147,18 +147,25 @@ __global__ void __launch_bounds__(64 * NWT) delta_bwd_walk_kernel(Args a, BwdArg
     f4 dy[NT], u[NT];
 #pragma unroll
     for (int ti = 0; ti < NT; ++ti) dy[ti] = dn.get(ti, t0, len, kq, gp && dv < a.Dv), u[ti] = zero;
-    if (n > n0) {
-      st.fetch(a, qp, kp, pairs + (long)(n - 1) * PAIR_FLOATS, t0 - C, len);
-      if (gp) dn.fetch(gcol, o.ot, t0 - C, len, kq);
+    // the next chunk on its way, a part at a time: see Stage
+    auto ahead = [&](auto part) {
+      if (n > n0) st.fetch(part, a, qp, kp, pairs + (long)(n - 1) * PAIR_FLOATS, t0 - C, len);
+    };
+    if (!works) {
+      each<0, 3>(ahead);
+      continue;
     }
-    if (!works) continue;
+    if (n > n0 && gp) dn.fetch(gcol, o.ot, t0 - C, len, kq);
     part_ends();
-#pragma unroll
-    for (int m2 = 0; m2 < DKT / 2; ++m2) {
+    each<0, DKT / 2>([&](auto M) {
+      constexpr int m2 = M;
       const Op16<SP> s0 = cut<SP>(S[2 * m2]), s1 = cut<SP>(S[2 * m2 + 1]);
 #pragma unroll
       for (int ti = 0; ti < NT; ++ti) u[ti] = mm32(st.k(ti, m2), s0, s1, u[ti]);
-    }
+      part_ends();
+      if constexpr (m2 < 2) ahead(M);
+    });
+    if constexpr (DKT == 2) ahead(std::integral_constant<int, 1>{});
     part_ends();
     // dR: backward substitution by blocks of 16 steps
     Op16<SP> ub[NT], db[NT];
@@ -170,6 +177,7 @@ __global__ void __launch_bounds__(64 * NWT) delta_bwd_walk_kernel(Args a, BwdArg
       r = mm_tiles<ti + 1, NT>([&](int x) { return st.A(x, ti); }, [&](auto x) { return ub[decltype(x)::value]; }, r);
       u[ti] = mm16o(st.Ti(ti), cut<SP>(r), zero);
       ub[ti] = cut<SP>(u[ti]);
+      if constexpr (ti == NT - 1) ahead(std::integral_constant<int, 2>{});
     });
     if (!MAP) {
       const long vstep = afresh((long)BH * a.Dv);
@@ -267,7 +275,7 @@ __global__ void __launch_bounds__(64 * DKT) delta_bwd_pair_kernel(Args a, BwdArg
   Gates<C>& s = l.s;
   float *sO = l.big_, *sR = sO + C * LV, *sU = sR + C * LV, *W1 = l.big_, *W2 = W1 + C * LC;
 
-  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, kq = lane >> 4, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, kq = lane >> 4, wave = wave_id();
   const int BH = a.B * a.Hv, bh = blockIdx.x % BH, n = blockIdx.x / BH, t0 = n * C;
   const int b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
   const int Dvp = pitch(a.Dv), Dve = 16 * ((a.Dv + 15) >> 4);
@@ -617,20 +625,24 @@ __device__ __forceinline__ f4 four(const bf16* p, int c, int D, bool vec) {
   return f4{ld1(p + min(c, D - 1)), ld1(p + min(c + 1, D - 1)), ld1(p + min(c + 2, D - 1)), ld1(p + min(c + 3, D - 1))};
 }
 
+// PRE: W1, W1^T and W2 + W2^T wait in LDS as the operands that all waves read, cut once, not by each of eight waves (half of
+// the vector instructions of the kernel); narrower heads keep the LDS for a second workgroup on the CU.
 template <typename T, int DKT>
 struct GradsLds {
-  static constexpr int NTL = 10, W = 2 * NTL * TS * 4, V = Values<T, 64 * DKT>::BYTES, BIG = W > V ? W : V;
+  static constexpr bool PRE = Stage<T, DKT, DKT, 3>::SP && DKT == 8;
+  static constexpr int NTL = 10, W = 2 * NTL * TS * 4, V = Values<T, 64 * DKT>::BYTES, P = W + (PRE ? 36 * 1536 : 0), BIG = P > V ? P : V;
   Gates<64> s;
   float rows[NTL][16], cols[NTL][16], rowb[NTL][16], dots[5][DKT][64], dRv[64], sd[DKT];
   __align__(16) unsigned char big[BIG], stage[Stage<T, DKT, DKT, 3>::BYTES];
 };
 
-// Chunks of 64: what sums over the value columns (the head of this file), one wave per 16 key columns.  A workgroup takes the
-// G value heads that share a key head one after the other and leaves the sum of their dq and dk; with few chunks (G = 1) the
-// heads go to workgroups of their own, and delta_head_sum_kernel adds them.
-// ONE: a single head (G = 1), whose sums live in fewer registers: two workgroups of narrow heads fit a CU.
+// Chunks of 64: what sums over the value columns (the head of this file), one wave per 16 key columns.  ONE: a value head a
+// workgroup, and delta_head_sum_kernel adds those that share a key head.  Else a workgroup takes the G value heads of a key
+// head one after the other and leaves the sum of their dq and dk, which is for heads wider than 64 alone, of which a CU holds
+// one workgroup in any case: of narrower ones it holds two, and 1024 steps x 32 x 8 heads of 64 took 281 us so and 363 us in
+// turn.
 template <typename T, int DKT, bool ONE>
-__global__ void __launch_bounds__(64 * DKT, ONE ? 2 : 1) delta_grads_kernel(Args a, BwdArgs o, int G_) {
+__global__ void __launch_bounds__(64 * DKT, ONE && DKT > 2 ? 2 : 1) delta_grads_kernel(Args a, BwdArgs o, int G_) {
   const int G = ONE ? 1 : G_;
   using L = GradsLds<T, DKT>;
   using St = Stage<T, DKT, DKT, 3>;
@@ -643,9 +655,10 @@ __global__ void __launch_bounds__(64 * DKT, ONE ? 2 : 1) delta_grads_kernel(Args
   St st(l.stage);
   Values<T, TH> val(l.big);
   float *W1 = reinterpret_cast<float*>(l.big), *W2 = W1 + NTL * TS;
+  u2* ops = reinterpret_cast<u2*>(W2 + NTL * TS);  // PRE: [36][part][lane]: 10 of W1, 10 of W1^T, 16 of W2 + W2^T
 
   int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, kq = lane >> 4;
-  const int wave = tid >> 6;
+  const int wave = wave_id();
   // the lane's place afresh in each turn over the heads: see afresh()
   auto turn = [&]() {
     st.turn();
@@ -693,33 +706,39 @@ __global__ void __launch_bounds__(64 * DKT, ONE ? 2 : 1) delta_grads_kernel(Args
   const long gt = o.dout ? o.ot : a.vt, gh = o.dout ? o.oh : a.vh;
   const long c_at = (long)b * a.Hv * a.N + n;  // the chunk of head h: c_at + h N
 
-  // the next DVB value columns on their way
+  // the next DVB value columns on their way, in four parts: issued all at once the reads of all waves queue up, and the waves
+  // with them, for as long as the products of a step take; between the products they cost a fraction of that
   f4 g_[RPT], r_[RPT], u_[RPT], v_[RPT], x_[2], y_[2];
-  auto fetch = [&](int h, int c0) {
+  auto fetch = [&](auto part, int h, int c0) {
+    constexpr int P = decltype(part)::value;
     const long ch = c_at + (long)h * a.N;
-    const float *up = o.U + ch * C * Dvp, *rp = o.dR + ch * C * Dvp;
-    const float* s0 = o.Sc + (ch * DKp + 16 * wave + l16) * Dvp + 4 * kq;
-    const float* ds = o.dSc + (ch * DKp + 16 * wave + l16) * Dvp + 4 * kq;
+    if constexpr (P < 3) {
 #pragma unroll
-    for (int x = 0; x < RPT; ++x) {
-      const int at = tid + x * TH, i = at / (DVB / 4), c = c0 + 4 * (at % (DVB / 4)), ce = min(c, Dve - 4);
-      const int t = min(t0 + i, len - 1);
-      r_[x] = row4(rp + i * Dvp + ce);
-      u_[x] = row4(up + i * Dvp + ce);
-      g_[x] = four(gp + t * gt + h * gh, c, a.Dv, o.vecg);
-      v_[x] = four(vp + t * a.vt + h * a.vh, c, a.Dv, o.vecv);
-    }
+      for (int x = 0; x < RPT; ++x) {
+        const int at = tid + x * TH, i = at / (DVB / 4), c = c0 + 4 * (at % (DVB / 4)), ce = min(c, Dve - 4);
+        const int t = min(t0 + i, len - 1);
+        if constexpr (P == 0) r_[x] = row4(o.dR + ch * C * Dvp + i * Dvp + ce);
+        if constexpr (P == 1) u_[x] = row4(o.U + ch * C * Dvp + i * Dvp + ce);
+        if constexpr (P == 2) {
+          g_[x] = four(gp + t * gt + h * gh, c, a.Dv, o.vecg);
+          v_[x] = four(vp + t * a.vt + h * a.vh, c, a.Dv, o.vecv);
+        }
+      }
+    } else {
+      const float* s0 = o.Sc + (ch * DKp + 16 * wave + l16) * Dvp + 4 * kq;
+      const float* ds = o.dSc + (ch * DKp + 16 * wave + l16) * Dvp + 4 * kq;
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      const int c = min(c0 + 16 * m, Dve - 16);
-      x_[m] = row4(s0 + c);
-      y_[m] = row4(ds + c);
+      for (int m = 0; m < 2; ++m) {
+        const int c = min(c0 + 16 * m, Dve - 16);
+        x_[m] = row4(s0 + c);
+        y_[m] = row4(ds + c);
+      }
     }
   };
 
   st.fetch(a, reinterpret_cast<const T*>(a.q) + (long)b * a.qb + (long)hk * a.qh, reinterpret_cast<const T*>(a.k) + (long)b * a.kb + (long)hk * a.kh,
            o.pairs + (c_at + (long)h0 * a.N) * PAIR_FLOATS, t0, len);
-  fetch(h0, 0);
+  each<0, 4>([&](auto part) { fetch(part, h0, 0); });
   f4 dQ[NT], dK[NT];
 #pragma unroll
   for (int ti = 0; ti < NT; ++ti) dQ[ti] = dK[ti] = zero;
@@ -733,12 +752,15 @@ __global__ void __launch_bounds__(64 * DKT, ONE ? 2 : 1) delta_grads_kernel(Args
   if (h > h0) lds_barrier();  // the head before is done with LDS
   turn();
   if (wave == NW - 1) chunk_gates<C>(a, s, b, h, t0, len, lane);
-  f4 GO[NT], GR[NT], GU[NT], D1[TPW], D2[TPW];
+  f4 GO[NT], GR[NT], GU[NT], D1[TPW], D2[TPW], pw[TPW];
   float dRv[RPT], sdot = 0.f;
 #pragma unroll
   for (int ti = 0; ti < NT; ++ti) GO[ti] = GR[ti] = GU[ti] = zero;
 #pragma unroll
-  for (int x = 0; x < TPW; ++x) D1[x] = D2[x] = zero;
+  for (int x = 0; x < TPW; ++x) {
+    D1[x] = D2[x] = zero;
+    pw[x] = row4(pair + (PAIR_P + min(wave + x * NW, NTL - 1)) * 256 + l16 * 16 + 4 * kq);
+  }
 #pragma unroll
   for (int x = 0; x < RPT; ++x) dRv[x] = 0.f;
 
@@ -760,20 +782,21 @@ __global__ void __launch_bounds__(64 * DKT, ONE ? 2 : 1) delta_grads_kernel(Args
     }
     const f4 x0 = x_[0], x1 = c0 + 16 < Dve ? x_[1] : zero, y0 = y_[0], y1 = c0 + 16 < Dve ? y_[1] : zero;
     lds_barrier();
-    if (c0 + DVB < Dve) fetch(h, c0 + DVB);
-    else if (!ONE && h + 1 < h0 + G) fetch(h + 1, 0);
+    const bool on = c0 + DVB < Dve, more = on || (!ONE && h + 1 < h0 + G);
+    const int hn = on ? h : h + 1, cn = on ? c0 + DVB : 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) sdot = fmaf(x0[j], y0[j], fmaf(x1[j], y1[j], sdot));
     part_ends();
     const Op16<SP> a0 = cut<SP>(x0), a1 = cut<SP>(x1), b0 = cut<SP>(y0), b1 = cut<SP>(y1);
-#pragma unroll
-    for (int ti = 0; ti < NT; ++ti) {
+    each<0, NT>([&](auto ti) {
+      if (more) fetch(ti, hn, cn);
       GO[ti] = mm32r(a0, a1, val.o(ti, l16, kq), GO[ti]);
       const auto r = val.r(ti, l16, kq);
       GR[ti] = mm32(a0, a1, r.a, r.b, GR[ti]);
       const auto u = val.u(ti, l16, kq);
       GU[ti] = mm32(b0, b1, u.a, u.b, GU[ti]);
-    }
+      part_ends();
+    });
 #pragma unroll
     for (int x = 0; x < TPW; ++x) {
       const int t = wave + x * NW;
@@ -798,6 +821,21 @@ __global__ void __launch_bounds__(64 * DKT, ONE ? 2 : 1) delta_grads_kernel(Args
   turn();
   part_ends();
 
+  auto put_op = [&](int x, f4 v) {
+    if constexpr (L::PRE) {
+      const Op16<true> c = cut3(v);
+      u2* p = ops + x * 192 + lane;
+      p[0] = c.p0, p[64] = c.p1, p[128] = c.p2;
+    }
+  };
+  auto get_op = [&](int x) -> Op16<SP> {
+    if constexpr (L::PRE) {
+      const u2* p = ops + x * 192 + lane;
+      return {p[0], p[64], p[128]};
+    } else {
+      return {};
+    }
+  };
   // W1, W2 in their place, and the row and column sums of what the decays see of them
 #pragma unroll
   for (int x = 0; x < TPW; ++x) {
@@ -806,7 +844,7 @@ __global__ void __launch_bounds__(64 * DKT, ONE ? 2 : 1) delta_grads_kernel(Args
       int ti, tj;
       lower_tile(t, ti, tj);
       const int i = 16 * ti + l16, j0 = 16 * tj + 4 * kq;
-      const f4 p = row4(pair + (PAIR_P + t) * 256 + l16 * 16 + 4 * kq);
+      const f4 p = pw[x];
       f4 kk = zero;
 #pragma unroll
       for (int m2 = 0; m2 < DKT / 2; ++m2) kk = mm32x(st.k(tj, m2), st.k(ti, m2), kk);
@@ -828,6 +866,7 @@ __global__ void __launch_bounds__(64 * DKT, ONE ? 2 : 1) delta_grads_kernel(Args
         const float cs = row16_sum(e);
         if (l16 == 0) l.cols[t][4 * kq + r] = cs;
       }
+      if constexpr (L::PRE) put_op(t, w1 * st.rk4(tj));
       *reinterpret_cast<f4*>(W1 + t * TS + l16 * TL + 4 * kq) = w1;
       *reinterpret_cast<f4*>(W2 + t * TS + l16 * TL + 4 * kq) = w2;
       rs += __shfl_xor(rs, 16, 64);
@@ -841,12 +880,45 @@ __global__ void __launch_bounds__(64 * DKT, ONE ? 2 : 1) delta_grads_kernel(Args
     }
   }
   lds_barrier();
-
   turn();
   part_ends();
-  // this wave's key columns of dQ^T and dK^T
   auto row_of = [&](const float* W, int ti, int tj) { return row4(W + (ti * (ti + 1) / 2 + tj) * TS + l16 * TL + 4 * kq); };
   auto col_of = [&](const float* W, int ti, int tj) { return col4(W + (ti * (ti + 1) / 2 + tj) * TS + 4 * kq * TL + l16, TL); };
+  // operands against steps of tile tk: rows of W1 and of W2 + W2^T, and of W1^T
+  auto w1_op = [&](int ti, int tk) -> Op16<SP> {
+    if constexpr (L::PRE) return tk <= ti ? get_op(ti * (ti + 1) / 2 + tk) : cut<SP>(zero);
+    else return cut<SP>(tk <= ti ? row_of(W1, ti, tk) * st.rk4(tk) : zero);
+  };
+  auto w1t_op = [&](int ti, int tk) -> Op16<SP> {
+    if constexpr (L::PRE) return tk >= ti ? get_op(NTL + tk * (tk + 1) / 2 + ti) : cut<SP>(zero);
+    else return cut<SP>(tk >= ti ? col_of(W1, tk, ti) * st.rq4(tk) : zero);
+  };
+  auto w2_sum = [&](int ti, int tk) {
+    f4 w = zero;
+    if (tk <= ti) w += row_of(W2, ti, tk);
+    if (tk >= ti) w += col_of(W2, tk, ti);
+    return w * st.rk4(tk);
+  };
+  auto w2_op = [&](int ti, int tk) -> Op16<SP> {
+    if constexpr (L::PRE) return get_op(2 * NTL + NT * ti + tk);
+    else return cut<SP>(w2_sum(ti, tk));
+  };
+  if constexpr (L::PRE) {
+    const int w0 = (int)afresh(wave);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int t = w0 + x * NW;
+      if (t < NT * NT) put_op(2 * NTL + t, w2_sum(t / NT, t % NT));
+      else if (t < NT * NT + NTL) {
+        int ti, tj;
+        lower_tile(t - NT * NT, ti, tj);
+        put_op(NTL + t - NT * NT, col_of(W1, ti, tj) * st.rq4(ti));
+      }
+    }
+    lds_barrier();
+    part_ends();
+  }
+  // this wave's key columns of dQ^T and dK^T
 #pragma unroll
   for (int ti = 0; ti < NT; ++ti) {
     const int i = 16 * ti + l16;
@@ -865,15 +937,12 @@ __global__ void __launch_bounds__(64 * DKT, ONE ? 2 : 1) delta_grads_kernel(Args
     for (int t2 = 0; t2 < 2; ++t2) {
       const int ta = 2 * t2, tb = 2 * t2 + 1;
       const Exact32<SP> kt = st.kt(wave, t2);
-      if (ta <= ti) x = mm32(kt, cut<SP>(row_of(W1, ti, ta) * st.rk4(ta)), cut<SP>(tb <= ti ? row_of(W1, ti, tb) * st.rk4(tb) : zero), x);
-      if (tb >= ti)
-        z = mm32(st.qt(wave, t2), cut<SP>(ta >= ti ? col_of(W1, ta, ti) * st.rq4(ta) : zero), cut<SP>(col_of(W1, tb, ti) * st.rq4(tb)), z);
-      f4 wa = zero, wb = zero;
-      if (ta <= ti) wa += row_of(W2, ti, ta);
-      if (ta >= ti) wa += col_of(W2, ta, ti);
-      if (tb <= ti) wb += row_of(W2, ti, tb);
-      if (tb >= ti) wb += col_of(W2, tb, ti);
-      w = mm32(kt, cut<SP>(wa * st.rk4(ta)), cut<SP>(wb * st.rk4(tb)), w);
+      if (ta <= ti) x = mm32(kt, w1_op(ti, ta), w1_op(ti, tb), x);
+      if (L::PRE) part_ends();
+      if (tb >= ti) z = mm32(st.qt(wave, t2), w1t_op(ti, ta), w1t_op(ti, tb), z);
+      if (L::PRE) part_ends();
+      w = mm32(kt, w2_op(ti, ta), w2_op(ti, tb), w);
+      if (L::PRE) part_ends();
     }
     dQ[ti] += a.scale * x;
     dK[ti] += w + a.scale * z - (be * ga) * GR[ti] + e * GU[ti];
@@ -966,17 +1035,26 @@ __global__ void __launch_bounds__(64 * DKT, ONE ? 2 : 1) delta_grads_kernel(Args
   }
 }
 
-// Per-value-head dq and dk in fp32 -> the sums over the value heads that share a key head, rounded once.
-template <typename T>
+// Per-value-head dq and dk in fp32 -> the sums over the value heads that share a key head, rounded once.  Bound by memory: V
+// neighbours a thread (4 where Dk allows).
+template <typename T, int V>
 __global__ void delta_head_sum_kernel(const float* xq, const float* xk, T* yq, T* yk, long n, int rep, int Dk) {
-  const long i = (long)blockIdx.x * blockDim.x + threadIdx.x;
+  const long i = ((long)blockIdx.x * blockDim.x + threadIdx.x) * V;
   if (i >= n) return;
   const float* x = blockIdx.y ? xk : xq;
-  T* y = blockIdx.y ? yk : yq;
+  T* y = (blockIdx.y ? yk : yq) + i;
   const long row = i / Dk, d = i % Dk;
-  float v = 0.f;
-  for (int r = 0; r < rep; ++r) v += x[(row * rep + r) * Dk + d];
-  st1(y + i, v);
+  x += row * rep * Dk + d;
+  if constexpr (V == 4) {
+    f4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int r = 0; r < rep; ++r) v += row4(x + (long)r * Dk);
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<f4*>(y) = v;
+    else *reinterpret_cast<u2*>(y) = part(v);
+  } else {
+    float v = 0.f;
+    for (int r = 0; r < rep; ++r) v += x[(long)r * Dk];
+    st1(y, v);
+  }
 }
 
 template <typename T, int DKT, int NWT, bool MAP>
@@ -1002,14 +1080,16 @@ static void launch_c(const Args& a, const BwdArgs& o, bool per_value_head, hipSt
     }
     if (nvs <= 4) launch_walk<T, DKT, 4, false>(a, o, st);
     else launch_walk<T, DKT, 8, false>(a, o, st);
-    const int lds = (int)sizeof(GradsLds<T, DKT>), G = per_value_head ? 1 : a.Hv / a.Hk;
-    if (G == 1) {
-      allow_lds<delta_grads_kernel<T, DKT, true>>(lds);
-      delta_grads_kernel<T, DKT, true><<<BH * a.N, 64 * DKT, lds, st>>>(a, o, 1);
-    } else {
-      allow_lds<delta_grads_kernel<T, DKT, false>>(lds);
-      delta_grads_kernel<T, DKT, false><<<BH / G * a.N, 64 * DKT, lds, st>>>(a, o, G);
+    const int lds = (int)sizeof(GradsLds<T, DKT>);
+    if constexpr (DKT == 8) {
+      if (const int G = a.Hv / a.Hk; G > 1 && !per_value_head) {
+        allow_lds<delta_grads_kernel<T, DKT, false>>(lds);
+        delta_grads_kernel<T, DKT, false><<<BH / G * a.N, 64 * DKT, lds, st>>>(a, o, G);
+        return;
+      }
     }
+    allow_lds<delta_grads_kernel<T, DKT, true>>(lds);
+    delta_grads_kernel<T, DKT, true><<<BH * a.N, 64 * DKT, lds, st>>>(a, o, 1);
   }
 }
 
@@ -1033,9 +1113,15 @@ void launch_delta_bwd(const Args& a, const BwdArgs& o, int C, bool is_bf16, bool
 
 void launch_delta_head_sum(const float* xq, const float* xk, void* yq, void* yk, long rows, int rep, int Dk, bool is_bf16, hipStream_t st) {
   const long n = rows * Dk;
-  const dim3 g((unsigned)((n + 255) / 256), 2);
-  if (is_bf16) delta_head_sum_kernel<bf16><<<g, 256, 0, st>>>(xq, xk, reinterpret_cast<bf16*>(yq), reinterpret_cast<bf16*>(yk), n, rep, Dk);
-  else delta_head_sum_kernel<float><<<g, 256, 0, st>>>(xq, xk, reinterpret_cast<float*>(yq), reinterpret_cast<float*>(yk), n, rep, Dk);
+  const int V = Dk % 4 == 0 ? 4 : 1;
+  const dim3 g((unsigned)((n / V + 255) / 256), 2);
+  auto launch = [&](auto* q, auto* k) {
+    using T = std::remove_pointer_t<decltype(q)>;
+    if (V == 4) delta_head_sum_kernel<T, 4><<<g, 256, 0, st>>>(xq, xk, q, k, n, rep, Dk);
+    else delta_head_sum_kernel<T, 1><<<g, 256, 0, st>>>(xq, xk, q, k, n, rep, Dk);
+  };
+  if (is_bf16) launch(reinterpret_cast<bf16*>(yq), reinterpret_cast<bf16*>(yk));
+  else launch(reinterpret_cast<float*>(yq), reinterpret_cast<float*>(yk));
 }
 
 }  // namespace delta

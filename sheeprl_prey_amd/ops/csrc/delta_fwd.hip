@@ -25,7 +25,7 @@ __global__ void __launch_bounds__(512) delta_short_kernel(Args a, FwdOut o) {
   float* P = A + C * LC;
   float* Td = P + C * LC;
 
-  const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4, wave = wave_id(), nw = blockDim.x >> 6;
   const int BH = a.B * a.Hv, bh = blockIdx.x, b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
   const int Dvp = pitch(a.Dv), dv = 16 * wave + l16;
   const int len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(256) delta_pairs_kernel(Args a, float* pairs, 
   L& l = *reinterpret_cast<L*>(lds);
   Gates<C>& s = l.s;
 
-  const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4, wave = wave_id();
   const int Hg = a.Hv / G, bg = blockIdx.x % (a.B * Hg), n = blockIdx.x / (a.B * Hg), t0 = n * C;
   const int b = bg / Hg, h0 = (bg % Hg) * G, hk = h0 / (a.Hv / a.Hk);
   const int len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(64 * NWT) delta_walk_kernel(Args a, FwdOut o) 
   extern __shared__ __align__(16) unsigned char lds[];
   St st(lds);
 
-  const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4, wave = wave_id();
   const int BH = a.B * a.Hv, bh = blockIdx.x % BH, seg = blockIdx.x / BH;
   const int b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
   const int nvs = (a.Dv + 15) >> 4;
@@ -308,25 +308,32 @@ __global__ void __launch_bounds__(64 * NWT) delta_walk_kernel(Args a, FwdOut o) 
     f4 u[NT];
 #pragma unroll
     for (int ti = 0; ti < NT; ++ti) u[ti] = st.beta(ti) * v.get(ti, t0, len, kq, vstrip && dv < a.Dv);
-    if (n + 1 < live) {
-      st.fetch(a, qp, kp, pairs + (long)(n + 1) * PAIR_FLOATS, t0 + C, len);
-      if (vstrip) v.fetch(vcol, a.vt, t0 + C, len, kq);
+    // the next chunk on its way, a part at a time: see Stage
+    auto ahead = [&](auto part) {
+      if (n + 1 < live) st.fetch(part, a, qp, kp, pairs + (long)(n + 1) * PAIR_FLOATS, t0 + C, len);
+    };
+    if (!works) {
+      each<0, 3>(ahead);
+      continue;
     }
-    if (!works) continue;
+    if (n + 1 < live && vstrip) v.fetch(vcol, a.vt, t0 + C, len, kq);
     part_ends();
     // K S0 and Q S0
     f4 ks[NT], y[NT];
 #pragma unroll
     for (int ti = 0; ti < NT; ++ti) ks[ti] = y[ti] = zero;
-#pragma unroll
-    for (int m2 = 0; m2 < DKT / 2; ++m2) {
+    each<0, DKT / 2>([&](auto M) {
+      constexpr int m2 = M;
       const Op16<SP> s0 = cut<SP>(S[2 * m2]), s1 = cut<SP>(S[2 * m2 + 1]);
 #pragma unroll
       for (int ti = 0; ti < NT; ++ti) {
         ks[ti] = mm32(st.k(ti, m2), s0, s1, ks[ti]);
         if constexpr (!MAP) y[ti] = mm32(st.q(ti, m2), s0, s1, y[ti]);
       }
-    }
+      part_ends();
+      if constexpr (m2 < 2) ahead(M);
+    });
+    if constexpr (DKT == 2) ahead(std::integral_constant<int, 1>{});
     part_ends();
     // U: forward substitution by blocks of 16 steps
     Op16<SP> ub[NT];
@@ -336,6 +343,7 @@ __global__ void __launch_bounds__(64 * NWT) delta_walk_kernel(Args a, FwdOut o) 
       r = mm_tiles<0, ti>([&](int x) { return st.A(ti, x); }, [&](auto x) { return ub[decltype(x)::value]; }, r);
       u[ti] = mm16o(st.Ti(ti), cut<SP>(r), zero);
       ub[ti] = cut<SP>(u[ti]);
+      if constexpr (ti == 0) ahead(std::integral_constant<int, 2>{});
     });
     part_ends();
     if constexpr (!MAP) {
@@ -414,7 +422,7 @@ __global__ void __launch_bounds__(64 * DKT) delta_scan_kernel(const float* first
                                                               int Dk, int Dv) {
   constexpr int DKp = 16 * DKT, LD = DKp + 8;
   __shared__ __align__(16) uint16_t S[2][3][16 * LD];
-  const int lane = threadIdx.x & 63, m = threadIdx.x >> 6, l16 = lane & 15, kq = lane >> 4;
+  const int lane = threadIdx.x & 63, m = wave_id(), l16 = lane & 15, kq = lane >> 4;
   // the strips of a head BH workgroups apart: on one chiplet, whose L2 then has the head's maps, where 8 divides BH
   const int nvs = (Dv + 15) >> 4, BH = gridDim.x / nvs, bh = blockIdx.x % BH, strip = blockIdx.x / BH, dv = 16 * strip + l16;
   f4 s, r[3], x[3][DKT];
