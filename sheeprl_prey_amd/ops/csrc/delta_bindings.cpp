@@ -2,7 +2,10 @@
 // operand's device, type, shape and strides are checked here against what the kernels index with; launches go to the current
 // stream of the operands' device.
 #include <torch/extension.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -49,6 +52,19 @@ void once(torch::autograd::variable_list& g, const char* name) {
   auto err = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " is differentiable once", (int64_t)in.size());
   auto out = (*err)(std::move(in));
   for (size_t j = 0; j < at.size(); ++j) g[at[j]] = out[j];
+}
+
+// A captured backward pass would have to wait for the default stream if an eager autograd graph that ran there still holds a
+// leaf of it; a capture does not allow that, and the error ends the process from the engine's thread.  It is refused here,
+// where the operands themselves are the leaves.
+void capturable(std::initializer_list<const Tensor*> operands, const char* name) {
+  for (const Tensor* t : operands) {
+    if (!wants(*t) || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    if (!node || !node->stream().has_value() || node->stream()->id() != 0) continue;
+    TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None, name,
+                ": a leaf of this captured pass belongs to an autograd graph of the default stream that is still alive: drop that graph first");
+  }
 }
 
 // ------------------------------------------------------------------ gated delta rule
@@ -320,6 +336,7 @@ std::pair<Tensor, Tensor> gated_delta(Tensor q, Tensor k, Tensor v, Tensor decay
   q = unit_last(q), k = unit_last(k), v = unit_last(v), decay = f32(decay), beta = f32(beta);
   if (state.defined()) state = state.contiguous();
   if (at::GradMode::is_enabled() && (wants(q) || wants(k) || wants(v) || wants(decay) || wants(beta) || wants(state))) {
+    capturable({&q, &k, &v, &decay, &beta, &state}, "gated_delta");
     auto r = GatedDeltaFn::apply(q, k, v, decay, beta, opt_of(state), opt_of(first), opt_of(lengths), opt.scale, normalize, eps, wants(state));
     return {r[0], r[1]};
   }
@@ -350,6 +367,10 @@ Tensor gated_delta_step(Tensor q, Tensor k, Tensor v, Tensor decay, Tensor beta,
     if (state.size(d) <= 1) continue;
     TORCH_CHECK_VALUE(state.stride(d) >= least, "the states must not overlap, got strides ", state.strides());
     least = state.stride(d) * state.size(d);
+  }
+  for (auto* t : {&q, &k, &v, &decay, &beta}) {
+    const auto o = at::get_overlap_status(state, *t);
+    TORCH_CHECK_VALUE(o != at::MemOverlapStatus::Full && o != at::MemOverlapStatus::Partial, "no operand may lie in the state that is updated");
   }
   const DeltaOpts opt{scale.has_value() ? *scale : 1.0 / std::sqrt((double)Dk), eps, normalize};
   if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
@@ -493,6 +514,7 @@ std::pair<Tensor, Tensor> gated_residual_norm(Tensor x, Tensor h, OptT gate_, Op
     want |= (int64_t)wants(w[i]) << (i + 1);
   }
   if (at::GradMode::is_enabled() && any) {
+    capturable({&x, &h, &gate, &w[0], &w[1], &w[2], &w[3], &w[4]}, "gated_residual_norm");
     auto r = ResidualNormFn::apply(x, h, opt_of(gate), opt_of(w[0]), opt_of(w[1]), opt_of(w[2]), opt_of(w[3]), opt_of(w[4]), layer, act, eps, s1, want);
     return {r[0], r[1]};
   }

@@ -96,7 +96,9 @@ def gated_delta(
     nothing else.
 
     Differentiable in ``q``, ``k``, ``v``, ``decay``, ``beta`` and ``state`` (once).  The sums, decays and states are fp32;
-    outputs and gradients are rounded once to the operand's type, those of shared key heads after their sum."""
+    outputs and gradients are rounded once to the operand's type, those of shared key heads after their sum.  A pass with its
+    backward can be captured into a graph as long as no eager autograd graph of the same leaves is alive on the default
+    stream (refused where ``q`` ... ``state`` are the leaves)."""
     if _fused(v) and v.numel() and q.numel():
         return ops._ext().gated_delta(q, k, v, decay, beta, state, is_first, lengths, scale, normalize, eps)
     _check(q, k, v, decay, beta, state, ("T", "B"))
@@ -115,7 +117,7 @@ def gated_delta_step(
 
     ``q``, ``k`` ``[B, Hk, Dk]``, ``v [B, Hv, Dv]``, ``decay``, ``beta`` ``[B, Hv]``, ``is_first [B(, 1)]`` as in
     :func:`gated_delta`; ``state`` fp32 ``[B, Hv, Dk, Dv]``, each ``[Dk, Dv]`` contiguous and none overlapping (a slice of a larger
-    store of states is fine).  No gradient; a captured graph replays it on the same state."""
+    store of states is fine) and without another operand in it.  No gradient; a captured graph replays it on the same state."""
     if _fused(v) and v.numel() and q.numel():
         return ops._ext().gated_delta_step(q, k, v, decay, beta, state, is_first, scale, normalize, eps)
     _check(q, k, v, decay, beta, state, ("B",))

@@ -90,6 +90,26 @@ def test_training_over_segments(T, B, Hk, Hv, Dk, Dv, dtype):
     check_train(delta_inputs(T, B, Hk, Hv, Dk, Dv, dtype, T, "cuda"))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("T,n,Hk,Hv,Dk,Dv", [(500, 32, 1, 2, 72, 20), (260, 26, 2, 6, 128, 16)])
+def test_training_with_many_chunks_of_shared_key_heads(T, n, Hk, Hv, Dk, Dv, dtype):
+    """A workgroup takes the value heads of a key head in turn: two sequences, n times over."""
+    x = delta_inputs(T, 2, Hk, Hv, Dk, Dv, dtype, T, "cuda")
+    g = torch.Generator().manual_seed(T)
+    d_out, d_last = torch.randn(T, 2, Hv, Dv, generator=g).to(dtype).cuda(), torch.randn(2, Hv, Dk, Dv, generator=g).cuda()
+    lengths = torch.tensor([T - 7, T // 3], dtype=torch.int32).cuda()
+    want, terms = oracle_train(x, d_out, d_last, lengths=lengths), projected(x, d_out, d_last, lengths=lengths)
+
+    def over(t, batch):
+        return torch.cat([t] * n, batch)
+
+    out, last, grads = run_train({k: over(t, int(k != "state")) for k, t in x.items()}, over(d_out, 1), over(d_last, 0), lengths=over(lengths, 0))
+    close(out, over(want[0], 1), tag("out", out))
+    close(last, over(want[1], 0), "last fp32")
+    for k in NAMES:
+        close(grads[k], over(want[2][k], int(k != "state")), tag("d_" + k, grads[k]), terms.get(k, 0.0))
+
+
 @pytest.mark.parametrize("T", [5, 70, 530])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
 def test_resets_and_lengths(T, dtype):
@@ -335,6 +355,60 @@ def test_captured_steps_carry_the_state():
         graph.replay()
         assert torch.equal(out, want[t])
     assert torch.equal(S, last)
+
+
+def test_a_capture_beside_a_living_graph_of_the_same_leaves_is_refused():
+    x = {n: t.requires_grad_() for n, t in delta_inputs(20, 2, 1, 1, 16, 16, torch.float32, 16, "cuda").items()}
+    out, _ = ops.gated_delta(**x)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        with pytest.raises(RuntimeError, match="still alive"):
+            ops.gated_delta(**x)
+        (torch.ones(1, device="cuda") + 1).detach()
+    torch.autograd.grad(out.sum(), list(x.values()), allow_unused=True)
+
+
+def test_offsets_past_32_bits():
+    """Operands of more than 2^31 elements: the last sequences come out as they do by themselves."""
+    B, T, Dk, Dv = 262200, 64, 16, 128
+    x = delta_inputs(T, 4, 1, 1, Dk, Dv, torch.bfloat16, 17, "cuda")
+    big = {n: t.new_zeros(*t.shape[:1 if n != "state" else 0], B, *t.shape[2 if n != "state" else 1:]) for n, t in x.items()}
+    for n, t in x.items():
+        (big[n] if n == "state" else big[n].transpose(0, 1))[-4:] = t if n == "state" else t.transpose(0, 1)
+    assert big["v"].numel() > 2**31
+    leaves = {n: t.clone().requires_grad_() for n, t in x.items()}
+    want = ops.gated_delta(**leaves)
+    d_out = torch.randn_like(want[0])
+    grads = torch.autograd.grad(want[0], list(leaves.values()), d_out)
+    big = {n: t.requires_grad_() for n, t in big.items()}
+    got = ops.gated_delta(**big)
+    assert torch.equal(got[0][:, -4:], want[0]) and torch.equal(got[1][-4:], want[1])
+    w = torch.zeros_like(got[0])
+    w[:, -4:] = d_out
+    for n, a, b in zip(x, torch.autograd.grad(got[0], list(big.values()), w), grads):
+        assert torch.equal(a[-4:] if n == "state" else a[:, -4:], b), n
+        assert not (a[:100] if n == "state" else a[:, :100]).any() or n in ("decay", "beta"), n
+
+
+def test_a_store_of_states_past_32_bits():
+    B, D = 140000, 128
+    x = delta_inputs(1, 3, 1, 1, D, D, torch.float32, 18, "cuda")
+    S = torch.zeros(B, 1, D, D, device="cuda")
+    assert S.numel() > 2**31
+    S[-3:] = x["state"]
+    a = [torch.zeros(B, *x[n].shape[2:], device="cuda") for n in NAMES[:5]]
+    for t, n in zip(a, NAMES):
+        t[-3:] = x[n][0]
+    out = ops.gated_delta_step(*a, S)
+    want = ops.gated_delta_step(*(x[n][0] for n in NAMES[:5]), x["state"])
+    assert torch.equal(out[-3:], want) and torch.equal(S[-3:], x["state"]) and not S[:-3].any()
+
+
+def test_an_operand_in_the_state_is_refused():
+    S = torch.zeros(2, 1, 8, 8, device="cuda")
+    q = torch.zeros(2, 1, 8, device="cuda")
+    with pytest.raises(ValueError, match="in the state"):
+        ops.gated_delta_step(q, q, S.view(-1)[:16].view(2, 1, 8), torch.zeros(2, 1, device="cuda"), torch.zeros(2, 1, device="cuda"), S)
 
 
 def test_eager_form_on_the_gpu_when_fusion_is_off():

@@ -104,6 +104,28 @@ def test_repeats_bit_by_bit_and_rows_are_apart():
     assert torch.equal(y[keep], y2[keep]) and torch.equal(u[keep], u2[keep]) and y2[7].isnan().all()
 
 
+def test_offsets_past_32_bits():
+    """Operands of more than 2^31 elements: the last rows come out as they do by themselves."""
+    rows, D = 2**20 + 8, 2048
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, h, gate, dy, du = ((torch.randn(8, D, generator=g, device="cuda")).bfloat16() for _ in range(5))
+    big = []
+    for t in (x, h, gate, dy, du):
+        b = torch.zeros(rows, D, device="cuda", dtype=torch.bfloat16)
+        b[-8:] = t
+        big.append(b)
+    assert big[0].numel() > 2**31
+
+    def run(x, h, gate, dy, du):
+        leaves = [t.requires_grad_() for t in (x, h, gate)]
+        y, u = ops.gated_residual_norm(*leaves, 0.5, norm="rms")
+        return [y.detach(), u.detach(), *torch.autograd.grad((y, u), leaves, (dy, du))]
+
+    for a, b in zip(run(*big), run(x, h, gate, dy, du)):
+        assert torch.equal(a[-8:], b)
+        assert not a[:100].any()
+
+
 def test_no_rows():
     y, u = ops.gated_residual_norm(torch.zeros(0, 16, device="cuda"), torch.zeros(0, 16, device="cuda"))
     assert y.shape == u.shape == (0, 16)
