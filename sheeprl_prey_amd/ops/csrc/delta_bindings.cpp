@@ -510,6 +510,7 @@ std::pair<Tensor, Tensor> gated_residual_norm(Tensor x, Tensor h, OptT gate_, Op
     shape(w[i], {D}, names[i]);
     operand(w[i]);
     w[i] = f32(w[i]).contiguous();
+    if (reinterpret_cast<uintptr_t>(w[i].data_ptr()) % 16) w[i] = w[i].clone();  // the kernels read four at a time
     any = any || wants(w[i]);
     want |= (int64_t)wants(w[i]) << (i + 1);
   }

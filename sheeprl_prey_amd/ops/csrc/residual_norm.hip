@@ -93,12 +93,23 @@ __device__ __forceinline__ void store_row(T* p, int i, int D, const float* v) {
     }
   }
 }
+// Weights of a lane's columns; those past D read the last one's, and no result takes them.  VEC: 16 bytes at a time, for each
+// element by itself reads every cache line eight times.
 template <typename T, int L, int V, bool VEC>
 __device__ __forceinline__ void load_par(const float* p, int i, int D, float other, float* o) {
+  if (!p) {
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    const int c = column<T, L, V, VEC>(e, i);
-    o[e] = p && c < D ? p[c] : other;
+    for (int e = 0; e < V; ++e) o[e] = other;
+  } else if constexpr (VEC) {
+#pragma unroll
+    for (int e = 0; e < V; e += 4) {
+      const delta::f4 x = *reinterpret_cast<const delta::f4*>(p + min(column<T, L, V, VEC>(e, i), D - 4));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[e + j] = x[j];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) o[e] = p[min(column<T, L, V, VEC>(e, i), D - 1)];
   }
 }
 

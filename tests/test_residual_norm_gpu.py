@@ -104,6 +104,26 @@ def test_repeats_bit_by_bit_and_rows_are_apart():
     assert torch.equal(y[keep], y2[keep]) and torch.equal(u[keep], u2[keep]) and y2[7].isnan().all()
 
 
+def test_weights_that_begin_anywhere():
+    rows, D = 5, 96
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x, h, gate = (torch.randn(rows, D, generator=g, device="cuda") for _ in range(3))
+    w = [torch.randn(D, generator=g, device="cuda") for _ in range(5)]
+    flat = torch.zeros(5, D + 1, device="cuda")
+    for a, b in zip(flat, w):
+        a[1:] = b
+
+    def run(ws):
+        leaves = [t.clone().requires_grad_() for t in (x, h, gate)]
+        y, u = ops.gated_residual_norm(*leaves, *ws)
+        return [y.detach(), u.detach(), *torch.autograd.grad(y.sum() + (u * x).sum(), leaves + ws)]
+
+    odd = [t[1:].requires_grad_() for t in flat]
+    assert any(t.data_ptr() % 16 for t in odd)
+    for a, b in zip(run(odd), run([t.requires_grad_() for t in w])):
+        assert torch.equal(a, b)
+
+
 def test_offsets_past_32_bits():
     """Operands of more than 2^31 elements: the last rows come out as they do by themselves."""
     rows, D = 2**20 + 8, 2048
