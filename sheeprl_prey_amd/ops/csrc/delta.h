@@ -129,6 +129,11 @@ __device__ __forceinline__ void chunk_gates(const Args& a, Gates<C>& s, int b, i
   }
 }
 
+// The state before the first step, which a reset there leaves unread, whatever it holds (gates of zero would not stop a NaN).
+__device__ __forceinline__ const float* state_before(const Args& a, int b, int len) {
+  return len > 0 && a.first && a.first[(long)b * a.fb] ? nullptr : a.state;
+}
+
 // A uniform value that the compiler does not carry over from one turn of a loop to the next: addresses that it would work out
 // once and hold in registers through the whole walk (32 of 64 bits each, to no end but spills) are worked out again instead.
 __device__ __forceinline__ long afresh(long x) {

@@ -58,8 +58,8 @@ struct BwdArgs {
 
 void launch_delta_fwd(const Args& a, const FwdOut& o, int C, bool is_bf16, hipStream_t st);
 void launch_delta_bwd(const Args& a, const BwdArgs& o, int C, bool is_bf16, bool per_value_head, hipStream_t st);
-void launch_delta_scan(const float* first, const float* P, const float* X, float* S, int BH, int nseg, int Dk, int Dv, bool rev,
-                       hipStream_t st);
+// S (or, rev, dS) at the segments' ends from that before the first step (or dlast), the maps P and X
+void launch_delta_scan(const Args& a, const float* dlast, const float* P, const float* X, float* S, bool rev, hipStream_t st);
 void launch_delta_head_sum(const float* xq, const float* xk, void* yq, void* yk, long rows, int rep, int Dk, bool is_bf16, hipStream_t st);
 // delta_step.hip: the recurrent form; S2 (the state after it) may be a.state itself
 void launch_delta_steps(const Args& a, void* out, float* S2, long sb, long sh, bool is_bf16, hipStream_t st);

@@ -151,15 +151,19 @@ srl::delta::Args delta_args(const Tensor& q, const Tensor& k, const Tensor& v, c
 
 int dkp(int Dk) { return Dk <= 32 ? 32 : Dk <= 64 ? 64 : 128; }
 
-// Chunks of 64 steps (16 where the whole sequence fits); a long axis is split into segments while the heads alone leave
-// the 256 CUs idle.  Returns C.
+// Chunks of 64 steps, or one of 16 where the whole sequence fits (16 steps x 128 x 2 heads of 32, forward and backward: 31 us
+// and 58 us as a chunk of 64; x 16 x 16 of 128: 73 and 89).  An axis of 8 chunks or more is split into segments while the
+// heads alone leave two thirds of the 256 CUs idle; the segments' maps cost as much as the walk itself.  Forward over 1024
+// steps with and without segments: 48 heads of 128 133 and 177 us, 64 heads 157 and 181, 80 heads 189 and 190, 96 heads (two
+// segments) 216 and 191; 64 heads of 64 105 and 158.  512 steps of 8 heads: 70 and 93; 256 steps of 16 heads of 64: 50 and 48.
+// Returns C.
 int delta_plan(srl::delta::Args& a) {
   const int C = a.T <= 16 ? 16 : 64, BH = a.B * a.Hv;
   a.N = (a.T + C - 1) / C;
   a.nseg = 1;
   a.cps = a.N;
-  if (a.N >= 8 && BH <= 128) {
-    const int want = std::min(a.N / 2, std::max(2, 256 / BH));
+  if (a.N >= 8 && 256 / BH >= 3) {
+    const int want = std::min(a.N / 2, 256 / BH);
     a.cps = (a.N + want - 1) / want;
     a.nseg = (a.N + a.cps - 1) / a.cps;
   }
@@ -323,8 +327,10 @@ Tensor delta_steps(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   return out;
 }
 
-// Up to this many steps without a gradient the recurrent kernel is taken.
-constexpr int RECURRENT_MAX_STEPS = 16;
+// Up to this many steps without a gradient the recurrent kernel is taken, whose time goes with the steps.  Against a chunk of
+// 16, in a graph: 4 steps x 64 x 16 heads of 128 57 and 58 us, 8 steps 86 and 58; x 16 x 16 heads 25 and 27, 6 steps 32
+// and 27; 4 steps x 64 x 8 heads of 64 17 and 18, 8 steps 24 and 18.
+constexpr int RECURRENT_MAX_STEPS = 4;
 
 std::pair<Tensor, Tensor> gated_delta(Tensor q, Tensor k, Tensor v, Tensor decay, Tensor beta, OptT state_, OptT first_, OptT lengths_,
                                       c10::optional<double> scale, bool normalize, double eps) {

@@ -1076,7 +1076,7 @@ static void launch_c(const Args& a, const BwdArgs& o, bool per_value_head, hipSt
     if (a.nseg > 1) {
       if (nvs <= 4) launch_walk<T, DKT, 4, true>(a, o, st);
       else launch_walk<T, DKT, 8, true>(a, o, st);
-      launch_delta_scan(o.dlast, o.Ptr, o.Xseg, o.dSseg, BH, a.nseg, a.Dk, a.Dv, true, st);
+      launch_delta_scan(a, o.dlast, o.Ptr, o.Xseg, o.dSseg, true, st);
     }
     if (nvs <= 4) launch_walk<T, DKT, 4, false>(a, o, st);
     else launch_walk<T, DKT, 8, false>(a, o, st);

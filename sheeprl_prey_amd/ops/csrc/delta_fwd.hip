@@ -39,13 +39,14 @@ __global__ void __launch_bounds__(512) delta_short_kernel(Args a, FwdOut o) {
   load_rows<T, DKT, C, 4>(K, s.rk, kp, a.kt, a.Dk, 0, len, a.veck, a.normalize, a.eps);
   load_rows<T, DKT, C, 4>(Q, s.rq, qp, a.qt, a.Dk, 0, len, a.vecq, a.normalize, a.eps);
   if (wave == 0) chunk_gates<C>(a, s, b, h, 0, len, lane);
+  const float* s0 = state_before(a, b, len);
   f4 S[DKT];
 #pragma unroll
   for (int m = 0; m < DKT; ++m)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int d = 16 * m + 4 * kq + r;
-      S[m][r] = (a.state && d < a.Dk && dv < a.Dv) ? a.state[((long)bh * a.Dk + d) * a.Dv + dv] : 0.f;
+      S[m][r] = (s0 && d < a.Dk && dv < a.Dv) ? s0[((long)bh * a.Dk + d) * a.Dv + dv] : 0.f;
       if (o.Sc) o.Sc[((long)bh * DKp + d) * Dvp + dv] = S[m][r];
     }
   lds_barrier();
@@ -276,13 +277,13 @@ __global__ void __launch_bounds__(64 * NWT) delta_walk_kernel(Args a, FwdOut o) 
     const float* p = o.Sseg + ((((long)bh * a.nseg + seg) * nvs + wave) * DKT * 64 + lane) * 4;
 #pragma unroll
     for (int m = 0; m < DKT; ++m) S[m] = row4(p + m * 256);
-  } else if (works && a.state) {
+  } else if (const float* s0 = state_before(a, b, len); works && s0) {
 #pragma unroll
     for (int m = 0; m < DKT; ++m)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int d = 16 * m + 4 * kq + r;
-        if (d < a.Dk && dv < a.Dv) S[m][r] = a.state[((long)bh * a.Dk + d) * a.Dv + dv];
+        if (d < a.Dk && dv < a.Dv) S[m][r] = s0[((long)bh * a.Dk + d) * a.Dv + dv];
       }
   }
   Column<T, NT> v;
@@ -418,13 +419,14 @@ __global__ void __launch_bounds__(64 * NWT) delta_walk_kernel(Args a, FwdOut o) 
 // transposed.  One workgroup per 16 columns, one wave per 16 rows; the state goes through LDS in three bf16 parts, and the
 // next two maps are on their way meanwhile.
 template <int DKT, bool REV>
-__global__ void __launch_bounds__(64 * DKT) delta_scan_kernel(const float* first, const float* P, const float* R, float* out, int nseg,
-                                                              int Dk, int Dv) {
+__global__ void __launch_bounds__(64 * DKT) delta_scan_kernel(Args a, const float* dlast, const float* P, const float* R, float* out) {
   constexpr int DKp = 16 * DKT, LD = DKp + 8;
   __shared__ __align__(16) uint16_t S[2][3][16 * LD];
   const int lane = threadIdx.x & 63, m = wave_id(), l16 = lane & 15, kq = lane >> 4;
   // the strips of a head BH workgroups apart: on one chiplet, whose L2 then has the head's maps, where 8 divides BH
-  const int nvs = (Dv + 15) >> 4, BH = gridDim.x / nvs, bh = blockIdx.x % BH, strip = blockIdx.x / BH, dv = 16 * strip + l16;
+  const int Dk = a.Dk, Dv = a.Dv, nseg = a.nseg, nvs = (Dv + 15) >> 4, BH = gridDim.x / nvs, bh = blockIdx.x % BH, strip = blockIdx.x / BH, dv = 16 * strip + l16;
+  const int len = a.lengths ? max(0, min(a.T, a.lengths[bh / a.Hv])) : a.T;
+  const float* first = REV ? dlast : state_before(a, bh / a.Hv, len);
   f4 s, r[3], x[3][DKT];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -495,7 +497,7 @@ static void launch_dk(const Args& a, const FwdOut& o, int C, hipStream_t st) {
   if (a.nseg > 1) {
     if (nvs + DKT <= 8) launch_walk<T, DKT, 8, true>(a, o, st);
     else launch_walk<T, DKT, 16, true>(a, o, st);
-    launch_delta_scan(a.state, o.Pseg, o.Rseg, o.Sseg, BH, a.nseg, a.Dk, a.Dv, false, st);
+    launch_delta_scan(a, nullptr, o.Pseg, o.Rseg, o.Sseg, false, st);
   }
   if (nvs <= 4) launch_walk<T, DKT, 4, false>(a, o, st);
   else launch_walk<T, DKT, 8, false>(a, o, st);
@@ -514,18 +516,16 @@ void launch_delta_fwd(const Args& a, const FwdOut& o, int C, bool is_bf16, hipSt
 }
 
 template <int DKT>
-static void launch_scan(const float* first, const float* P, const float* X, float* S, int BH, int nseg, int Dk, int Dv, bool rev,
-                        hipStream_t st) {
-  const int g = BH * ((Dv + 15) / 16);
-  if (rev) delta_scan_kernel<DKT, true><<<g, 64 * DKT, 0, st>>>(first, P, X, S, nseg, Dk, Dv);
-  else delta_scan_kernel<DKT, false><<<g, 64 * DKT, 0, st>>>(first, P, X, S, nseg, Dk, Dv);
+static void launch_scan(const Args& a, const float* dlast, const float* P, const float* X, float* S, bool rev, hipStream_t st) {
+  const int g = a.B * a.Hv * ((a.Dv + 15) / 16);
+  if (rev) delta_scan_kernel<DKT, true><<<g, 64 * DKT, 0, st>>>(a, dlast, P, X, S);
+  else delta_scan_kernel<DKT, false><<<g, 64 * DKT, 0, st>>>(a, dlast, P, X, S);
 }
 
-void launch_delta_scan(const float* first, const float* P, const float* X, float* S, int BH, int nseg, int Dk, int Dv, bool rev,
-                       hipStream_t st) {
-  if (Dk <= 32) launch_scan<2>(first, P, X, S, BH, nseg, Dk, Dv, rev, st);
-  else if (Dk <= 64) launch_scan<4>(first, P, X, S, BH, nseg, Dk, Dv, rev, st);
-  else launch_scan<8>(first, P, X, S, BH, nseg, Dk, Dv, rev, st);
+void launch_delta_scan(const Args& a, const float* dlast, const float* P, const float* X, float* S, bool rev, hipStream_t st) {
+  if (a.Dk <= 32) launch_scan<2>(a, dlast, P, X, S, rev, st);
+  else if (a.Dk <= 64) launch_scan<4>(a, dlast, P, X, S, rev, st);
+  else launch_scan<8>(a, dlast, P, X, S, rev, st);
 }
 
 }  // namespace delta

@@ -93,7 +93,7 @@ def gated_delta(
     zero state; there ``decay`` has no effect.  ``lengths [B]`` (clamped to 0..T): steps at or after a sequence's length change nothing,
     give zero outputs and get zero gradients, and are not read.  ``scale`` defaults to ``Dk ** -0.5``.  A value that is
     not finite in a step that counts spoils the results of its own sequence and key head, before it and after it, and
-    nothing else.
+    nothing else; one in ``state`` those of its sequence and head, unless ``is_first`` marks the first step.
 
     Differentiable in ``q``, ``k``, ``v``, ``decay``, ``beta`` and ``state`` (once).  The sums, decays and states are fp32;
     outputs and gradients are rounded once to the operand's type, those of shared key heads after their sum.  A pass with its

@@ -183,10 +183,11 @@ def test_extreme_decays_and_rates(T):
     close(last, want[1], "last fp32")
 
 
-def test_a_reset_forgets_a_state_that_is_not_finite():
-    x = delta_inputs(4, 1, 1, 1, 16, 16, torch.float32, 4, "cuda")
+@pytest.mark.parametrize("T", [4, 16, 70, 530])
+def test_a_reset_forgets_a_state_that_is_not_finite(T):
+    x = delta_inputs(T, 1, 1, 1, 16, 16, torch.float32, 4, "cuda")
     bad = {**x, "state": torch.full_like(x["state"], float("nan"))}
-    first = torch.zeros(4, 1, dtype=torch.bool, device="cuda")
+    first = torch.zeros(T, 1, dtype=torch.bool, device="cuda")
     first[0] = True
     with torch.no_grad():
         a, b = ops.gated_delta(**x, is_first=first), ops.gated_delta(**bad, is_first=first)
@@ -195,6 +196,10 @@ def test_a_reset_forgets_a_state_that_is_not_finite():
         out = ops.gated_delta_step(*(x[n][0] for n in NAMES[:5]), S, is_first=first[0])
     close(out, a[0][0], "out fp32")
     assert torch.isfinite(S).all()
+    w, z = torch.randn_like(x["v"]), torch.randn_like(x["state"])
+    c, d = run_train(x, w, z, is_first=first), run_train(bad, w, z, is_first=first)
+    assert torch.equal(c[0], d[0]) and torch.equal(c[1], d[1]) and all(torch.equal(c[2][n], d[2][n]) for n in NAMES)
+    assert not d[2]["state"].any()
 
 
 @pytest.mark.parametrize("T", [9, 70])
@@ -280,7 +285,10 @@ def test_steps_follow_the_rule(B, Hk, Hv, Dk, Dv, dtype):
     assert (store[:, 0] == 7.0).all()
     with torch.no_grad():
         out, l2 = ops.gated_delta(**x, is_first=first)
-    assert torch.equal(out, torch.stack(outs)) and torch.equal(l2, S)
+        few, _ = ops.gated_delta(**{n: t if n == "state" else t[:4] for n, t in x.items()}, is_first=first[:4])
+    close(out, want, tag("out", out))
+    close(l2, last, "last fp32")
+    assert torch.equal(few, torch.stack(outs[:4]))  # the same kernel
 
 
 def test_results_repeat_bit_by_bit():
@@ -338,7 +346,7 @@ def test_captured_training_replays_beside_eager_work():
 
 
 def test_captured_steps_carry_the_state():
-    x = delta_inputs(5, 4, 1, 2, 32, 32, torch.float32, 14, "cuda")
+    x = delta_inputs(4, 4, 1, 2, 32, 32, torch.float32, 14, "cuda")
     S = x["state"].clone()
     cur = {n: x[n][0].clone() for n in NAMES[:5]}
     graph = torch.cuda.CUDAGraph()
@@ -349,7 +357,7 @@ def test_captured_steps_carry_the_state():
     S.copy_(x["state"])
     with torch.no_grad():
         want, last = ops.gated_delta(**x)
-    for t in range(5):
+    for t in range(4):
         for n in NAMES[:5]:
             cur[n].copy_(x[n][t])
         graph.replay()
