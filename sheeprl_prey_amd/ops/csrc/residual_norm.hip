@@ -15,6 +15,11 @@
 // is on its way while this one is worked on.  The parameter sums stay in registers over the rows that a group of lanes
 // walks; each workgroup leaves one partial sum of every column and residual_norm_sum_kernel adds them in a fixed order,
 // so results repeat bit by bit.
+//
+// Measured: forward, bf16, 8191 x 2048 29 us (5.8 TB/s), 8192 x 4096 61 us (5.5 TB/s; a copy of that size 5.2); backward
+// 8192 x 4096 129 us (4.2 TB/s: two workgroups of 512 a CU, for the partial sums' sake) and 13 us for the sums; fp32, 16384
+// x 256 16 and 26 us and 6 us.  bf16 rows of 1001 go by elements: 5003 of them 19 and 39 us.  Outputs are stored through the
+// caches: past them the kernel is up to 12 % faster by itself, but what reads y and u next loses more (98 -> 109 us together).
 #include "delta.h"
 #include "residual_norm.h"
 
@@ -391,6 +396,8 @@ static void run(const Args& a, const BwdArgs* o, int W, hipStream_t st) {
 
 template <typename T, bool VEC>
 static void pick(const Args& a, const BwdArgs* o, int W, hipStream_t st) {
+  // as few lanes a row as leave a lane at most 8 elements of each operand: with more of them the weights and the parameter
+  // sums of the backward pass do not fit the registers
   if (a.D <= 64) run<T, 16, 4, VEC>(a, o, W, st);
   else if (a.D <= 256) run<T, 64, 4, VEC>(a, o, W, st);
   else if (a.D <= 512) run<T, 64, 8, VEC>(a, o, W, st);
