@@ -54,7 +54,7 @@ class RecurrentModel(nn.Module):
         return (z, z.clone())
 
     def step(self, input: Tensor, states: Tuple[Tensor, ...]):
-        """One step without a gradient; the states given may be updated in place."""
+        """One step without a gradient."""
         return self(input, states)
 
     def forward(self, input: Tensor, states: Tuple[Tensor, Tensor], mask: Optional[Tensor] = None):
@@ -89,8 +89,9 @@ class GatedDeltaModel(nn.Module):
         return self._post_mlp(out.reshape(-1, out.shape[-1])).view(*out.shape[:-1], -1)
 
     def step(self, input: Tensor, states: Tuple[Tensor, ...]):
-        """One step without a gradient, the state updated in place."""
-        return self._end(self._blocks.step(self._pre_mlp(input), states[0])), states
+        """One step without a gradient; the states given stay as they are."""
+        state = states[0].clone()
+        return self._end(self._blocks.step(self._pre_mlp(input), state)), (state,)
 
     def forward(self, input: Tensor, states: Tuple[Tensor, ...], mask: Optional[Tensor] = None):
         lengths = None if mask is None else mask.reshape(mask.shape[0], -1).sum(0, dtype=torch.int32)
@@ -195,7 +196,6 @@ class RecurrentPPOAgent(nn.Module):
     def get_greedy_actions(self, obs: Dict[str, Tensor], prev_states, prev_actions: Tensor, mask=None):
         emb = self.feature_extractor(obs)
         x = torch.cat((emb, prev_actions), -1)
-        # single steps without a gradient may update the states they are given in place
         single = mask is None and x.shape[0] == 1 and not torch.is_grad_enabled()
         out, states = self.rnn.step(x, prev_states) if single else self.rnn(x, prev_states, mask)
         pre = self.get_pre_dist(out)

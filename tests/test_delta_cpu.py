@@ -187,6 +187,22 @@ def _blocks(num_blocks=2, **kw):
     return m
 
 
+def test_the_policys_step_leaves_the_callers_states():
+    from sheeprl_prey_amd.algos.ppo_recurrent.agent import build_recurrent_model
+    from sheeprl_prey_amd.utils.utils import dotdict
+
+    mlp = dotdict({"apply": False})
+    m, _ = build_recurrent_model(7, dotdict(cell="gated_delta", pre_rnn_mlp=mlp, post_rnn_mlp=mlp, gated_delta=dict(
+        hidden_size=12, num_blocks=2, key_heads=1, value_heads=2, key_dim=5, value_dim=6)))
+    x, states = torch.randn(1, 3, 7), m.initial_states(3)
+    with torch.no_grad():
+        out, after = m.step(x, states)
+        assert not states[0].any()
+        want, last = m(x, states)
+    torch.testing.assert_close(out, want)
+    torch.testing.assert_close(after[0], last[0])
+
+
 def test_blocks_step_by_step_are_the_sequence():
     m = _blocks()
     x, state = torch.randn(5, 3, 7), m.initial_state(3)
