@@ -145,6 +145,12 @@ __device__ __forceinline__ long afresh(long x) {
 // itself): rows behind the end and columns past the width are read from the nearest that is there, and zeroed afterwards.
 // There is a first step in any case.
 
+// What scales a row of sum of squares ss to unit length.  Zero for rows behind the end, which are read as zeros: with eps = 0 their
+// factor would be infinite, and a NaN in a row that does not count spoils the sums over the chunk.
+__device__ __forceinline__ float unit_factor(float ss, bool live, bool normalize, float eps) {
+  return !live ? 0.f : normalize ? 1.f / sqrtf(ss + eps) : 1.f;
+}
+
 // Rows t0.. of one head into LDS as fp32 [C][16 DKT + 4], scaled to unit length; 16 lanes a row, R rows a thread.
 template <typename T, int DKT, int C, int R>
 __device__ __forceinline__ void load_rows(float* dst, float* rn, const T* src, long st, int D, int t0, int len, bool vec,
@@ -176,7 +182,7 @@ __device__ __forceinline__ void load_rows(float* dst, float* rn, const T* src, l
       x[r][j] = (t0 + i < len && c0 + j < D) ? x[r][j] : 0.f;
       ss = fmaf(x[r][j], x[r][j], ss);
     }
-    const float n = normalize ? 1.f / sqrtf(row16_sum(ss) + eps) : 1.f;
+    const float n = unit_factor(row16_sum(ss), t0 + i < len, normalize, eps);
     if (i < C) {
       float* d = dst + i * LD + c0;
 #pragma unroll

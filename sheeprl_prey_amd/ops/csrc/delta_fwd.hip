@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(256) delta_pairs_kernel(Args a, float* pairs, 
           ss = fmaf(f, f, ss);
           M[i * LD + place(c0 + j)] = x[r][j].x;
         }
-        const float nn = a.normalize ? 1.f / sqrtf(row16_sum(ss) + a.eps) : 1.f;
+        const float nn = unit_factor(row16_sum(ss), t0 + i < len, a.normalize, a.eps);
         if (sub == 0) rn[i] = nn;
       }
     };

@@ -223,11 +223,14 @@ def gated_delta(q: Tensor, k: Tensor, v: Tensor, decay: Tensor, beta: Tensor, st
     if lengths is not None:  # what lies behind a sequence's end is not read
         live = torch.arange(T, device=v.device)[:, None] < lengths[None]
         wide, narrow = live[..., None, None], live[..., None]
-        qf, kf, vf = (torch.where(wide, t, 0.0) for t in (qf, kf, vf))
+        qf, kf = (torch.where(wide, t, 1.0) for t in (qf, kf))  # a length above zero, whatever eps is
+        vf = torch.where(wide, vf, 0.0)
         gf, bf = (torch.where(narrow, t, 0.0) for t in (gf, bf))
         is_first = None if is_first is None else is_first.bool() & live
     if normalize:
         qf, kf = (t * torch.rsqrt((t * t).sum(-1, keepdim=True) + eps) for t in (qf, kf))
+    if lengths is not None:
+        qf, kf = (torch.where(wide, t, 0.0) for t in (qf, kf))
     qf, kf = (t.repeat_interleave(Hv // Hk, 2) for t in (qf, kf))
     S = torch.zeros(B, Hv, Dk, Dv, device=v.device, dtype=ct) if state is None else state
     keep = gf.exp()[..., None, None]

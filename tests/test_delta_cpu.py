@@ -274,3 +274,16 @@ def test_recurrent_ppo_refuses_another_cell():
 
     with pytest.raises(ValueError, match="algo.rnn.cell"):
         build_recurrent_model(4, dotdict({"cell": "gru"}))
+
+
+@pytest.mark.parametrize("T", [5, 70])
+def test_rows_behind_a_length_need_no_eps(T):
+    x = {n: t.requires_grad_() for n, t in delta_inputs(T, 2, 1, 2, 8, 6).items()}
+    lengths = torch.tensor([T, T // 2])
+    out, last = ops.gated_delta(**x, lengths=lengths, eps=0.0)
+    eo, el = delta_oracle(**x, lengths=lengths, eps=0.0)
+    tol = (T + 8) * 8 * 2.0**-24  # as above
+    torch.testing.assert_close(out.double(), eo, rtol=tol, atol=tol)
+    torch.testing.assert_close(last.double(), el, rtol=tol, atol=tol * 8)
+    for g in torch.autograd.grad(out.sum() + last.sum(), list(x.values())):
+        assert torch.isfinite(g).all()

@@ -1,0 +1,52 @@
+"""The options of the gated delta rule through the kernels, against the rule in 64 bits: ``eps``, ``scale``, ``normalize``, gradients
+of one output alone, strides in bf16."""
+import pytest
+import torch
+
+from sheeprl_prey_amd import ops
+from tests.test_delta_cpu import delta_inputs, delta_oracle
+from tests.test_delta_gpu import NAMES, close, oracle_train, run_train, tag
+
+pytestmark = pytest.mark.gpu
+TYPES = pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+
+
+def projected(x, d_out, d_last, eps, **kw):
+    """Root mean square of r d, with d the gradient of the unit vectors and r their factor: d_q and d_k are differences of vectors of
+    that length, whose roundings they carry, where q and k are scaled to unit length."""
+    y = {n: t.detach().double().cpu() for n, t in x.items()}
+    r = {n: (y[n].square().sum(-1, keepdim=True) + eps).rsqrt() for n in "qk"}
+    for n in "qk":
+        y[n] = (y[n] * r[n]).requires_grad_()
+    kw = {n: t.cpu() if isinstance(t, torch.Tensor) else t for n, t in kw.items()}
+    d = torch.autograd.grad(delta_oracle(**y, **kw, normalize=False), [y["q"], y["k"]], (d_out.double().cpu(), d_last.double().cpu()))
+    return {n: (r[n] * g).square().mean().sqrt() for n, g in zip("qk", d)}
+
+
+def gradients_of(x, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(x["v"].shape, generator=g).to(x["v"].dtype).cuda(), torch.randn(x["state"].shape, generator=g).cuda())
+
+
+def check_train(x, **kw):
+    d_out, d_last = gradients_of(x)
+    got, want = run_train(x, d_out, d_last, **kw), oracle_train(x, d_out, d_last, **kw)
+    terms = {} if not kw.get("normalize", True) else projected(x, d_out, d_last, **{"eps": 1e-6, **kw})
+    close(got[0], want[0], tag("out", got[0]))
+    close(got[1], want[1], "last fp32")
+    for n in NAMES:
+        close(got[2][n], want[2][n], tag("d_" + n, got[2][n]), terms.get(n, 0.0))
+
+
+@TYPES
+@pytest.mark.parametrize("T", [3, 5, 16, 70, 530])
+def test_no_eps_with_chunks_that_are_not_full(T, dtype):
+    x = delta_inputs(T, 3, 1, 2, 24, 40, dtype, T, "cuda")
+    check_train(x, eps=0.0)
+    lengths = torch.tensor([T, T // 2 + 1, 0], dtype=torch.int32).cuda()
+    check_train(x, eps=0.0, lengths=lengths)
+    with torch.no_grad():
+        out, last = ops.gated_delta(**x, eps=0.0, lengths=lengths)
+    want, el = delta_oracle(**{n: t.cpu() for n, t in x.items()}, eps=0.0, lengths=lengths.cpu())
+    close(out, want, tag("out", out))
+    close(last, el, "last fp32")
