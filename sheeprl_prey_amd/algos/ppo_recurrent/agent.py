@@ -40,7 +40,7 @@ class RecurrentModel(nn.Module):
 
     def __init__(self, input_size: int, lstm_hidden_size: int, pre_rnn_mlp_cfg, post_rnn_mlp_cfg) -> None:
         super().__init__()
-        self._hidden_size = lstm_hidden_size
+        self.hidden_size = lstm_hidden_size
         self._pre_mlp, d = _opt_mlp(input_size, pre_rnn_mlp_cfg)
         self._lstm = nn.LSTM(input_size=d, hidden_size=lstm_hidden_size, batch_first=False)
         self._post_mlp, self._output_dim = _opt_mlp(lstm_hidden_size, post_rnn_mlp_cfg)
@@ -50,7 +50,7 @@ class RecurrentModel(nn.Module):
         return self._output_dim
 
     def initial_states(self, n: int, device=None) -> Tuple[Tensor, ...]:
-        z = torch.zeros(1, n, self._hidden_size, device=device)
+        z = torch.zeros(1, n, self.hidden_size, device=device)
         return (z, z.clone())
 
     def step(self, input: Tensor, states: Tuple[Tensor, ...]):
@@ -75,6 +75,7 @@ class GatedDeltaModel(nn.Module):
     def __init__(self, input_size: int, cfg, pre_rnn_mlp_cfg, post_rnn_mlp_cfg) -> None:
         super().__init__()
         self._pre_mlp, d = _opt_mlp(input_size, pre_rnn_mlp_cfg)
+        self.hidden_size = cfg.hidden_size
         self._blocks = GatedDeltaBlocks(d, cfg.hidden_size, cfg.num_blocks, cfg.key_heads, cfg.value_heads, cfg.key_dim, cfg.value_dim)
         self._post_mlp, self._output_dim = _opt_mlp(cfg.hidden_size, post_rnn_mlp_cfg)
 
@@ -103,10 +104,12 @@ def build_recurrent_model(input_size: int, rnn_cfg) -> Tuple[nn.Module, int]:
     """The cell that ``algo.rnn.cell`` names, and the width of its output."""
     cell = str(rnn_cfg.get("cell", "lstm")).lower()
     if cell == "lstm":
-        return RecurrentModel(input_size, rnn_cfg.lstm.hidden_size, rnn_cfg.pre_rnn_mlp, rnn_cfg.post_rnn_mlp), rnn_cfg.lstm.hidden_size
-    if cell == "gated_delta":
-        return GatedDeltaModel(input_size, rnn_cfg.gated_delta, rnn_cfg.pre_rnn_mlp, rnn_cfg.post_rnn_mlp), rnn_cfg.gated_delta.hidden_size
-    raise ValueError(f"algo.rnn.cell must be 'lstm' or 'gated_delta', got {rnn_cfg.cell!r}")
+        model = RecurrentModel(input_size, rnn_cfg.lstm.hidden_size, rnn_cfg.pre_rnn_mlp, rnn_cfg.post_rnn_mlp)
+    elif cell == "gated_delta":
+        model = GatedDeltaModel(input_size, rnn_cfg.gated_delta, rnn_cfg.pre_rnn_mlp, rnn_cfg.post_rnn_mlp)
+    else:
+        raise ValueError(f"algo.rnn.cell must be 'lstm' or 'gated_delta', got {rnn_cfg.cell!r}")
+    return model, model.output_dim
 
 
 class _SeqCNNEncoder(CNNEncoder):
@@ -136,11 +139,12 @@ class RecurrentPPOAgent(nn.Module):
         self.feature_extractor = MultiEncoder(cnn_encoder, mlp_encoder)
         self.is_continuous = is_continuous
         features_dim = self.feature_extractor.output_dim
-        self.rnn, self.rnn_hidden_size = build_recurrent_model(int(features_dim + sum(actions_dim)), rnn_cfg)
+        self.rnn, rnn_output_dim = build_recurrent_model(int(features_dim + sum(actions_dim)), rnn_cfg)
+        self.rnn_hidden_size = self.rnn.hidden_size
 
         def mlp(out, cfg):
             n = cfg.mlp_layers
-            return MLP(input_dims=self.rnn_hidden_size, output_dim=out, hidden_sizes=[cfg.dense_units] * n,
+            return MLP(input_dims=rnn_output_dim, output_dim=out, hidden_sizes=[cfg.dense_units] * n,
                        activation=_act(cfg.dense_act), flatten_dim=None,
                        norm_layer=[nn.LayerNorm] * n if cfg.layer_norm else None,
                        norm_args=[{"normalized_shape": cfg.dense_units} for _ in range(n)] if cfg.layer_norm else None)

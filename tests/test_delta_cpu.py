@@ -287,3 +287,23 @@ def test_rows_behind_a_length_need_no_eps(T):
     torch.testing.assert_close(last.double(), el, rtol=tol, atol=tol * 8)
     for g in torch.autograd.grad(out.sum() + last.sum(), list(x.values())):
         assert torch.isfinite(g).all()
+
+
+@pytest.mark.parametrize("cell", ["lstm", "gated_delta"])
+@pytest.mark.parametrize("apply", [True, False])
+def test_the_policys_heads_are_as_wide_as_the_recurrent_models_output(cell, apply):
+    from sheeprl_prey_amd.algos.ppo_recurrent.agent import RecurrentPPOAgent
+    from sheeprl_prey_amd.config.compose import compose
+    from sheeprl_prey_amd.envs import spaces
+    from sheeprl_prey_amd.utils.utils import dotdict
+
+    cfg = dotdict(compose(["exp=ppo_recurrent", "env=gym", f"algo.rnn.cell={cell}", "algo.rnn.lstm.hidden_size=24", "algo.rnn.gated_delta.hidden_size=16",
+                           f"algo.rnn.post_rnn_mlp.apply={apply}", "algo.rnn.post_rnn_mlp.dense_units=20"]))
+    obs_space = spaces.Dict({"state": spaces.Box(-1, 1, (5,), "float32")})
+    agent = RecurrentPPOAgent([3], obs_space, cfg.algo.encoder, cfg.algo.rnn, cfg.algo.actor, cfg.algo.critic, [], ["state"], False,
+                              cfg.distribution, 2)
+    assert agent.rnn.output_dim == (20 if apply else agent.rnn_hidden_size) and agent.rnn_hidden_size == (24 if cell == "lstm" else 16)
+    actions, logp, _, values, states = agent({"state": torch.randn(4, 2, 5)}, torch.zeros(4, 2, 3), agent.initial_states)
+    assert actions[0].shape == (4, 2, 3) and logp.shape == values.shape == (4, 2, 1) and len(states) == len(agent.rnn.state_keys)
+    (values.sum() + logp.sum()).backward()
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in agent.parameters())
