@@ -104,12 +104,13 @@ Tensor delta_first(const OptT& x, c10::IntArrayRef s, const Tensor& like) {
   return f.scalar_type() == torch::kBool || f.scalar_type() == torch::kUInt8 ? f : f.ne(0);
 }
 
-Tensor delta_lengths(const OptT& x, int64_t B, const Tensor& like) {
+Tensor delta_lengths(const OptT& x, int64_t B, int64_t T, const Tensor& like) {
   if (!has(x)) return Tensor();
   TORCH_CHECK_VALUE(x->dim() == 1 && x->size(0) == B && (x->scalar_type() == torch::kInt32 || x->scalar_type() == torch::kInt64),
                     "lengths must be int32 or int64 [", B, "], got ", x->scalar_type(), " ", x->sizes());
   on(*x, like);
-  return x->to(torch::kInt32).contiguous();
+  // the kernels clamp to 0..T; 64 bits are clamped before they are cut to 32, which would turn a length of 2^31 into a negative one
+  return x->scalar_type() == torch::kInt32 ? x->contiguous() : x->clamp(0, T).to(torch::kInt32).contiguous();
 }
 
 struct DeltaOpts {
@@ -337,7 +338,7 @@ std::pair<Tensor, Tensor> gated_delta(Tensor q, Tensor k, Tensor v, Tensor decay
   Tensor state = val(state_);
   delta_check(q, k, v, decay, beta, state, 2);
   const int64_t T = v.size(0), B = v.size(1);
-  const Tensor first = delta_first(first_, {T, B}, v), lengths = delta_lengths(lengths_, B, v);
+  const Tensor first = delta_first(first_, {T, B}, v), lengths = delta_lengths(lengths_, B, T, v);
   const DeltaOpts opt{scale.has_value() ? *scale : 1.0 / std::sqrt((double)q.size(3)), eps, normalize};
   q = unit_last(q), k = unit_last(k), v = unit_last(v), decay = f32(decay), beta = f32(beta);
   if (state.defined()) state = state.contiguous();

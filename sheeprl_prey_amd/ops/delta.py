@@ -64,14 +64,14 @@ def _flags(x: Optional[Tensor], shape, name: str, device) -> Optional[Tensor]:
     return x if x.dtype in (torch.bool, torch.uint8) else x != 0
 
 
-def _lengths(x: Optional[Tensor], B: int, device) -> Optional[Tensor]:
+def _lengths(x: Optional[Tensor], B: int, T: int, device) -> Optional[Tensor]:
     if x is None:
         return None
     if tuple(x.shape) != (B,) or x.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"lengths must be int32 or int64 [{B}], got {x.dtype} {tuple(x.shape)}")
     if x.device != device:
         raise ValueError(f"lengths must be on {device}, got {x.device}")
-    return x.to(torch.int32).contiguous()
+    return x.clamp(0, T)
 
 
 def _fused(t: Tensor) -> bool:
@@ -104,7 +104,7 @@ def gated_delta(
     _check(q, k, v, decay, beta, state, ("T", "B"))
     T, B = v.shape[:2]
     first = _flags(is_first, (T, B), "is_first", v.device)
-    lens = _lengths(lengths, B, v.device)
+    lens = _lengths(lengths, B, T, v.device)
     scale = float(q.shape[-1]) ** -0.5 if scale is None else float(scale)
     return ref.gated_delta(q, k, v, decay, beta, state, first, lens, scale, normalize, eps)
 

@@ -307,3 +307,14 @@ def test_the_policys_heads_are_as_wide_as_the_recurrent_models_output(cell, appl
     assert actions[0].shape == (4, 2, 3) and logp.shape == values.shape == (4, 2, 1) and len(states) == len(agent.rnn.state_keys)
     (values.sum() + logp.sum()).backward()
     assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in agent.parameters())
+
+
+LONG_LENGTHS = [2**31, 2**63 - 1, 2**32 + 2, -(2**32) + 2, -1, 3]  # in 32 bits: negative, -1, 2, 2, -1, 3
+
+
+@pytest.mark.parametrize("T", [5])
+def test_lengths_past_32_bits_are_clamped(T):
+    x = delta_inputs(T, len(LONG_LENGTHS), 1, 2, 4, 4)
+    out, last = ops.gated_delta(**x, lengths=torch.tensor(LONG_LENGTHS))
+    want, el = ops.gated_delta(**x, lengths=torch.tensor([T, T, T, 0, 0, 3], dtype=torch.int32))
+    assert torch.equal(out, want) and torch.equal(last, el)

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from sheeprl_prey_amd import ops
-from tests.test_delta_cpu import delta_inputs, delta_oracle
+from tests.test_delta_cpu import LONG_LENGTHS, delta_inputs, delta_oracle
 from tests.test_delta_gpu import NAMES, close, oracle_train, run_train, tag
 
 pytestmark = pytest.mark.gpu
@@ -50,3 +50,15 @@ def test_no_eps_with_chunks_that_are_not_full(T, dtype):
     want, el = delta_oracle(**{n: t.cpu() for n, t in x.items()}, eps=0.0, lengths=lengths.cpu())
     close(out, want, tag("out", out))
     close(last, el, "last fp32")
+
+
+@pytest.mark.parametrize("T", [4, 5, 70, 530])
+def test_lengths_past_32_bits_are_clamped(T):
+    x = delta_inputs(T, len(LONG_LENGTHS), 1, 2, 32, 32, torch.float32, T, "cuda")
+    long, short = (torch.tensor(n).cuda() for n in (LONG_LENGTHS, [T, T, T, 0, 0, 3]))
+    w, z = gradients_of(x)
+    a, b = run_train(x, w, z, lengths=long), run_train(x, w, z, lengths=short.int())
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and all(torch.equal(a[2][n], b[2][n]) for n in NAMES)
+    with torch.no_grad():
+        a, b = ops.gated_delta(**x, lengths=long), ops.gated_delta(**x, lengths=short.int())
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
