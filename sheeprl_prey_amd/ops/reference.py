@@ -242,8 +242,10 @@ def gated_delta(q: Tensor, k: Tensor, v: Tensor, decay: Tensor, beta: Tensor, st
         u = bf[t][..., None] * (vf[t] - (kf[t].unsqueeze(-2) @ S).squeeze(-2))
         S = S + kf[t].unsqueeze(-1) * u.unsqueeze(-2)
         out.append(scale * (qf[t].unsqueeze(-2) @ S).squeeze(-2))
-    o = torch.stack(out).to(v.dtype) if out else torch.zeros_like(v)
-    return o, S if T or state is None else S.clone()
+    o = torch.stack(out) if out else torch.zeros_like(v)
+    if lengths is not None:  # nor is the gradient of an output behind the end
+        o = torch.where(wide, o, 0.0)
+    return o.to(v.dtype), S if T or state is None else S.clone()
 
 
 def gated_residual_norm(x: Tensor, h: Tensor, gate: Optional[Tensor], scale, post_weight: Optional[Tensor], post_bias: Optional[Tensor],

@@ -318,3 +318,20 @@ def test_lengths_past_32_bits_are_clamped(T):
     out, last = ops.gated_delta(**x, lengths=torch.tensor(LONG_LENGTHS))
     want, el = ops.gated_delta(**x, lengths=torch.tensor([T, T, T, 0, 0, 3], dtype=torch.int32))
     assert torch.equal(out, want) and torch.equal(last, el)
+
+
+def test_what_lies_behind_a_length_is_not_read():
+    x = delta_inputs(7, 2, 1, 2, 8, 6)
+    lengths = torch.tensor([4, 7])
+    d_out, d_last = torch.randn_like(x["v"]), torch.randn_like(x["state"])
+
+    def run():
+        leaves = {n: t.clone().requires_grad_() for n, t in x.items()}
+        out = ops.gated_delta(**leaves, lengths=lengths)
+        return (*out, *torch.autograd.grad(out, list(leaves.values()), (d_out, d_last)))
+
+    want = run()
+    for t in (d_out, *(x[n] for n in ("q", "k", "v", "decay", "beta"))):
+        t[4:, 0] = float("nan")
+    for a, b in zip(run(), want):
+        assert torch.equal(a, b)
