@@ -233,12 +233,15 @@ def gated_delta(q: Tensor, k: Tensor, v: Tensor, decay: Tensor, beta: Tensor, st
         qf, kf = (torch.where(wide, t, 0.0) for t in (qf, kf))
     qf, kf = (t.repeat_interleave(Hv // Hk, 2) for t in (qf, kf))
     S = torch.zeros(B, Hv, Dk, Dv, device=v.device, dtype=ct) if state is None else state
+    first = None if is_first is None else is_first.bool()
+    if first is not None:
+        gf = torch.where(first[..., None], 0.0, gf)
     keep = gf.exp()[..., None, None]
     out = []
     for t in range(T):
+        if first is not None:  # before the decay: neither the state nor the decay there is read, by the gradients either
+            S = torch.where(first[t][:, None, None, None], 0.0, S)
         S = keep[t] * S
-        if is_first is not None:
-            S = torch.where(is_first[t].bool()[:, None, None, None], 0.0, S)
         u = bf[t][..., None] * (vf[t] - (kf[t].unsqueeze(-2) @ S).squeeze(-2))
         S = S + kf[t].unsqueeze(-1) * u.unsqueeze(-2)
         out.append(scale * (qf[t].unsqueeze(-2) @ S).squeeze(-2))

@@ -335,3 +335,20 @@ def test_what_lies_behind_a_length_is_not_read():
         t[4:, 0] = float("nan")
     for a, b in zip(run(), want):
         assert torch.equal(a, b)
+
+
+def test_a_reset_reads_neither_the_state_nor_the_decay():
+    x = delta_inputs(6, 2, 1, 2, 8, 6)
+    first = torch.zeros(6, 2, dtype=torch.bool)
+    first[0, 0] = first[3, 1] = True
+
+    def run():
+        leaves = {n: t.clone().requires_grad_() for n, t in x.items()}
+        out = ops.gated_delta(**leaves, is_first=first)
+        return (*out, *torch.autograd.grad(out, list(leaves.values()), [torch.ones_like(t) for t in out]))
+
+    want = run()
+    x["state"][0] = float("nan")
+    x["decay"][0, 0] = x["decay"][3, 1] = float("nan")
+    for a, b in zip(run(), want):
+        assert torch.equal(a, b)

@@ -62,3 +62,20 @@ def test_lengths_past_32_bits_are_clamped(T):
     with torch.no_grad():
         a, b = ops.gated_delta(**x, lengths=long), ops.gated_delta(**x, lengths=short.int())
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("T", [4, 16, 70, 530])
+def test_a_reset_reads_neither_the_state_nor_the_decay(T):
+    x = delta_inputs(T, 2, 1, 2, 32, 24, torch.float32, T, "cuda")
+    first = torch.zeros(T, 2, dtype=torch.bool, device="cuda")
+    first[0, 0] = first[T - 2, 1] = True
+    w, z = gradients_of(x)
+    a = run_train(x, w, z, is_first=first)
+    with torch.no_grad():
+        few = ops.gated_delta(**x, is_first=first)
+    x["state"][0] = float("nan")
+    x["decay"][0, 0] = x["decay"][T - 2, 1] = float("nan")
+    b = run_train(x, w, z, is_first=first)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and all(torch.equal(a[2][n], b[2][n]) for n in NAMES)
+    with torch.no_grad():
+        assert all(torch.equal(p, q) for p, q in zip(few, ops.gated_delta(**x, is_first=first)))
