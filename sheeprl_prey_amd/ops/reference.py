@@ -237,14 +237,19 @@ def gated_delta(q: Tensor, k: Tensor, v: Tensor, decay: Tensor, beta: Tensor, st
     if first is not None:
         gf = torch.where(first[..., None], 0.0, gf)
     keep = gf.exp()[..., None, None]
+    amp = torch.is_autocast_enabled(v.device.type)
+
+    def read(x, S):  # S^T x; an autocast region would take the matrix product in bf16, and that of its backward pass
+        return (x.unsqueeze(-1) * S).sum(-2) if amp else (x.unsqueeze(-2) @ S).squeeze(-2)
+
     out = []
     for t in range(T):
         if first is not None:  # before the decay: neither the state nor the decay there is read, by the gradients either
             S = torch.where(first[t][:, None, None, None], 0.0, S)
         S = keep[t] * S
-        u = bf[t][..., None] * (vf[t] - (kf[t].unsqueeze(-2) @ S).squeeze(-2))
+        u = bf[t][..., None] * (vf[t] - read(kf[t], S))
         S = S + kf[t].unsqueeze(-1) * u.unsqueeze(-2)
-        out.append(scale * (qf[t].unsqueeze(-2) @ S).squeeze(-2))
+        out.append(scale * read(qf[t], S))
     o = torch.stack(out) if out else torch.zeros_like(v)
     if lengths is not None:  # nor is the gradient of an output behind the end
         o = torch.where(wide, o, 0.0)

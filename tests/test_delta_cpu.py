@@ -352,3 +352,26 @@ def test_a_reset_reads_neither_the_state_nor_the_decay():
     x["decay"][0, 0] = x["decay"][3, 1] = float("nan")
     for a, b in zip(run(), want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_sums_stay_in_fp32_under_autocast(dtype):
+    x = delta_inputs(9, 2, 1, 2, 8, 6, dtype)
+    one = [x[n][0] for n in ("q", "k", "v", "decay", "beta")]
+
+    def run():
+        leaves = {n: t.clone().requires_grad_() for n, t in x.items()}
+        out = ops.gated_delta(**leaves)
+        res = [*out, *torch.autograd.grad(out, list(leaves.values()), [torch.ones_like(t) for t in out])]
+        S = x["state"].clone()
+        return [*res, ops.gated_delta_step(*one, S), S, *ops.gated_residual_norm(x["v"], x["v"] + 1, x["v"] - 1)]
+
+    want = run()
+    with torch.autocast("cpu", torch.bfloat16):
+        got = run()
+    # two fp32 forms, each (T + Dk) roundings of terms at most 8 times the result, then half a step of the type each
+    tol = 2 * (9 + 8) * 8 * 2.0**-24
+    for a, b in zip(got, want):
+        step = 2.0**-7 if b.dtype == torch.bfloat16 else 0.0
+        assert a.dtype == b.dtype
+        torch.testing.assert_close(a.double(), b.double(), rtol=tol + step, atol=tol * 8)
