@@ -81,7 +81,7 @@ void delta_check(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
   TORCH_CHECK_VALUE(Hk >= 1 && Hv >= Hk && Hv % Hk == 0, "the value heads (", Hv, ") must be a multiple of the key heads (", Hk, ")");
   TORCH_CHECK_VALUE(Dk >= 1 && Dk <= srl::delta::MAXD && Dv >= 1 && Dv <= srl::delta::MAXD, "head dimensions must be 1..",
                     srl::delta::MAXD, ", got ", Dk, " and ", Dv);
-  TORCH_CHECK_VALUE((lead == 1 || v.size(0) < (1 << 24)) && B * Hv < (1 << 20), "at most 2^24 steps and 2^20 states, got ", v.sizes());
+  TORCH_CHECK_VALUE((lead == 1 || v.size(0) <= (1 << 24)) && B * Hv <= (1 << 20), "at most 2^24 steps and 2^20 states, got ", v.sizes());
   TORCH_CHECK_VALUE(q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type(), "q, k, v must have one type, got ",
                     q.scalar_type(), ", ", k.scalar_type(), ", ", v.scalar_type());
   TORCH_CHECK_VALUE(two_types(v), "q, k, v must be float32 or bfloat16, got ", v.scalar_type());

@@ -79,3 +79,45 @@ def test_a_reset_reads_neither_the_state_nor_the_decay(T):
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and all(torch.equal(a[2][n], b[2][n]) for n in NAMES)
     with torch.no_grad():
         assert all(torch.equal(p, q) for p, q in zip(few, ops.gated_delta(**x, is_first=first)))
+
+
+@pytest.mark.parametrize("T", [2, 5, 20])
+def test_as_many_states_as_are_allowed(T):
+    """2^20 states: the last ones come out as they do by themselves; one more is refused."""
+    B = 2**20
+    x = delta_inputs(T, 3, 1, 1, 2, 3, torch.float32, T, "cuda")
+    big = {n: t.new_zeros(*t.shape[:int(n != "state")], B, *t.shape[1 + int(n != "state"):]) for n, t in x.items()}
+    for n, t in x.items():
+        (big[n] if n == "state" else big[n].transpose(0, 1))[-3:] = t if n == "state" else t.transpose(0, 1)
+    with torch.no_grad():
+        (a, la), (b, lb) = ops.gated_delta(**big), ops.gated_delta(**x)
+        assert torch.equal(a[:, -3:], b) and torch.equal(la[-3:], lb) and not a[:, :-3].any() and not la[:-3].any()
+        with pytest.raises(ValueError, match="2\\^20 states"):
+            ops.gated_delta(**{n: torch.cat((t, t[:1] if n == "state" else t[:, :1]), int(n != "state")) for n, t in big.items()})
+    w, z = gradients_of(x)
+    want = run_train(x, w, z)[2]
+    bw, bz = torch.zeros_like(big["v"]), torch.zeros_like(big["state"])
+    bw[:, -3:], bz[-3:] = w, z
+    got = run_train(big, bw, bz)[2]
+    for n in NAMES:
+        assert torch.equal(got[n][-3:] if n == "state" else got[n][:, -3:], want[n]), n
+
+
+def test_as_many_steps_as_are_allowed():
+    """2^24 steps of one head as they are in two halves; one more is refused."""
+    T = 2**24
+    x = delta_inputs(1, 1, 1, 1, 4, 4, torch.float32, 1, "cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v = (torch.randn(T, 1, 1, 4, generator=g, device="cuda") for _ in range(3))
+    decay = -torch.rand(T, 1, 1, generator=g, device="cuda")
+    beta = torch.rand(T, 1, 1, generator=g, device="cuda")
+    with torch.no_grad():
+        out, last = ops.gated_delta(q, k, v, decay, beta, x["state"])
+        h = T // 2
+        a, mid = ops.gated_delta(*(t[:h] for t in (q, k, v, decay, beta)), x["state"])
+        b, end = ops.gated_delta(*(t[h:] for t in (q, k, v, decay, beta)), mid)
+        close(out[:h], a, "out fp32")
+        close(out[h:], b, "out fp32")
+        close(last, end, "last fp32")
+        with pytest.raises(ValueError, match="2\\^24 steps"):
+            ops.gated_delta(*(torch.cat((t, t[:1])) for t in (q, k, v, decay, beta)), x["state"])
