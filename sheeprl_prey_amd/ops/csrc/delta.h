@@ -13,7 +13,6 @@
 // taken in the order k = 16 m + 4 (l/16) + j, j = 0..3, for which the A operand is one 16-byte read of a row:
 // products chain from registers to registers, and only K, Q, A and P, which all strips share, go through LDS.
 #pragma once
-#include <atomic>
 #include <type_traits>
 
 #include "common.h"
@@ -687,16 +686,11 @@ __device__ __forceinline__ f4 mm_tiles(FA&& tile, FB&& operand, f4 c) {
   }
 }
 
-// More than 64 KB of LDS has to be asked for, once for each kernel and device.
+// See AskedLds.
 template <auto F>
 static void allow_lds(int bytes) {
-  static std::atomic<uint64_t> done{0};
-  int dev = 0;
-  (void)hipGetDevice(&dev);
-  const uint64_t bit = 1ull << (dev & 63);
-  if (done.load(std::memory_order_relaxed) & bit) return;
-  (void)hipFuncSetAttribute(reinterpret_cast<const void*>(F), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  done.fetch_or(bit, std::memory_order_relaxed);
+  static AskedLds asked;
+  asked.allow(reinterpret_cast<const void*>(F), bytes);
 }
 
 // LDS bytes of the strip kernels

@@ -3,12 +3,27 @@
 #include <hip/hip_runtime_api.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace srl {
 namespace delta {
 
 constexpr int MAXD = 128;        // head dimensions
 inline __host__ __device__ int pitch(int Dv) { return Dv <= 64 ? 64 : 128; }  // of a row of value columns in the workspaces: Dvp below
 constexpr float GONE = -104.0f;  // exp(g) rounds to zero in fp32 below this: the step forgets all that was before it
+
+// More than 64 KB of LDS has to be asked for, once for each kernel and device.  A request that fails is made again by the next
+// call; the launch after it reports the error.
+struct AskedLds {
+  std::atomic<uint64_t> done{0};
+  void allow(const void* kernel, int bytes) {
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return;
+    if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  }
+};
 
 struct Args {
   const void *q, *k, *v;

@@ -375,3 +375,39 @@ def test_sums_stay_in_fp32_under_autocast(dtype):
         step = 2.0**-7 if b.dtype == torch.bfloat16 else 0.0
         assert a.dtype == b.dtype
         torch.testing.assert_close(a.double(), b.double(), rtol=tol + step, atol=tol * 8)
+
+
+def test_a_failed_request_for_lds_is_made_again(tmp_path):
+    """The host code that asks for a kernel's LDS, with the two runtime calls that it makes replaced: the first request fails."""
+    import os
+    import shutil
+    import subprocess
+
+    cxx = shutil.which("g++")
+    rocm = os.environ.get("ROCM_HOME", "/opt/rocm")
+    if not cxx or not os.path.isdir(os.path.join(rocm, "include", "hip")):
+        pytest.skip("needs g++ and the HIP headers")
+    src = tmp_path / "lds.cpp"
+    src.write_text("""
+#include "delta_args.h"
+static int device = 0, asked = 0;
+static hipError_t answer = hipErrorInvalidValue;
+extern "C" hipError_t hipGetDevice(int* d) { *d = device; return hipSuccess; }
+extern "C" hipError_t hipFuncSetAttribute(const void*, hipFuncAttribute, int) { ++asked; return answer; }
+int main() {
+  srl::delta::AskedLds l;
+  l.allow(nullptr, 1 << 16);
+  answer = hipSuccess;
+  l.allow(nullptr, 1 << 16);
+  if (asked != 2) return 1;
+  l.allow(nullptr, 1 << 16);
+  if (asked != 2) return 2;
+  device = 3;
+  l.allow(nullptr, 1 << 16);
+  return asked == 3 ? 0 : 3;
+}
+""")
+    csrc = os.path.join(os.path.dirname(ops.__file__), "csrc")
+    exe = str(tmp_path / "lds")
+    subprocess.check_call([cxx, "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I", csrc, "-I", os.path.join(rocm, "include"), str(src), "-o", exe])
+    assert subprocess.call([exe]) == 0
