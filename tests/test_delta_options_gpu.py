@@ -121,3 +121,144 @@ def test_as_many_steps_as_are_allowed():
         close(last, end, "last fp32")
         with pytest.raises(ValueError, match="2\\^24 steps"):
             ops.gated_delta(*(torch.cat((t, t[:1])) for t in (q, k, v, decay, beta)), x["state"])
+
+
+def unscaled(x):
+    """Keys and queries of a length near one, taken as they are: the rule without the scaling is stable below a length of sqrt(2)."""
+    D = x["k"].shape[-1]
+    return {**x, "q": (x["q"].float() * D**-0.5).to(x["q"].dtype), "k": (0.7 * x["k"].float() * D**-0.5).to(x["k"].dtype)}
+
+
+OPTIONS = pytest.mark.parametrize("kw", [dict(normalize=False), dict(scale=0.7), dict(eps=0.3), dict(normalize=False, scale=-1.3)],
+                                  ids=["unscaled", "scale", "eps", "unscaled-scale"])
+SIZES = pytest.mark.parametrize("T,Hk,Hv,Dk,Dv", [(3, 1, 2, 32, 24), (8, 1, 2, 40, 24), (70, 2, 2, 72, 40), (530, 1, 2, 24, 20)])
+
+
+@TYPES
+@OPTIONS
+@SIZES
+def test_options_in_training(T, Hk, Hv, Dk, Dv, kw, dtype):
+    x = delta_inputs(T, 2, Hk, Hv, Dk, Dv, dtype, T, "cuda")
+    check_train(unscaled(x) if "normalize" in kw else x, **kw)
+
+
+@TYPES
+@OPTIONS
+@SIZES
+def test_options_without_a_gradient(T, Hk, Hv, Dk, Dv, kw, dtype):
+    x = delta_inputs(T, 2, Hk, Hv, Dk, Dv, dtype, T, "cuda")
+    x = unscaled(x) if "normalize" in kw else x
+    with torch.no_grad():
+        out, last = ops.gated_delta(**x, **kw)
+        S = x["state"].clone()
+        steps = torch.stack([ops.gated_delta_step(*(x[n][t] for n in NAMES[:5]), S, **kw) for t in range(min(T, 8))])
+    want, el = delta_oracle(**{n: t.cpu() for n, t in x.items()}, **kw)
+    close(out, want, tag("out", out))
+    close(last, el, "last fp32")
+    close(steps, want[:8], tag("out", steps))
+    if T <= 8:
+        close(S, el, "state fp32")
+
+
+@TYPES
+@pytest.mark.parametrize("kw", [dict(normalize=False, scale=0.7), dict(eps=0.3)], ids=["unscaled", "eps"])
+def test_options_with_shared_key_heads_in_turn(kw, dtype):
+    """Wide heads and enough chunks that one workgroup takes the value heads of a key head in turn: two sequences, 32 times over."""
+    T, n = 500, 32
+    x = delta_inputs(T, 2, 1, 2, 72, 20, dtype, T, "cuda")
+    x = unscaled(x) if "normalize" in kw else x
+    w, z = gradients_of(x)
+    want = oracle_train(x, w, z, **kw)
+    terms = {} if "normalize" in kw else projected(x, w, z, **kw)
+
+    def over(t, batch):
+        return torch.cat([t] * n, batch)
+
+    out, last, grads = run_train({k: over(t, int(k != "state")) for k, t in x.items()}, over(w, 1), over(z, 0), **kw)
+    close(out, over(want[0], 1), tag("out", out))
+    close(last, over(want[1], 0), "last fp32")
+    for k in NAMES:
+        close(grads[k], over(want[2][k], int(k != "state")), tag("d_" + k, grads[k]), terms.get(k, 0.0))
+
+
+@TYPES
+@pytest.mark.parametrize("which", [0, 1], ids=["out", "last"])
+@pytest.mark.parametrize("T", [9, 70, 530])
+def test_the_gradient_of_one_output_alone(T, which, dtype):
+    x = delta_inputs(T, 2, 1, 2, 32, 24, dtype, T, "cuda")
+    d = gradients_of(x)
+    leaves = {n: t.clone().requires_grad_() for n, t in x.items()}
+    got = torch.autograd.grad(ops.gated_delta(**leaves)[which], list(leaves.values()), d[which], allow_unused=True)
+    exact = {n: t.double().cpu().requires_grad_() for n, t in x.items()}
+    want = torch.autograd.grad(delta_oracle(**exact)[which], list(exact.values()), d[which].double().cpu(), allow_unused=True)
+    zero = [torch.zeros_like(t) for t in d]
+    terms = projected(x, *(d[i] if i == which else zero[i] for i in range(2)), 1e-6)
+    for n, a, b in zip(NAMES, got, want):
+        if b is None:  # the last state does not see the queries
+            assert not a.any(), n
+        else:
+            close(a, b, tag("d_" + n, a), terms.get(n, 0.0))
+
+
+@TYPES
+@pytest.mark.parametrize("T", [3, 9, 70, 530])
+def test_strides(T, dtype):
+    """Batch first, heads first, a slice of a wider projection, a last stride of 2, one decay for all heads."""
+    B, H, D = 2, 2, 32
+    x = delta_inputs(T, B, H, H, D, D, dtype, T, "cuda")
+    w, z = gradients_of(x)
+    wide = torch.zeros(T, B, H, D + 3, device="cuda", dtype=dtype)
+    wide[..., 1:D + 1] = x["v"]
+    pairs = torch.zeros(T, B, H, D, 2, device="cuda", dtype=dtype)
+    pairs[..., 0] = x["k"]
+    x["decay"] = x["decay"][..., :1].contiguous().expand(T, B, H)
+    y = {"q": x["q"].transpose(0, 1).contiguous().transpose(0, 1), "k": pairs[..., 0], "v": wide[..., 1:D + 1],
+         "decay": x["decay"], "beta": x["beta"].permute(2, 0, 1).contiguous().permute(1, 2, 0),
+         "state": x["state"].transpose(0, 1).contiguous().transpose(0, 1)}
+    dw = torch.zeros(T, B, H, D + 1, device="cuda", dtype=dtype)
+    dw[..., 1:] = w
+    want = oracle_train(x, w, z)
+    terms = projected(x, w, z, 1e-6)
+    leaves = {n: t.requires_grad_() for n, t in y.items()}
+    out, last = ops.gated_delta(**leaves)
+    grads = torch.autograd.grad((out, last), list(leaves.values()), (dw[..., 1:], z.transpose(0, 1).contiguous().transpose(0, 1)))
+    close(out, want[0], tag("out", out))
+    close(last, want[1], "last fp32")
+    for n, g in zip(NAMES, grads):
+        close(g, want[2][n], tag("d_" + n, g), terms.get(n, 0.0))
+    with torch.no_grad():
+        out, last = ops.gated_delta(**y)
+    close(out, want[0], tag("out", out))
+    close(last, want[1], "last fp32")
+
+
+@TYPES
+@pytest.mark.parametrize("name", ["q", "k", "v", "decay", "beta", "state"])
+@pytest.mark.parametrize("T", [3, 9, 70, 530])
+def test_a_value_that_is_not_finite_stays_in_its_sequence_and_key_head(T, name, dtype):
+    x = delta_inputs(T, 2, 2, 4, 16, 16, dtype, T, "cuda")
+    w, z = gradients_of(x)
+    a = run_train(x, w, z)
+    with torch.no_grad():
+        c = ops.gated_delta(**x)
+    if name == "state":
+        x["state"][1, 1, 3, 3] = float("nan")
+    else:
+        x[name][T // 2, 1, 0] = float("nan")
+    b = run_train(x, w, z)
+    with torch.no_grad():
+        d = ops.gated_delta(**x)
+
+    def equal(s, t, axis):  # heads of key head 1, and all of sequence 0
+        half = s.shape[axis + 1] // 2
+        for u in range(2):
+            p, q = s.select(axis, u), t.select(axis, u)
+            if u == 1:
+                p, q = p.narrow(axis, half, p.shape[axis] - half), q.narrow(axis, half, q.shape[axis] - half)
+            if not torch.equal(p, q):
+                return False
+        return True
+
+    assert equal(a[0], b[0], 1) and equal(a[1], b[1], 0) and equal(c[0], d[0], 1) and equal(c[1], d[1], 0)
+    for n in NAMES:
+        assert equal(a[2][n], b[2][n], int(n != "state")), n
