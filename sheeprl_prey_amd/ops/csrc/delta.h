@@ -220,18 +220,16 @@ __device__ __forceinline__ void lower_tile(int t, int& ti, int& tj) {
   tj = t - ti * (ti + 1) / 2;
 }
 
-// A = tril(diag(beta) (M o K K^T), -1) and, with Q, P = scale M o Q K^T, lower tiles only, one tile a wave at a time.
-template <int DKT, int C>
-__device__ __forceinline__ void pair_tiles(const float* K, const float* Q, float* A, float* P, const Gates<C>& s, float scale,
+// A chunk of 16: A = tril(diag(beta) (M o K K^T), -1) and P = scale M o Q K^T, a wave each where there are two.
+constexpr int LT = 20;  // a row of a 16 x 16 tile in LDS
+template <int DKT>
+__device__ __forceinline__ void pair_tiles(const float* K, const float* Q, float* A, float* P, const Gates<16>& s, float scale,
                                            int wave, int nw) {
-  constexpr int LD = 16 * DKT + 4, LC = C + 4, NT = C / 16, NTL = NT * (NT + 1) / 2;
+  constexpr int LD = 16 * DKT + 4;
   const int l16 = threadIdx.x & 15, kq = (threadIdx.x >> 4) & 3;
-  const int n = Q ? 2 * NTL : NTL;
-  for (int task = wave; task < n; task += nw) {
-    int ti, tj;
-    lower_tile(task < NTL ? task : task - NTL, ti, tj);
-    const float* kj = K + (16 * tj + l16) * LD + 4 * kq;
-    const float* xi = (task < NTL ? K : Q) + (16 * ti + l16) * LD + 4 * kq;
+  for (int task = wave; task < 2; task += nw) {
+    const float* kj = K + l16 * LD + 4 * kq;
+    const float* xi = (task == 0 ? K : Q) + l16 * LD + 4 * kq;
     f4 d = {0.f, 0.f, 0.f, 0.f}, d2 = d;
 #pragma unroll
     for (int m = 0; m < DKT; m += 2) {
@@ -239,35 +237,31 @@ __device__ __forceinline__ void pair_tiles(const float* K, const float* Q, float
       d2 = mm16(row4(kj + 16 * m + 16), row4(xi + 16 * m + 16), d2);
     }
     d += d2;
-    const int i = 16 * ti + l16, j0 = 16 * tj + 4 * kq;
+    const int i = l16, j0 = 4 * kq;
     const double Gi = s.G[i];
     const int segi = s.seg[i];
     const float be = s.beta[i];
     f4 o;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const float m = pair_decay<C>(s, i, j0 + r, Gi, segi);
-      o[r] = task < NTL ? (j0 + r < i ? be * m * d[r] : 0.f) : scale * m * d[r];
+      const float m = pair_decay<16>(s, i, j0 + r, Gi, segi);
+      o[r] = task == 0 ? (j0 + r < i ? be * m * d[r] : 0.f) : scale * m * d[r];
     }
-    *reinterpret_cast<f4*>((task < NTL ? A : P) + i * LC + j0) = o;
+    *reinterpret_cast<f4*>((task == 0 ? A : P) + i * LT + j0) = o;
   }
 }
 
-// One wave: the inverses of the 16 x 16 diagonal blocks of I + A, a column a lane, by forward substitution.
-constexpr int LT = 20;
-template <int C>
+// One wave: the inverse of I + A for a chunk of 16, a column a lane, by forward substitution.
 __device__ __forceinline__ void diag_inverse(const float* A, float* Td) {
-  constexpr int LC = C + 4, NT = C / 16;
-  const int c = threadIdx.x & 15, q = (threadIdx.x >> 4) & 3;
-  if (q >= NT) return;
-  const float* a = A + 16 * q * (LC + 1);
+  const int c = threadIdx.x & 63;
+  if (c >= 16) return;
   float x[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     float s = i == c ? 1.f : 0.f;
 #pragma unroll
     for (int m4 = 0; m4 < i; m4 += 4) {
-      const f4 r = row4(a + i * LC + m4);
+      const f4 r = row4(A + i * LT + m4);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (m4 + j < i) s = fmaf(-r[j], x[m4 + j], s);
@@ -275,7 +269,7 @@ __device__ __forceinline__ void diag_inverse(const float* A, float* Td) {
     x[i] = s;
   }
 #pragma unroll
-  for (int i = 0; i < 16; ++i) Td[(16 * q + i) * LT + c] = x[i];
+  for (int i = 0; i < 16; ++i) Td[i * LT + c] = x[i];
 }
 
 // A barrier for what goes through LDS: __syncthreads() would also wait for every store to memory on its way.
@@ -693,10 +687,10 @@ static void allow_lds(int bytes) {
   asked.allow(reinterpret_cast<const void*>(F), bytes);
 }
 
-// LDS bytes of the strip kernels
-template <int DKT, int C>
-constexpr size_t strip_lds(bool q) {
-  return sizeof(float) * ((q ? 2 : 1) * C * (16 * DKT + 4) + (q ? 2 : 1) * C * (C + 4) + C * LT) + sizeof(Gates<C>);
+// LDS bytes of the kernels of a chunk of 16: the gates; K and Q; A, P and the inverse
+template <int DKT>
+constexpr size_t strip_lds() {
+  return sizeof(Gates<16>) + sizeof(float) * (2 * 16 * (16 * DKT + 4) + 3 * 16 * LT);
 }
 
 }  // namespace delta

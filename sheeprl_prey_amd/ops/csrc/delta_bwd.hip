@@ -26,14 +26,14 @@ namespace delta {
 
 template <typename T, int DKT>
 __global__ void __launch_bounds__(512) delta_bwd_short_kernel(Args a, BwdArgs o) {
-  constexpr int C = 16, LD = 16 * DKT + 4, LC = C + 4, DKp = 16 * DKT;
+  constexpr int C = 16, LD = 16 * DKT + 4, DKp = 16 * DKT;
   extern __shared__ __align__(16) unsigned char lds[];
   Gates<C>& s = *reinterpret_cast<Gates<C>*>(lds);
   float* K = reinterpret_cast<float*>(lds + sizeof(Gates<C>));
   float* Q = K + C * LD;
   float* A = Q + C * LD;
-  float* P = A + C * LC;
-  float* Td = P + C * LC;
+  float* P = A + C * LT;
+  float* Td = P + C * LT;
 
   const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4, wave = wave_id(), nw = blockDim.x >> 6;
   const int BH = a.B * a.Hv, bh = blockIdx.x, b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
@@ -59,15 +59,15 @@ __global__ void __launch_bounds__(512) delta_bwd_short_kernel(Args a, BwdArgs o)
     }
   lds_barrier();
   const f4 dy = dc.get(0, 0, len, kq, gp && dv < a.Dv);
-  pair_tiles<DKT, C>(K, Q, A, P, s, a.scale, wave, nw);
+  pair_tiles<DKT>(K, Q, A, P, s, a.scale, wave, nw);
   f4 u = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int m = 0; m < DKT; ++m) u = mm16(row4(K + l16 * LD + 16 * m + 4 * kq), S[m], u);
   lds_barrier();
-  if (wave == 0) diag_inverse<C>(A, Td);
+  if (wave == 0) diag_inverse(A, Td);
   lds_barrier();
   const f4 be = row4(s.beta + 4 * kq), ga = row4(s.gam + 4 * kq);
-  u = mm16(col4(P + 4 * kq * LC + l16, LC), dy, u * row4(s.e + 4 * kq));
+  u = mm16(col4(P + 4 * kq * LT + l16, LT), dy, u * row4(s.e + 4 * kq));
   u = mm16(col4(Td + 4 * kq * LT + l16, LT), u, f4{0.f, 0.f, 0.f, 0.f});
   T* vp = reinterpret_cast<T*>(o.dv) + (long)bh * a.Dv + dv;
 #pragma unroll
@@ -260,74 +260,68 @@ __device__ __forceinline__ float segment_suffix(const Gates<C>& s, double dG, in
   return (float)(suf - (later ? beyond : 0.0));
 }
 
-// Chunks of 16 (whole sequences): what sums over the value columns, one wave per 16 key columns.
-template <int DKT, int C>
+// A chunk of 16 (a whole sequence): what sums over the value columns, one wave per 16 key columns.
+template <int DKT>
 struct PairLds {
-  static constexpr int LD = 16 * DKT + 4, LC = C + 4, LV = DVB + 4, NT = C / 16, NTL = NT * (NT + 1) / 2;
-  static constexpr int stage = 3 * C * LV, w = 2 * C * LC, big = stage > w ? stage : w;
-  float K[C * LD], Q[C * LD], big_[big];
-  Gates<C> s;
-  float rows[2 * NTL][16], cols[2 * NTL][16], rowb[NTL][16], dots[5][DKT][C], dRv[C], sd[DKT];
+  static constexpr int LD = 16 * DKT + 4, LV = DVB + 4, stage = 3 * 16 * LV, w = 2 * 16 * LT, big = stage > w ? stage : w;
+  float K[16 * LD], Q[16 * LD], big_[big];
+  Gates<16> s;
+  float rows[2][16], cols[2][16], rowb[16], dots[5][DKT][16], dRv[16], sd[DKT];
 };
 
-template <typename T, int DKT, int C>
+template <typename T, int DKT>
 __global__ void __launch_bounds__(64 * DKT) delta_bwd_pair_kernel(Args a, BwdArgs o, int per_value_head) {
-  using L = PairLds<DKT, C>;
-  constexpr int LD = L::LD, LC = L::LC, LV = L::LV, NT = L::NT, NTL = L::NTL, DKp = 16 * DKT, NW = DKT;
-  constexpr int TPW = (2 * NTL + NW - 1) / NW, RPT = (C * (DVB / 4) + 64 * NW - 1) / (64 * NW);
+  using L = PairLds<DKT>;
+  constexpr int C = 16, LD = L::LD, LV = L::LV, DKp = 16 * DKT, NW = DKT;
+  constexpr int RPT = (C * (DVB / 4) + 64 * NW - 1) / (64 * NW);
   extern __shared__ __align__(16) unsigned char lds[];
   L& l = *reinterpret_cast<L*>(lds);
   Gates<C>& s = l.s;
-  float *sO = l.big_, *sR = sO + C * LV, *sU = sR + C * LV, *W1 = l.big_, *W2 = W1 + C * LC;
+  float *sO = l.big_, *sR = sO + C * LV, *sU = sR + C * LV, *W1 = l.big_, *W2 = W1 + C * LT;
 
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, kq = lane >> 4, wave = wave_id();
-  const int BH = a.B * a.Hv, bh = blockIdx.x % BH, n = blockIdx.x / BH, t0 = n * C;
+  const int BH = a.B * a.Hv, bh = blockIdx.x;
   const int b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
   const int Dvp = pitch(a.Dv), Dve = 16 * ((a.Dv + 15) >> 4);
   const int len = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
   const int Ho = per_value_head ? a.Hv : a.Hk, ho = per_value_head ? h : hk;
   const bool same = per_value_head == 0;  // the outputs have the inputs' type
 
-  auto put = [&](void* base, int i, int d, float v) {
-    const long at = (((long)(t0 + i) * a.B + b) * Ho + ho) * a.Dk + d;
+  auto put = [&](void* base, int t, int d, float v) {
+    const long at = (((long)t * a.B + b) * Ho + ho) * a.Dk + d;
     if (same) st1(reinterpret_cast<T*>(base) + at, v);
     else reinterpret_cast<float*>(base)[at] = v;
   };
 
-  if (t0 >= len) {
-    const int m = min(C, a.T - t0);
-    for (int x = tid; x < m * a.Dk; x += 64 * NW) {
+  if (len == 0) {
+    for (int x = tid; x < a.T * a.Dk; x += 64 * NW) {
       put(o.dq, x / a.Dk, x % a.Dk, 0.f);
       put(o.dk, x / a.Dk, x % a.Dk, 0.f);
     }
-    if (tid < m) {
-      o.dg[(long)(t0 + tid) * BH + bh] = 0.f;
-      o.db[(long)(t0 + tid) * BH + bh] = 0.f;
+    if (tid < a.T) {
+      o.dg[(long)tid * BH + bh] = 0.f;
+      o.db[(long)tid * BH + bh] = 0.f;
     }
     return;
   }
 
   constexpr int RL = C * 16 / (64 * NW) > 0 ? C * 16 / (64 * NW) : 1;
-  load_rows<T, DKT, C, RL>(l.K, s.rk, reinterpret_cast<const T*>(a.k) + (long)b * a.kb + (long)hk * a.kh, a.kt, a.Dk, t0, len, a.veck,
+  load_rows<T, DKT, C, RL>(l.K, s.rk, reinterpret_cast<const T*>(a.k) + (long)b * a.kb + (long)hk * a.kh, a.kt, a.Dk, 0, len, a.veck,
                        a.normalize, a.eps);
-  load_rows<T, DKT, C, RL>(l.Q, s.rq, reinterpret_cast<const T*>(a.q) + (long)b * a.qb + (long)hk * a.qh, a.qt, a.Dk, t0, len, a.vecq,
+  load_rows<T, DKT, C, RL>(l.Q, s.rq, reinterpret_cast<const T*>(a.q) + (long)b * a.qb + (long)hk * a.qh, a.qt, a.Dk, 0, len, a.vecq,
                        a.normalize, a.eps);
-  if (wave == 0) chunk_gates<C>(a, s, b, h, t0, len, lane);
+  if (wave == 0) chunk_gates<C>(a, s, b, h, 0, len, lane);
 
   const T* vp = reinterpret_cast<const T*>(a.v) + (long)b * a.vb + (long)h * a.vh;
   const T* gp = o.dout ? reinterpret_cast<const T*>(o.dout) + (long)b * o.ob + (long)h * o.oh : nullptr;
-  const float* up = o.U + ((long)bh * a.N + n) * C * Dvp;
-  const float* rp = o.dR + ((long)bh * a.N + n) * C * Dvp;
-  const float* s0 = o.Sc + (((long)bh * a.N + n) * DKp + 16 * wave + l16) * Dvp;
-  const float* ds = o.dSc + (((long)bh * a.N + n) * DKp + 16 * wave + l16) * Dvp;
+  const float* up = o.U + (long)bh * C * Dvp;
+  const float* rp = o.dR + (long)bh * C * Dvp;
+  const float* s0 = o.Sc + ((long)bh * DKp + 16 * wave + l16) * Dvp;
+  const float* ds = o.dSc + ((long)bh * DKp + 16 * wave + l16) * Dvp;
 
-  f4 GO[NT], GR[NT], GU[NT], D[TPW];
-  float dRv[RPT], sdot = 0.f;
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int ti = 0; ti < NT; ++ti) GO[ti] = GR[ti] = GU[ti] = zero;
-#pragma unroll
-  for (int x = 0; x < TPW; ++x) D[x] = zero;
+  f4 GO = zero, GR = zero, GU = zero, D = zero;
+  float dRv[RPT], sdot = 0.f;
 #pragma unroll
   for (int x = 0; x < RPT; ++x) dRv[x] = 0.f;
 
@@ -340,13 +334,12 @@ __global__ void __launch_bounds__(64 * DKT) delta_bwd_pair_kernel(Args a, BwdArg
         if (c < Dve) {
           r = row4(rp + i * Dvp + c);
           u = row4(up + i * Dvp + c);
-          const int t = t0 + i;
-          if (t < len) {
+          if (i < len) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
               if (c + j < a.Dv) {
-                if (gp) g[j] = ld1(gp + (long)t * o.ot + c + j);
-                dRv[x] = fmaf(r[j], ld1(vp + (long)t * a.vt + c + j), dRv[x]);
+                if (gp) g[j] = ld1(gp + (long)i * o.ot + c + j);
+                dRv[x] = fmaf(r[j], ld1(vp + (long)i * a.vt + c + j), dRv[x]);
               }
           }
         }
@@ -364,23 +357,11 @@ __global__ void __launch_bounds__(64 * DKT) delta_bwd_pair_kernel(Args a, BwdArg
         const f4 x = row4(s0 + c + 4 * kq), y = row4(ds + c + 4 * kq);
 #pragma unroll
         for (int j = 0; j < 4; ++j) sdot = fmaf(x[j], y[j], sdot);
-#pragma unroll
-        for (int ti = 0; ti < NT; ++ti) {
-          const int w = (16 * ti + l16) * LV + 16 * m + 4 * kq;
-          GO[ti] = mm16(x, row4(sO + w), GO[ti]);
-          GR[ti] = mm16(x, row4(sR + w), GR[ti]);
-          GU[ti] = mm16(y, row4(sU + w), GU[ti]);
-        }
-#pragma unroll
-        for (int x2 = 0; x2 < TPW; ++x2) {
-          const int task = wave + x2 * NW;
-          if (task < 2 * NTL) {
-            int ti, tj;
-            lower_tile(task < NTL ? task : task - NTL, ti, tj);
-            D[x2] = mm16(row4(sU + (16 * tj + l16) * LV + 16 * m + 4 * kq),
-                         row4((task < NTL ? sO : sR) + (16 * ti + l16) * LV + 16 * m + 4 * kq), D[x2]);
-          }
-        }
+        const int w = l16 * LV + 16 * m + 4 * kq;
+        GO = mm16(x, row4(sO + w), GO);
+        GR = mm16(x, row4(sR + w), GR);
+        GU = mm16(y, row4(sU + w), GU);
+        if (wave < 2) D = mm16(row4(sU + w), row4((wave == 0 ? sO : sR) + w), D);
       }
     }
     __syncthreads();
@@ -394,164 +375,130 @@ __global__ void __launch_bounds__(64 * DKT) delta_bwd_pair_kernel(Args a, BwdArg
   sdot = wave_sum(sdot);
   if (lane == 0) l.sd[wave] = sdot;
 
-  // W1, W2 (over the staging area) and the row and column sums of what the decays see of them
+  // W1 (wave 0) and W2 (wave 1), over the staging area, and the row and column sums of what the decays see of them
+  if (wave < 2) {
+    const bool first = wave == 0;
+    const float* kj = l.K + l16 * LD + 4 * kq;
+    const float* xi = (first ? l.Q : l.K) + l16 * LD + 4 * kq;
+    f4 d = zero;
 #pragma unroll
-  for (int x2 = 0; x2 < TPW; ++x2) {
-    const int task = wave + x2 * NW;
-    if (task < 2 * NTL) {
-      const bool first = task < NTL;
-      int ti, tj;
-      lower_tile(first ? task : task - NTL, ti, tj);
-      const float* kj = l.K + (16 * tj + l16) * LD + 4 * kq;
-      const float* xi = (first ? l.Q : l.K) + (16 * ti + l16) * LD + 4 * kq;
-      f4 d = zero;
+    for (int m = 0; m < DKT; ++m) d = mm16(row4(kj + 16 * m), row4(xi + 16 * m), d);
+    const int i = l16, j0 = 4 * kq;
+    const double Gi = s.G[i];
+    const int segi = s.seg[i];
+    const float be = s.beta[i];
+    f4 w;
+    float rs = 0.f, rb = 0.f;
 #pragma unroll
-      for (int m = 0; m < DKT; ++m) d = mm16(row4(kj + 16 * m), row4(xi + 16 * m), d);
-      const int i = 16 * ti + l16, j0 = 16 * tj + 4 * kq;
-      const double Gi = s.G[i];
-      const int segi = s.seg[i];
-      const float be = s.beta[i];
-      f4 w;
-      float rs = 0.f, rb = 0.f;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float m = pair_decay<C>(s, i, j0 + r, Gi, segi);
-        float e;
-        if (first) {
-          w[r] = m * D[x2][r];
-          e = a.scale * w[r] * d[r];
-        } else {
-          const float z = j0 + r < i ? -m * D[x2][r] : 0.f;
-          w[r] = be * z;
-          rb = fmaf(z, d[r], rb);
-          e = w[r] * d[r];
-        }
-        rs += e;
-        const float cs = row16_sum(e);
-        if (l16 == 0) l.cols[task][4 * kq + r] = cs;
+    for (int r = 0; r < 4; ++r) {
+      const float m = pair_decay<C>(s, i, j0 + r, Gi, segi);
+      float e;
+      if (first) {
+        w[r] = m * D[r];
+        e = a.scale * w[r] * d[r];
+      } else {
+        const float z = j0 + r < i ? -m * D[r] : 0.f;
+        w[r] = be * z;
+        rb = fmaf(z, d[r], rb);
+        e = w[r] * d[r];
       }
-      *reinterpret_cast<f4*>((first ? W1 : W2) + i * LC + j0) = w;
-      rs += __shfl_xor(rs, 16, 64);
-      rs += __shfl_xor(rs, 32, 64);
-      rb += __shfl_xor(rb, 16, 64);
-      rb += __shfl_xor(rb, 32, 64);
-      if (kq == 0) {
-        l.rows[task][l16] = rs;
-        if (!first) l.rowb[task - NTL][l16] = rb;
-      }
+      rs += e;
+      const float cs = row16_sum(e);
+      if (l16 == 0) l.cols[wave][4 * kq + r] = cs;
+    }
+    *reinterpret_cast<f4*>((first ? W1 : W2) + i * LT + j0) = w;
+    rs += __shfl_xor(rs, 16, 64);
+    rs += __shfl_xor(rs, 32, 64);
+    rb += __shfl_xor(rb, 16, 64);
+    rb += __shfl_xor(rb, 32, 64);
+    if (kq == 0) {
+      l.rows[wave][l16] = rs;
+      if (!first) l.rowb[l16] = rb;
     }
   }
   __syncthreads();
 
   // this wave's 16 key columns of dQ^T and dK^T
-  f4 dQ[NT], dK[NT];
-  const int kc = 16 * wave;
+  const int kc = 16 * wave, i = l16;
+  const f4 q = row4(l.Q + i * LD + kc + 4 * kq), k = row4(l.K + i * LD + kc + 4 * kq);
+  float dd[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int ti = 0; ti < NT; ++ti) {
-    const int i = 16 * ti + l16;
-    const float ga = s.gam[i], be = s.beta[i], e = s.e[i];
-    const f4 q = row4(l.Q + i * LD + kc + 4 * kq), k = row4(l.K + i * LD + kc + 4 * kq);
-    float d0 = 0.f, d1 = 0.f, d2 = 0.f;
+  for (int r = 0; r < 4; ++r) {
+    dd[0] = fmaf(q[r], GO[r], dd[0]);
+    dd[1] = fmaf(k[r], GR[r], dd[1]);
+    dd[2] = fmaf(k[r], GU[r], dd[2]);
+  }
+  const float ga = s.gam[i], be = s.beta[i], e = s.e[i];
+  const f4 kcol = col4(l.K + 4 * kq * LD + kc + l16, LD), qcol = col4(l.Q + 4 * kq * LD + kc + l16, LD);
+  f4 dQ = mm16(kcol, row4(W1 + i * LT + 4 * kq), ga * GO);
+  f4 w = mm16(kcol, row4(W2 + i * LT + 4 * kq), zero);
+  const f4 z = mm16(qcol, col4(W1 + 4 * kq * LT + i, LT), zero);
+  w = mm16(kcol, col4(W2 + 4 * kq * LT + i, LT), w);
+  dQ *= a.scale;
+  f4 dK = w + a.scale * z - (be * ga) * GR + e * GU;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      d0 = fmaf(q[r], GO[ti][r], d0);
-      d1 = fmaf(k[r], GR[ti][r], d1);
-      d2 = fmaf(k[r], GU[ti][r], d2);
-    }
-    dQ[ti] = ga * GO[ti];
-    f4 w = zero;
+  for (int r = 0; r < 4; ++r) {
+    dd[3] = fmaf(q[r], dQ[r], dd[3]);
+    dd[4] = fmaf(k[r], dK[r], dd[4]);
+  }
 #pragma unroll
-    for (int tj = 0; tj <= ti; ++tj) {
-      const f4 x = col4(l.K + (16 * tj + 4 * kq) * LD + kc + l16, LD);
-      dQ[ti] = mm16(x, row4(W1 + i * LC + 16 * tj + 4 * kq), dQ[ti]);
-      w = mm16(x, row4(W2 + i * LC + 16 * tj + 4 * kq), w);
-    }
-    f4 z = zero;
-#pragma unroll
-    for (int tr = ti; tr < NT; ++tr) {
-      z = mm16(col4(l.Q + (16 * tr + 4 * kq) * LD + kc + l16, LD), col4(W1 + (16 * tr + 4 * kq) * LC + i, LC), z);
-      w = mm16(col4(l.K + (16 * tr + 4 * kq) * LD + kc + l16, LD), col4(W2 + (16 * tr + 4 * kq) * LC + i, LC), w);
-    }
-    dQ[ti] *= a.scale;
-    dK[ti] = w + a.scale * z - (be * ga) * GR[ti] + e * GU[ti];
-    float d3 = 0.f, d4 = 0.f;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      d3 = fmaf(q[r], dQ[ti][r], d3);
-      d4 = fmaf(k[r], dK[ti][r], d4);
-    }
-    float dd[5] = {d0, d1, d2, d3, d4};
-#pragma unroll
-    for (int x = 0; x < 5; ++x) {
-      dd[x] += __shfl_xor(dd[x], 16, 64);
-      dd[x] += __shfl_xor(dd[x], 32, 64);
-      if (kq == 0) l.dots[x][wave][i] = dd[x];
-    }
+  for (int x = 0; x < 5; ++x) {
+    dd[x] += __shfl_xor(dd[x], 16, 64);
+    dd[x] += __shfl_xor(dd[x], 32, 64);
+    if (kq == 0) l.dots[x][wave][i] = dd[x];
   }
   __syncthreads();
-#pragma unroll
-  for (int ti = 0; ti < NT; ++ti) {
-    const int i = 16 * ti + l16;
+  if (a.normalize) {
     float dq = 0.f, dk = 0.f;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      dq += l.dots[3][w][i];
-      dk += l.dots[4][w][i];
+    for (int x = 0; x < NW; ++x) {
+      dq += l.dots[3][x][i];
+      dk += l.dots[4][x][i];
     }
-    const f4 q = row4(l.Q + i * LD + kc + 4 * kq), k = row4(l.K + i * LD + kc + 4 * kq);
-    if (a.normalize) {
-      dQ[ti] = s.rq[i] * (dQ[ti] - dq * q);
-      dK[ti] = s.rk[i] * (dK[ti] - dk * k);
-    }
-    if (t0 + i < a.T) {
+    dQ = s.rq[i] * (dQ - dq * q);
+    dK = s.rk[i] * (dK - dk * k);
+  }
+  if (i < a.T) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int d = kc + 4 * kq + r;
-        if (d < a.Dk) {
-          put(o.dq, i, d, t0 + i < len ? dQ[ti][r] : 0.f);
-          put(o.dk, i, d, t0 + i < len ? dK[ti][r] : 0.f);
-        }
+    for (int r = 0; r < 4; ++r) {
+      const int d = kc + 4 * kq + r;
+      if (d < a.Dk) {
+        put(o.dq, i, d, i < len ? dQ[r] : 0.f);
+        put(o.dk, i, d, i < len ? dK[r] : 0.f);
       }
     }
   }
   if (wave == 0) {
-    const int i = lane;
     double dG = 0.0;
     float F = 0.f, db = 0.f;
-    if (i < C) {
+    if (lane < C) {
       float go = 0.f, gr = 0.f, gu = 0.f;
 #pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        go += l.dots[0][w][i];
-        gr += l.dots[1][w][i];
-        gu += l.dots[2][w][i];
+      for (int x = 0; x < NW; ++x) {
+        go += l.dots[0][x][i];
+        gr += l.dots[1][x][i];
+        gu += l.dots[2][x][i];
       }
-      const float ga = s.gam[i], be = s.beta[i];
-      F = s.e[i] * gu;
+      F = e * gu;
       db = l.dRv[i] - ga * gr;
       dG = (double)(a.scale * ga * go) - (double)(be * ga * gr) - (double)F;
-#pragma unroll
-      for (int task = 0; task < 2 * NTL; ++task) {
-        int ti, tj;
-        lower_tile(task < NTL ? task : task - NTL, ti, tj);
-        if (ti == i >> 4) {
-          dG += (double)l.rows[task][i & 15];
-          if (task >= NTL) db += l.rowb[task - NTL][i & 15];
-        }
-        if (tj == i >> 4) dG -= (double)l.cols[task][i & 15];
-      }
+      dG += (double)l.rows[0][i];
+      dG -= (double)l.cols[0][i];
+      dG += (double)l.rows[1][i];
+      db += l.rowb[i];
+      dG -= (double)l.cols[1][i];
     }
-    float sumF = wave_sum(F);
-    if (i == C - 1) {
+    const float sumF = wave_sum(F);
+    if (lane == C - 1) {
       float sd = 0.f;
 #pragma unroll
-      for (int w = 0; w < NW; ++w) sd += l.sd[w];
-      dG += (double)(sumF + s.gam[C - 1] * sd);
+      for (int x = 0; x < NW; ++x) sd += l.sd[x];
+      dG += (double)(sumF + ga * sd);
     }
-    const float g = segment_suffix<C>(s, dG, i);
-    if (i < C && t0 + i < a.T) {
-      o.dg[(long)(t0 + i) * BH + bh] = s.rst[i] ? 0.f : g;
-      o.db[(long)(t0 + i) * BH + bh] = t0 + i < len ? db : 0.f;
+    const float g = segment_suffix<C>(s, dG, lane);
+    if (lane < a.T) {
+      o.dg[(long)lane * BH + bh] = s.rst[lane] ? 0.f : g;
+      o.db[(long)lane * BH + bh] = lane < len ? db : 0.f;
     }
   }
 }
@@ -1073,10 +1020,10 @@ template <typename T, int DKT, int C>
 static void launch_c(const Args& a, const BwdArgs& o, bool per_value_head, hipStream_t st) {
   const int nvs = (a.Dv + 15) / 16, BH = a.B * a.Hv;
   if constexpr (C == 16) {
-    delta_bwd_short_kernel<T, DKT><<<BH, 64 * nvs, strip_lds<DKT, 16>(true), st>>>(a, o);
-    const int lds = (int)sizeof(PairLds<DKT, C>);
-    allow_lds<delta_bwd_pair_kernel<T, DKT, C>>(lds);
-    delta_bwd_pair_kernel<T, DKT, C><<<BH, 64 * DKT, lds, st>>>(a, o, per_value_head ? 1 : 0);
+    delta_bwd_short_kernel<T, DKT><<<BH, 64 * nvs, strip_lds<DKT>(), st>>>(a, o);
+    const int lds = (int)sizeof(PairLds<DKT>);
+    allow_lds<delta_bwd_pair_kernel<T, DKT>>(lds);
+    delta_bwd_pair_kernel<T, DKT><<<BH, 64 * DKT, lds, st>>>(a, o, per_value_head ? 1 : 0);
   } else {
     if (a.nseg > 1) {
       if (nvs <= 4) launch_walk<T, DKT, 4, true>(a, o, st);

@@ -22,14 +22,14 @@ namespace delta {
 
 template <typename T, int DKT>
 __global__ void __launch_bounds__(512) delta_short_kernel(Args a, FwdOut o) {
-  constexpr int C = 16, LD = 16 * DKT + 4, LC = C + 4, DKp = 16 * DKT;
+  constexpr int C = 16, LD = 16 * DKT + 4, DKp = 16 * DKT;
   extern __shared__ __align__(16) unsigned char lds[];
   Gates<C>& s = *reinterpret_cast<Gates<C>*>(lds);
   float* K = reinterpret_cast<float*>(lds + sizeof(Gates<C>));
   float* Q = K + C * LD;
   float* A = Q + C * LD;
-  float* P = A + C * LC;
-  float* Td = P + C * LC;
+  float* P = A + C * LT;
+  float* Td = P + C * LT;
 
   const int lane = threadIdx.x & 63, l16 = lane & 15, kq = lane >> 4, wave = wave_id(), nw = blockDim.x >> 6;
   const int BH = a.B * a.Hv, bh = blockIdx.x, b = bh / a.Hv, h = bh % a.Hv, hk = h / (a.Hv / a.Hk);
@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(512) delta_short_kernel(Args a, FwdOut o) {
     }
   lds_barrier();
   const f4 v = vc.get(0, 0, len, kq, dv < a.Dv);
-  pair_tiles<DKT, C>(K, Q, A, P, s, a.scale, wave, nw);
+  pair_tiles<DKT>(K, Q, A, P, s, a.scale, wave, nw);
   f4 u = {0.f, 0.f, 0.f, 0.f}, y = u;
 #pragma unroll
   for (int m = 0; m < DKT; ++m) {
@@ -65,11 +65,11 @@ __global__ void __launch_bounds__(512) delta_short_kernel(Args a, FwdOut o) {
     y = mm16(row4(Q + l16 * LD + 16 * m + 4 * kq), S[m], y);
   }
   lds_barrier();
-  if (wave == 0) diag_inverse<C>(A, Td);
+  if (wave == 0) diag_inverse(A, Td);
   lds_barrier();
   const f4 ga = row4(s.gam + 4 * kq);
   u = mm16(row4(Td + l16 * LT + 4 * kq), row4(s.beta + 4 * kq) * (v - ga * u), f4{0.f, 0.f, 0.f, 0.f});
-  y = mm16(row4(P + l16 * LC + 4 * kq), u, y * (a.scale * ga));
+  y = mm16(row4(P + l16 * LT + 4 * kq), u, y * (a.scale * ga));
   T* op = reinterpret_cast<T*>(o.out) + (long)bh * a.Dv + dv;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
@@ -494,7 +494,7 @@ template <typename T, int DKT>
 static void launch_dk(const Args& a, const FwdOut& o, int C, hipStream_t st) {
   const int nvs = (a.Dv + 15) / 16, BH = a.B * a.Hv;
   if (C == 16) {
-    const int lds = (int)strip_lds<DKT, 16>(true);
+    const int lds = (int)strip_lds<DKT>();
     delta_short_kernel<T, DKT><<<BH, 64 * nvs, lds, st>>>(a, o);
     return;
   }
