@@ -355,6 +355,38 @@ std::pair<Tensor, Tensor> gated_delta(Tensor q, Tensor k, Tensor v, Tensor decay
   return delta_forward(q, k, v, decay, beta, state, first, lengths, opt, nullptr);
 }
 
+// Whether an operand shares memory with one of the states, outer and inner their leading axes by stride.  Where either has gaps
+// (a slice of a larger store), every run of the operand is looked up among the states, which lie one behind the other.
+bool lies_in(const Tensor& t, const Tensor& state, int64_t outer, int64_t inner) {
+  const auto o = at::get_overlap_status(state, t);
+  if (o != at::MemOverlapStatus::TooHard) return o != at::MemOverlapStatus::No;
+  if (!t.is_alias_of(state)) return false;
+  const int64_t e = state.element_size(), n1 = state.size(outer), n2 = state.size(inner), s1 = state.stride(outer) * e, s2 = state.stride(inner) * e,
+                one = state.size(2) * state.size(3) * e;
+  const char* base = static_cast<const char*>(state.const_data_ptr());
+  auto hit = [&](const char* p, int64_t n) {  // the last state that begins before the end of the n bytes: does it reach into them?
+    const int64_t r = p - base, z = r + n - 1;
+    if (z < 0) return false;
+    const int64_t i = n1 > 1 ? std::min(z / s1, n1 - 1) : 0, rest = z - i * (n1 > 1 ? s1 : 0), j = n2 > 1 ? std::min(rest / s2, n2 - 1) : 0;
+    return i * (n1 > 1 ? s1 : 0) + j * (n2 > 1 ? s2 : 0) + one > r;
+  };
+  const int64_t te = t.element_size(), nd = t.dim(), last = t.size(-1);
+  const bool runs = last == 1 || t.stride(-1) == 1;
+  std::vector<int64_t> at(nd, 0);
+  const char* p = static_cast<const char*>(t.const_data_ptr());
+  while (true) {
+    if (hit(p, runs ? last * te : te)) return true;
+    int64_t d = runs ? nd - 2 : nd - 1;  // the next run, or element
+    for (; d >= 0; --d) {
+      p += t.stride(d) * te;
+      if (++at[d] < t.size(d)) break;
+      p -= at[d] * t.stride(d) * te;
+      at[d] = 0;
+    }
+    if (d < 0) return false;
+  }
+}
+
 Tensor gated_delta_step(Tensor q, Tensor k, Tensor v, Tensor decay, Tensor beta, Tensor state, OptT first_, c10::optional<double> scale,
                         bool normalize, double eps) {
   delta_check(q, k, v, decay, beta, state, 1);
@@ -375,10 +407,8 @@ Tensor gated_delta_step(Tensor q, Tensor k, Tensor v, Tensor decay, Tensor beta,
     TORCH_CHECK_VALUE(state.stride(d) >= least, "the states must not overlap, got strides ", state.strides());
     least = state.stride(d) * state.size(d);
   }
-  for (auto* t : {&q, &k, &v, &decay, &beta}) {
-    const auto o = at::get_overlap_status(state, *t);
-    TORCH_CHECK_VALUE(o != at::MemOverlapStatus::Full && o != at::MemOverlapStatus::Partial, "no operand may lie in the state that is updated");
-  }
+  for (const Tensor* t : std::initializer_list<const Tensor*>{&q, &k, &v, &decay, &beta, &first})
+    TORCH_CHECK_VALUE(!t->defined() || !lies_in(*t, state, d0, d1), "no operand may lie in the state that is updated");
   const DeltaOpts opt{scale.has_value() ? *scale : 1.0 / std::sqrt((double)Dk), eps, normalize};
   if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
   return delta_steps(unit_last(q), unit_last(k), unit_last(v), f32(decay), f32(beta), state, first, Tensor(), opt, state, 1);

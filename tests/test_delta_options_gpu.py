@@ -262,3 +262,32 @@ def test_a_value_that_is_not_finite_stays_in_its_sequence_and_key_head(T, name, 
     assert equal(a[0], b[0], 1) and equal(a[1], b[1], 0) and equal(c[0], d[0], 1) and equal(c[1], d[1], 0)
     for n in NAMES:
         assert equal(a[2][n], b[2][n], int(n != "state")), n
+
+
+def test_an_operand_in_a_slice_of_a_store_of_states_is_refused():
+    """States with gaps between them: what lies in the gaps is an operand like any other, what lies in a state is refused."""
+    B, Hv, D = 4, 2, 8
+    row = Hv * D * D
+    flat = torch.randn(B, row + 5 * Hv * D, device="cuda")
+    S, gap = flat[:, :row].view(B, Hv, D, D), flat[:, row:].view(B, 5, Hv, D)
+    gates = torch.rand(2, B, Hv, device="cuda")
+    q, k, v = (gap[:, i] for i in range(3))
+    copies, T = [t.clone() for t in (q, k, v, -gates[0], gates[1])], S.clone()
+    want = ops.gated_delta_step(*copies, T)
+    rest = flat[:, row:].clone()
+    assert torch.equal(ops.gated_delta_step(q, k, v, -gates[0], gates[1], S), want) and torch.equal(S, T) and torch.equal(flat[:, row:], rest)
+    before = flat.clone()
+    decay, beta = -gates[0], gates[1]
+    flags = flat.view(torch.uint8)
+    for bad in (dict(q=S[:, :, 0]), dict(k=S[:, :, :, 3]), dict(v=flat[:, row - 1:row - 1 + Hv * D].view(B, Hv, D)),
+                dict(beta=S[:, :, D - 1, D - 1]), dict(decay=flat[3:, row - 1:row + Hv - 1].expand(B, Hv)), dict(is_first=flags[:, 7])):
+        with pytest.raises(ValueError, match="in the state"):
+            ops.gated_delta_step(**{**dict(q=q, k=k, v=v, decay=decay, beta=beta, state=S), **bad})
+    heads = flat[:, :row].view(B, Hv, D, D)[:, :1]  # the other head's state is free
+    one = dict(q=q[:, :1], k=k[:, :1], v=S[:, 1:, 0], decay=decay[:, :1], beta=beta[:, :1], state=heads)
+    T = heads.clone()
+    want = ops.gated_delta_step(**{**one, "v": one["v"].clone(), "state": T})
+    with pytest.raises(ValueError, match="in the state"):
+        ops.gated_delta_step(**{**one, "v": S[:, :1, 0]})
+    assert torch.equal(flat, before)
+    assert torch.equal(ops.gated_delta_step(**one), want) and torch.equal(heads, T)
