@@ -390,8 +390,8 @@ __device__ __forceinline__ void each(F&& f) {
 // A chunk of 64 steps on its way from memory to LDS for the strip kernels: K (and Q) as they lie in memory, the pair tiles,
 // the gates.  fetch() starts the reads for the next chunk, commit() writes what has arrived to LDS: the reads have the whole
 // walk over the present chunk to arrive in, and are issued in three parts (K; Q; tiles and gates) between its products: all at
-// once they queue up, and the waves with them, for 2000 to 5000 of a chunk's 16000 to 23000 cycles.  MODE: 0 forward, 1 forward without Q and P (maps), 2 backward,
-// 3 without the tiles (gradients of q and k).
+// once they queue up, and the waves with them, for 2000 to 5000 of a chunk's 17000 to 24000 cycles.  MODE: 0 forward,
+// 1 forward without Q and P (maps), 2 backward, 3 without the tiles (gradients of q and k).
 // What the kernels read: k(ti, m2), q(ti, m2): rows of steps against 32 key columns; kt(m, t2), qt(m, t2): rows of key columns
 // against 32 steps; A (negated), P, Ti: tiles, transposed in the backward mode; rk4, rq4: factors that are not in k and q yet.
 constexpr int TS = 320, TL = 20;  // a fp32 tile in LDS: 16 rows of 20: reads of rows and of columns are free of bank conflicts

@@ -152,7 +152,7 @@ srl::delta::Args delta_args(const Tensor& q, const Tensor& k, const Tensor& v, c
 
 int dkp(int Dk) { return Dk <= 32 ? 32 : Dk <= 64 ? 64 : 128; }
 
-// Chunks of 64 steps, or one of 16 where the whole sequence fits (16 steps x 128 x 2 heads of 32, forward and backward: 31 us
+// Chunks of 64 steps, or one of 16 where the whole sequence fits (16 steps x 128 x 2 heads of 32, forward and backward: 30 us
 // and 58 us as a chunk of 64; x 16 x 16 of 128: 73 and 89).  An axis of 8 chunks or more is split into segments while the
 // heads alone leave two thirds of the 256 CUs idle; the segments' maps cost as much as the walk itself.  Forward over 1024
 // steps with and without segments: 48 heads of 128 133 and 177 us, 64 heads 157 and 181, 80 heads 189 and 190, 96 heads (two
@@ -328,9 +328,11 @@ Tensor delta_steps(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   return out;
 }
 
-// Up to this many steps without a gradient the recurrent kernel is taken, whose time goes with the steps.  Against a chunk of
-// 16, in a graph: 4 steps x 64 x 16 heads of 128 57 and 58 us, 8 steps 86 and 58; x 16 x 16 heads 25 and 27, 6 steps 32
-// and 27; 4 steps x 64 x 8 heads of 64 17 and 18, 8 steps 24 and 18.
+// Up to this many steps without a gradient the recurrent kernel is taken, whose time goes with the steps.  Against a chunk of 16,
+// in a graph over four states in turn: 64 x 16 heads of 128 in fp32 4 steps 39 and 46 us, 6 steps 47 and 47, 8 steps 55 and 47,
+// in bf16 2 steps 39 and 46, 3 steps 48 and 46, 4 steps 59 and 46; 64 x 8 heads of 64 in fp32 3 steps 12.4 and 13.3, 4 steps
+// 14.1 and 13.4; 256 x 2 heads of 32 in fp32 4 steps 8.7 and 9.7, 6 steps 11.1 and 9.7.  The forms cross at 4 to 6 steps in fp32
+// and at 3 in bf16.
 constexpr int RECURRENT_MAX_STEPS = 4;
 
 std::pair<Tensor, Tensor> gated_delta(Tensor q, Tensor k, Tensor v, Tensor decay, Tensor beta, OptT state_, OptT first_, OptT lengths_,
@@ -524,7 +526,7 @@ std::pair<Tensor, Tensor> gated_residual_norm(Tensor x, Tensor h, OptT gate_, Op
   const int64_t D = x.size(-1);
   TORCH_CHECK_VALUE(D >= 1 && D <= srl::rnorm::MAXD, "the last axis must be 1..", srl::rnorm::MAXD, " wide, got ", D);
   TORCH_CHECK_VALUE(two_types(x), "x must be float32 or bfloat16, got ", x.scalar_type());
-  TORCH_CHECK_VALUE(x.numel() / D < (1ll << 31) - 64, "at most 2^31 rows, got ", x.sizes());
+  TORCH_CHECK_VALUE(x.numel() / D < (1ll << 31) - 64, "fewer than 2^31 - 64 rows, got ", x.sizes());
   auto operand = [&](const Tensor& t) {
     TORCH_CHECK_VALUE(t.device() == x.device() && t.is_floating_point(), "every operand must be floating point on ", x.device(), ", got ",
                       t.scalar_type(), " on ", t.device());

@@ -15,8 +15,8 @@
 // F_i = e_i k_i . GU_i, dG of the chunk's last step takes sum F + gam_C <S0, dS> too, and the gradient of g_i is the
 // sum of dG over the steps from i to the end of its segment.
 //
-// Measured at 4096 steps x 2 x 16 heads of 128 in bf16, us: maps 94, joins 24, walk 106 (bound as the forward walk is),
-// gradients of q and k 264.  The last reads the states and their gradients at every chunk, 192 KB a chunk and head of which
+// Measured at 4096 steps x 2 x 16 heads of 128 in bf16, us in a kernel trace: maps 99, joins 24, walk 111 (bound as the forward
+// walk is), gradients of q and k 273.  The last reads the states and their gradients at every chunk, 192 KB a chunk and head of which
 // a third of its time is, and has one workgroup on a CU; the rest is products on operands cut into three parts, whose reads
 // from LDS take as long as the matrix instructions.
 #include "delta.h"

@@ -9,12 +9,13 @@
 // every segment walks again from its first state and writes the outputs.
 //
 // Sequences of at most 16 steps are one chunk of 16: delta_short_kernel does all of it at once (8 steps x 128 x 2 heads of 32
-// in 10 us: latency, of its reads, the substitution and the joins of the waves).
+// in 9 us: latency, of its reads, the substitution and the joins of the waves).
 //
-// Measured at 4096 steps x 2 x 16 heads of 128 in bf16 (8 segments a head), us: pairs 38, maps 106, joins
-// 18, walk 110.  The bytes would take 20 us and the products 13: a walk is bound by the chain of one chunk (16000 to 23000
-// cycles: the arrival of operands and their way into LDS 3500, K S and Q S 3500, the substitution, each block of which waits
-// for the one before, 3500, the outputs 3400, the state 1700) with two waves a SIMD to hide its waits.
+// Measured at 4096 steps x 2 x 16 heads of 128 in bf16 (8 segments a head), us in a kernel trace: pairs 38, maps 110, joins
+// 18, walk 112.  The bytes would take 20 us and the products 13: a walk is bound by the chain of one chunk (23500 cycles by the
+// clock, 21500 with 8 heads: operands and the other waves 6000 and 4500, their way into LDS 2000, K S and Q S 4300, the
+// substitution, each block of which waits for the one before, 3900, the outputs 3400 to 3700, the state 1700), with two waves a
+// SIMD to hide its waits.  Q S and the outputs wait for no later chunk and are in the chain all the same.
 #include "delta.h"
 
 namespace srl {
@@ -425,7 +426,7 @@ __global__ void __launch_bounds__(64 * NWT) delta_walk_kernel(Args a, FwdOut o) 
 // Joins the segments: S_{s+1} = Pseg_s S_s + Rseg_s, or backwards (REV) dS_s = Pseg_s^T dS_{s+1} + Xseg_s with the maps
 // transposed.  One workgroup per 16 columns, one wave per 16 rows; the state goes through LDS in three bf16 parts, and the
 // next two maps are on their way meanwhile.  Every strip of a head reads the head's maps, 64 KB each: 32 heads of 128 in 8
-// segments take 18 us (7.5 TB/s out of the L2s), 8 heads in 32 segments 47 us, 1.5 us a join, which is bound by the join's chain.
+// segments take 18 us (7.5 TB/s out of the L2s), 8 heads in 32 segments 48 us, 1.5 us a join, which is bound by the join's chain.
 template <int DKT, bool REV>
 __global__ void __launch_bounds__(64 * DKT) delta_scan_kernel(Args a, const float* dlast, const float* P, const float* R, float* out) {
   constexpr int DKp = 16 * DKT, LD = DKp + 8;

@@ -16,7 +16,7 @@
 // walks; each workgroup leaves one partial sum of every column and residual_norm_sum_kernel adds them in a fixed order,
 // so results repeat bit by bit.
 //
-// Measured: forward, bf16, 8191 x 2048 29 us (5.8 TB/s), 8192 x 4096 61 us (5.5 TB/s; a copy of that size 5.2); backward
+// Measured, in a kernel trace: forward, bf16, 8191 x 2048 29 us (5.8 TB/s), 8192 x 4096 61 us (5.5 TB/s; a copy of that size 5.2); backward
 // 8192 x 4096 129 us (4.2 TB/s: two workgroups of 512 a CU, for the partial sums' sake) and 13 us for the sums; fp32, 16384
 // x 256 16 and 26 us and 6 us.  bf16 rows of 1001 go by elements: 5003 of them 19 and 39 us.  Outputs are stored through the
 // caches: past them the kernel is up to 12 % faster by itself, but what reads y and u next loses more (98 -> 109 us together).

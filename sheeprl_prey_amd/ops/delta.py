@@ -91,7 +91,8 @@ def gated_delta(
     strides (a copy is made only where the last one is not 1); ``decay`` (the logarithm of what a step keeps, <= 0) and
     ``beta`` ``[T, B, Hv]``; ``state`` fp32, zeros if None.  ``is_first [T, B(, 1)]`` marks steps that start from a
     zero state; there ``decay`` has no effect.  ``lengths [B]`` (clamped to 0..T): steps at or after a sequence's length change nothing,
-    give zero outputs and get zero gradients, and are not read.  ``scale`` defaults to ``Dk ** -0.5``.  A value that is
+    give zero outputs and get zero gradients, and are not read.  ``scale`` defaults to ``Dk ** -0.5``; ``eps`` is added to the sum of
+    squares and may be zero where no row that counts is.  A value that is
     not finite in a step that counts spoils the results of its own sequence and key head, before it and after it, and
     nothing else; one in ``state`` those of its sequence and head, unless ``is_first`` marks the first step.
 
